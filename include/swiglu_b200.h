@@ -501,6 +501,106 @@ int sgl_mgpu_fused_swiglu(sgl_mgpu* g, int mode, const void* const* x, const voi
 int sgl_mgpu_size(const sgl_mgpu* g);
 int sgl_mgpu_destroy(sgl_mgpu* g);
 
+/* ---- mixture-of-experts operators ------------------------------------------------------
+ *
+ * A slot is one (token, choice) pair s = t * k + j of a router's answer ids[T, k] (int32 or
+ * int64, row pitch ld_ids elements).  A slot whose id lies outside [0, E) is dropped (padding
+ * tokens carry -1).  k <= 64, E <= 1024, T * k < 2^31.  All of these enqueue only, allocate
+ * nothing and use no atomics: results are fixed bit for bit.  No counterpart in the reference.
+ *
+ * sgl_expert_order: stable counting sort of the slots by expert, one launch.
+ *   offsets[E + 1] int32  offsets[e] = kept slots with an id below e; offsets[E] = kept slots
+ *   slots[T * k]   int32  slot held by row r, -1 at and behind offsets[E]
+ *   rows[T, k]     int32  row of slot (t, j), -1 if dropped (dense)
+ * sgl_expert_dispatch: out[rows[t, j]] = x[t] for every kept slot; out is [R, D] with R >= T * k
+ *   or at least every row named in `rows` (an index outside [0, R) is not followed).  Rows
+ *   behind offsets[E] are left as they were.
+ * sgl_expert_combine: out[t] = sum_j weights[t, j] * in[rows[t, j]], summed in fp32 in the order
+ *   of j.  weights: fp32 or bf16 [T, k], row pitch ld_w, or NULL for ones (which is dispatch's
+ *   gradient).  Dropped slots add nothing; a token without any gets zeros.
+ * sgl_expert_combine_grad: grad_rows[rows[t, j]] = weights[t, j] * grad_out[t] (other rows are left
+ *   as they were) and grad_weights[t, j] = <grad_out[t], in[rows[t, j]]> (fp32 sums, stored in the
+ *   weights' type, dense [T, k]; 0 for dropped slots).  in and grad_weights may both be NULL:
+ *   grad_rows alone.  grad_rows may be `in` itself.
+ * D must be a multiple of 8; the bf16 tensors follow the conventions above.
+ */
+int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, int64_t ld_ids,
+                     int64_t E, void* offsets, void* slots, void* rows, void* stream);
+int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
+                        int64_t R, int64_t ldx, int64_t ldo, void* stream);
+int sgl_expert_combine(const void* in, const void* rows, const void* weights, int weights_bf16,
+                       void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
+                       int64_t ld_w, int64_t ldo, void* stream);
+int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* rows,
+                            const void* weights, int weights_bf16, void* grad_rows,
+                            void* grad_weights, int64_t T, int64_t k, int64_t D, int64_t R,
+                            int64_t ld_go, int64_t ld_in, int64_t ld_w, int64_t ld_gr,
+                            void* stream);
+
+/*
+ * Products over rows grouped by expert: rows [offsets[e], offsets[e + 1]) of the [R, *] tensors
+ * meet expert e's matrix.  offsets[E + 1] is int32 DEVICE memory, non-decreasing, from 0 to at
+ * most R (values outside [0, R] are clamped); groups may be empty.  Rows behind offsets[E] are
+ * neither used nor written.  Expert e's matrix starts e * *_stride elements (a multiple of 8)
+ * behind the first's; all matrices are row-major with the given pitch.
+ *
+ * sgl_grouped_fused_swiglu: h[r] = silu(x[r] @ Wg) * (x[r] @ Wu), w[E, K, 2N] = [W_up | W_gate].
+ * sgl_grouped_fused_swiglu_save: the same h, and the pre-activations [up | gate] for the backward
+ *   pass: bits = 16 in bf16, bits = 8 in e4m3 with a power-of-two scale per row and 32 columns
+ *   (the smallest 2^e, e >= -127, with max|v| <= 448 * 2^e; a block that holds an infinity or
+ *   a NaN reads as NaN).  `pre` takes sgl_preact_bytes() bytes, `scales` *scale_bytes (bits = 8).
+ *   E = 1 with offsets == NULL is the dense stage over all R rows.
+ * sgl_grouped_matmul: c[r] = a[r] @ b_e, or a[r] @ b_e^T with b_e stored [N, K] (b_transposed).
+ * sgl_grouped_weight_grad: c[e] = a_e^T @ g_e, a[R, M], g[R, N], c[E, M, N]; an empty group's
+ *   matrix is zero.  M and N are multiples of 8, the groups' row counts are arbitrary.
+ */
+int sgl_grouped_fused_swiglu(const void* x, const void* w, const void* offsets, void* h, int64_t R,
+                             int64_t N, int64_t K, int64_t E, int64_t ldx, int64_t ldw,
+                             int64_t w_stride, int64_t ldh, void* stream);
+int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offsets, void* h,
+                                  void* pre, void* scales, int bits, int64_t R, int64_t N,
+                                  int64_t K, int64_t E, int64_t ldx, int64_t ldw, int64_t w_stride,
+                                  int64_t ldh, void* stream);
+int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
+                       int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
+                       int64_t ldc, int b_transposed, void* stream);
+int sgl_grouped_weight_grad(const void* a, const void* g, const void* offsets, void* c, int64_t R,
+                            int64_t M, int64_t N, int64_t E, int64_t lda, int64_t ldg, int64_t ldc,
+                            int64_t c_stride, void* stream);
+
+/*
+ * Saved pre-activations of `rows` rows: bytes of the code (or bf16) buffer, its row pitch, and for
+ * bits = 8 bytes and pitch of the scale buffer.  A row holds the up half, padded to whole blocks of
+ * 32 columns, then the gate half; a scale row the exponents + 127 of the up blocks (an even
+ * number of bytes), then of the gate blocks.  Negative sgl_status on bad sizes.
+ */
+int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int64_t* scale_bytes,
+                         int64_t* scale_pitch);
+/*
+ * Backward elementwise step from saved pre-activations: grad_preact[rows, 2N] =
+ * [dy * silu(gate) | dy * up * silu'(gate)] and, unless h is NULL, h = silu(gate) * up.  `end`, if
+ * not NULL, is a device int32 (such as offsets + E): rows at and behind it are not touched.
+ */
+int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* scales, int bits,
+                                 void* grad_preact, void* h, const void* end, int64_t rows,
+                                 int64_t N, int64_t lddy, int64_t ldo, int64_t ldh, void* stream);
+
+/*
+ * The whole expert layer at inference: order, dispatch, gate/up stage, down projection, combine.
+ *   y[t] = sum_j weights[t, j] * (silu(x[t] @ Wg) * (x[t] @ Wu)) @ Wd,  expert ids[t, j]
+ * x[T, D], w[E, D, 2N], w_down[E, N, D_out], y[T, D_out].  `workspace`: caller-owned device memory
+ * of sgl_experts_swiglu_workspace_bytes bytes, overwritten; calls that overlap on the GPU must not
+ * share it.
+ */
+int64_t sgl_experts_swiglu_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N,
+                                           int64_t D_out);
+int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const void* weights,
+                       int weights_bf16, const void* w, const void* w_down, void* y,
+                       void* workspace, int64_t workspace_bytes, int64_t T, int64_t k, int64_t E,
+                       int64_t D, int64_t N, int64_t D_out, int64_t ldx, int64_t ld_ids,
+                       int64_t ld_weights, int64_t ldw, int64_t w_stride, int64_t ldd,
+                       int64_t d_stride, int64_t ldy, void* stream);
+
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char* sgl_last_error(void);
 

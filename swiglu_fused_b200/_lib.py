@@ -75,6 +75,18 @@ EXPORTED_SYMBOLS = (
     "sgl_mgpu_fused_swiglu",
     "sgl_mgpu_size",
     "sgl_mgpu_destroy",
+    "sgl_expert_order",
+    "sgl_expert_dispatch",
+    "sgl_expert_combine",
+    "sgl_expert_combine_grad",
+    "sgl_grouped_fused_swiglu",
+    "sgl_grouped_fused_swiglu_save",
+    "sgl_grouped_matmul",
+    "sgl_grouped_weight_grad",
+    "sgl_preact_bytes",
+    "sgl_swiglu_grad_preact_saved",
+    "sgl_experts_swiglu_workspace_bytes",
+    "sgl_experts_swiglu",
     "sgl_last_error",
     "sgl_version",
 )
@@ -267,6 +279,30 @@ def load() -> C.CDLL:
         lib.sgl_mgpu_size.argtypes = [vp]
         lib.sgl_mgpu_destroy.restype = ip
         lib.sgl_mgpu_destroy.argtypes = [vp]
+        lib.sgl_expert_order.restype = ip
+        lib.sgl_expert_order.argtypes = [vp, ip, i64, i64, i64, i64, vp, vp, vp, vp]
+        lib.sgl_expert_dispatch.restype = ip
+        lib.sgl_expert_dispatch.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]
+        lib.sgl_expert_combine.restype = ip
+        lib.sgl_expert_combine.argtypes = [vp, vp, vp, ip, vp] + [i64] * 7 + [vp]
+        lib.sgl_expert_combine_grad.restype = ip
+        lib.sgl_expert_combine_grad.argtypes = [vp, vp, vp, vp, ip, vp, vp] + [i64] * 8 + [vp]
+        lib.sgl_grouped_fused_swiglu.restype = ip
+        lib.sgl_grouped_fused_swiglu.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [vp]
+        lib.sgl_grouped_fused_swiglu_save.restype = ip
+        lib.sgl_grouped_fused_swiglu_save.argtypes = [vp] * 6 + [ip] + [i64] * 8 + [vp]
+        lib.sgl_grouped_matmul.restype = ip
+        lib.sgl_grouped_matmul.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [ip, vp]
+        lib.sgl_grouped_weight_grad.restype = ip
+        lib.sgl_grouped_weight_grad.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [vp]
+        lib.sgl_preact_bytes.restype = i64
+        lib.sgl_preact_bytes.argtypes = [ip, i64, i64] + [C.POINTER(i64)] * 3
+        lib.sgl_swiglu_grad_preact_saved.restype = ip
+        lib.sgl_swiglu_grad_preact_saved.argtypes = [vp, vp, vp, ip, vp, vp, vp] + [i64] * 5 + [vp]
+        lib.sgl_experts_swiglu_workspace_bytes.restype = i64
+        lib.sgl_experts_swiglu_workspace_bytes.argtypes = [i64] * 6
+        lib.sgl_experts_swiglu.restype = ip
+        lib.sgl_experts_swiglu.argtypes = [vp, vp, ip, vp, ip, vp, vp, vp, vp, i64] + [i64] * 14 + [vp]
         lib.sgl_last_error.restype = C.c_char_p
         lib.sgl_last_error.argtypes = []
         lib.sgl_version.restype = ip

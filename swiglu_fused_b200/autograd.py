@@ -11,6 +11,10 @@ from __future__ import annotations
 
 import torch
 
+from .experts import (ExpertOrder, SavedPreact, _checkpoint_bits, _layer_operands, expert_combine,
+                      expert_combine_grad, expert_dispatch, expert_order, grouped_fused_swiglu_save,
+                      grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
+                      swiglu_grad_preact_saved)
 from .ops import matmul_bf16, matmul_fused_swiglu_save_factors, swiglu_grad_preact
 
 
@@ -41,6 +45,87 @@ class FusedSwiGLUFunction(torch.autograd.Function):
         return grad_x, grad_w
 
 
-def fused_swiglu(x: torch.Tensor, w: torch.Tensor) -> torch.Tensor:
-    """Differentiable ``silu(x @ W_gate) * (x @ W_up)`` with ``w = [W_up | W_gate]``."""
-    return FusedSwiGLUFunction.apply(x, w)
+class FusedSwiGLUPreactFunction(torch.autograd.Function):
+    """The same stage over saved pre-activations (8 bits or bf16) instead of the two factors.  The
+    backward recomputes what it needs from them and leaves them as they are."""
+
+    @staticmethod
+    def forward(ctx, x: torch.Tensor, w: torch.Tensor, checkpoint: str) -> torch.Tensor:
+        h, pre = matmul_fused_swiglu_save_preact(x, w, checkpoint=checkpoint)
+        ctx.save_for_backward(x, w, pre.data, pre.scales)
+        ctx.bits, ctx.hidden = pre.bits, pre.hidden
+        return h
+
+    @staticmethod
+    def backward(ctx, grad_h: torch.Tensor):
+        x, w, data, scales = ctx.saved_tensors
+        pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
+        grad_preact = swiglu_grad_preact_saved(grad_h.contiguous(), pre)
+        if x.shape[0] == 0:
+            return torch.zeros_like(x), torch.zeros_like(w), None
+        grad_x = matmul_bf16(grad_preact, w, transpose_b=True) if ctx.needs_input_grad[0] else None
+        grad_w = matmul_bf16(x, grad_preact, transpose_a=True) if ctx.needs_input_grad[1] else None
+        return grad_x, grad_w, None
+
+
+def fused_swiglu(x: torch.Tensor, w: torch.Tensor, *, checkpoint: str | None = None) -> torch.Tensor:
+    """Differentiable ``silu(x @ W_gate) * (x @ W_up)`` with ``w = [W_up | W_gate]``.
+
+    ``checkpoint`` says what the forward keeps for the backward besides its inputs: ``None`` two
+    bf16 factors (``4N`` bytes per row), ``"bf16"`` the bf16 pre-activations (``4N``), ``"e4m3"`` the
+    pre-activations in 8 bits (``2N + N/16``)."""
+    if checkpoint is None:
+        return FusedSwiGLUFunction.apply(x, w)
+    _checkpoint_bits(checkpoint)
+    return FusedSwiGLUPreactFunction.apply(x, w, checkpoint)
+
+
+class FusedSwiGLUExpertsFunction(torch.autograd.Function):
+    """The expert layer.  Kept for the backward: the inputs, the order, the pre-activations and,
+    if the routing weights need a gradient, the experts' outputs.  The grouped copy of x and h
+    are made again."""
+
+    @staticmethod
+    def forward(ctx, x, expert_ids, weights, w, w_down, checkpoint):
+        order = expert_order(expert_ids, w.shape[0])
+        xs = expert_dispatch(x, order)
+        h, pre = grouped_fused_swiglu_save(xs, w, order.offsets, checkpoint=checkpoint)
+        ys = grouped_matmul(h, w_down, order.offsets)
+        y = expert_combine(ys, order, weights)
+        ctx.save_for_backward(x, weights, w, w_down, *order, pre.data, pre.scales,
+                              ys if ctx.needs_input_grad[2] else None)
+        ctx.bits, ctx.hidden = pre.bits, pre.hidden
+        return y
+
+    @staticmethod
+    def backward(ctx, grad_y: torch.Tensor):
+        x, weights, w, w_down, offsets, slots, rows, data, scales, ys = ctx.saved_tensors
+        need_x, _, need_weights, need_w, need_down, _ = ctx.needs_input_grad
+        if x.shape[0] == 0:
+            return (torch.zeros_like(x), None, torch.zeros_like(weights), torch.zeros_like(w),
+                    torch.zeros_like(w_down), None)
+        order = ExpertOrder(offsets, slots, rows)
+        grad_ys, grad_weights = expert_combine_grad(grad_y.contiguous(), ys, order, weights)
+        grad_x = grad_w = grad_down = None
+        if need_x or need_w or need_down:
+            pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
+            grad_h = grouped_matmul(grad_ys, w_down, offsets, transpose_b=True)
+            grad_preact, h = swiglu_grad_preact_saved(grad_h, pre, offsets=offsets, return_h=True)
+            del grad_h
+            if need_down:
+                grad_down = grouped_weight_grad(h, grad_ys, offsets)
+            del h, grad_ys
+            if need_w:
+                grad_w = grouped_weight_grad(expert_dispatch(x, order), grad_preact, offsets)
+            if need_x:
+                grad_x = expert_combine(grouped_matmul(grad_preact, w, offsets, transpose_b=True),
+                                        order)
+        return grad_x, None, grad_weights if need_weights else None, grad_w, grad_down, None
+
+
+def fused_swiglu_experts(x, expert_ids, weights, w, w_down, *, checkpoint: str = "bf16"):
+    """Differentiable expert layer: ``experts_swiglu`` with gradients for ``x``, ``weights``, ``w``
+    and ``w_down``.  ``checkpoint`` is how the pre-activations are kept: ``"bf16"`` or ``"e4m3"``."""
+    _checkpoint_bits(checkpoint)
+    _layer_operands(x, expert_ids, weights, w, w_down)
+    return FusedSwiGLUExpertsFunction.apply(x, expert_ids, weights, w, w_down, checkpoint)

@@ -20,6 +20,10 @@ SOURCES = [os.path.join(CSRC_DIR, "swiglu_abi.cu")]
 HEADERS = [
     os.path.join(CSRC_DIR, "swiglu_kernel.cuh"),
     os.path.join(CSRC_DIR, "swiglu_elementwise.cuh"),
+    os.path.join(CSRC_DIR, "swiglu_preact.cuh"),
+    os.path.join(CSRC_DIR, "experts_order.cuh"),
+    os.path.join(CSRC_DIR, "experts_products.cuh"),
+    os.path.join(CSRC_DIR, "experts_abi.cuh"),
     os.path.join(CSRC_DIR, "ptx_sm100.cuh"),
     os.path.join(CSRC_DIR, "swiglu_host_pipeline.cuh"),
     os.path.join(CSRC_DIR, "swiglu_mgpu.cuh"),

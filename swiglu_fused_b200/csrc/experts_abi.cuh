@@ -1,0 +1,782 @@
+// C entry points of the mixture-of-experts operators and of the saved pre-activations.
+// Included at the end of swiglu_abi.cu (one translation unit; uses its validation helpers).
+#pragma once
+
+namespace {
+
+using ExpertKernelFn = void (*)(const sgl::ExpertMaps, const sgl::ExpertParams);
+
+struct ExpertVariant {
+  ExpertKernelFn fn;
+  int (*max_stages)(int groups, int a_rows, int acc_cols);
+  int (*smem_bytes)(int groups, int a_rows, int acc_cols, int stages);
+};
+
+template <int F, int G, int BK>
+ExpertVariant make_expert_variant() {
+  using T = sgl::ExpertTraits<F, G, BK>;
+  ExpertVariant v;
+  v.fn = sgl::experts_kernel<F, G, BK>;
+  v.max_stages = T::max_stages;
+  v.smem_bytes = T::smem_bytes;
+  return v;
+}
+
+constexpr int kExpertVariants = 10;   // form * 2 + (cta_group - 1)
+constexpr int kExpertBlockK = 64;
+
+const ExpertVariant& expert_variant(int form, int cta_group) {
+  static const ExpertVariant table[kExpertVariants] = {
+      make_expert_variant<sgl::EXP_SWIGLU, 1, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_SWIGLU, 2, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_SAVE16, 1, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_SAVE16, 2, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_SAVE8, 1, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_SAVE8, 2, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_GEMM, 1, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_GEMM, 2, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_WGRAD, 1, kExpertBlockK>(),
+      make_expert_variant<sgl::EXP_WGRAD, 2, kExpertBlockK>(),
+  };
+  return table[form * 2 + cta_group - 1];
+}
+
+struct ExpertDevice {
+  bool ready[kExpertVariants] = {};
+  int clusters2[kExpertVariants] = {};
+  bool order_ready = false;
+};
+std::map<int, ExpertDevice> g_expert_devices;   // by device ordinal, under g_dev_mutex
+
+int current_device(int* dev) {
+  cudaError_t e = cudaGetDevice(dev);
+  return e == cudaSuccess ? SGL_OK : fail_cuda(e, "cudaGetDevice");
+}
+
+// First use of a variant on a device: its shared-memory limit, and how many CTA pairs fit.
+int prepare_expert_variant(int form, int cta_group, const DeviceInfo* info, int* clusters) {
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(g_dev_mutex);
+  ExpertDevice& d = g_expert_devices[dev];
+  const int vi = form * 2 + cta_group - 1;
+  const ExpertVariant& v = expert_variant(form, cta_group);
+  if (!d.ready[vi]) {
+    cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(v.fn),
+                                         cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(max dynamic smem)");
+    int n = info->sm_count / cta_group;
+    if (cta_group == 2) {
+      cudaLaunchConfig_t qc = {};
+      qc.gridDim = dim3(static_cast<unsigned>(info->sm_count / 2 * 2), 1, 1);
+      qc.blockDim = dim3(sgl::kExpThreads, 1, 1);
+      qc.dynamicSmemBytes = 227 * 1024;
+      cudaLaunchAttribute qa[1];
+      qa[0].id = cudaLaunchAttributeClusterDimension;
+      qa[0].val.clusterDim.x = 2;
+      qa[0].val.clusterDim.y = 1;
+      qa[0].val.clusterDim.z = 1;
+      qc.attrs = qa;
+      qc.numAttrs = 1;
+      int q = 0;
+      e = cudaOccupancyMaxActiveClusters(&q, reinterpret_cast<const void*>(v.fn), &qc);
+      if (e == cudaSuccess && q > 0) {
+        if (q < n) n = q;
+      } else {
+        cudaGetLastError();
+      }
+    }
+    d.clusters2[vi] = n > 0 ? n : 1;
+    d.ready[vi] = true;
+  }
+  *clusters = d.clusters2[vi];
+  return SGL_OK;
+}
+
+// Tensor map over bf16 (or bytes) [outer][rows][cols]; rank 2 when outer == 0.
+int make_expert_map(CUtensorMap* out, const void* base, int64_t cols, int64_t rows, int64_t outer,
+                    int64_t ld_bytes, int64_t outer_bytes, int box_cols, int box_rows,
+                    const char* name, bool bytes = false,
+                    CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B,
+                    CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
+  EncodeTiledFn fn = encode_tiled_fn();
+  if (!fn) return fail(SGL_ERR_NO_DRIVER, "cuTensorMapEncodeTiled is not available");
+  const cuuint32_t rank = outer > 0 ? 3 : 2;
+  cuuint64_t dims[3] = {static_cast<cuuint64_t>(cols), static_cast<cuuint64_t>(rows),
+                        static_cast<cuuint64_t>(outer)};
+  cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_bytes), static_cast<cuuint64_t>(outer_bytes)};
+  cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = fn(out, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  rank, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(SGL_ERR_TENSOR_MAP,
+                "cuTensorMapEncodeTiled(%s) failed with CUresult %d (cols=%lld rows=%lld outer=%lld "
+                "pitch=%lld)",
+                name, static_cast<int>(r), static_cast<long long>(cols),
+                static_cast<long long>(rows), static_cast<long long>(outer),
+                static_cast<long long>(ld_bytes));
+  return SGL_OK;
+}
+
+int validate_groups(int64_t R, int64_t E, const void* offsets, bool need_offsets) {
+  if (R < 1 || R > 0x7fffff00ll)
+    return fail(SGL_ERR_BAD_SHAPE, "R=%lld rows must be in [1, 2^31)", static_cast<long long>(R));
+  if (E < 1 || E > sgl::kExpMaxGroups)
+    return fail(SGL_ERR_BAD_SHAPE, "E=%lld experts outside [1, %d]", static_cast<long long>(E),
+                sgl::kExpMaxGroups);
+  if (!offsets && need_offsets) return fail(SGL_ERR_NULL_POINTER, "offsets is NULL");
+  if (reinterpret_cast<uintptr_t>(offsets) & 3u)
+    return fail(SGL_ERR_MISALIGNED, "offsets is not 4-byte aligned");
+  return SGL_OK;
+}
+
+int validate_expert_stride(int64_t stride, int64_t rows, int64_t ld, int64_t E, const char* name) {
+  if (E == 1) return SGL_OK;
+  if (stride % 8 != 0 || stride < (rows - 1) * ld)
+    return fail(SGL_ERR_BAD_STRIDE,
+                "%s=%lld: an expert's matrix must be a multiple of 8 elements and at least its "
+                "rows apart from the next one's",
+                name, static_cast<long long>(stride));
+  return SGL_OK;
+}
+
+// One launch of experts_kernel.
+struct ExpertLaunch {
+  int form = sgl::EXP_GEMM;
+  const char* name = "";
+  const void* a = nullptr;
+  const void* b = nullptr;
+  void* out = nullptr;
+  const int* offsets = nullptr;
+  int64_t R = 0, N = 0, K = 0, M = 0, E = 0;
+  int64_t lda = 0, ldb = 0, b_stride = 0, ld_out = 0, out_stride = 0;
+  int b_transposed = 0;
+  void* pre = nullptr;       // saved pre-activations (see preact_layout)
+  void* scales = nullptr;
+};
+
+// Byte layout of saved pre-activations: rows of [up | gate], each half padded to whole blocks.
+struct PreactLayout {
+  int64_t pitch, gate_off;             // bytes
+  int64_t scale_pitch, gate_scale_off; // bytes (8-bit form)
+};
+PreactLayout preact_layout(int bits, int64_t N) {
+  PreactLayout l;
+  const int64_t half = (N + 31) / 32 * 32 * (bits / 8);
+  l.pitch = 2 * half;
+  l.gate_off = half;
+  l.gate_scale_off = bits == 8 ? (N + 63) / 64 * 2 : 0;
+  l.scale_pitch = 2 * l.gate_scale_off;
+  return l;
+}
+
+int launch_experts(const ExpertLaunch& s, void* stream) {
+  DeviceInfo* info = nullptr;
+  int rc = check_device(&info);
+  if (rc) return rc;
+  const bool wgrad = s.form == sgl::EXP_WGRAD;
+  const bool swiglu = s.form != sgl::EXP_GEMM && !wgrad;
+
+  // CTA pairs (256-row tiles) once the groups fill them on average; single CTAs (128 rows) else.
+  int cta_group = 1;
+  if (wgrad) {
+    cta_group = s.M > sgl::kBlockM ? 2 : 1;
+  } else if (s.R / s.E >= 192) {
+    cta_group = 2;
+  }
+  int clusters = 0;
+  if ((rc = prepare_expert_variant(s.form, cta_group, info, &clusters))) return rc;
+  const ExpertVariant& v = expert_variant(s.form, cta_group);
+
+  const int tile_rows = sgl::kBlockM * cta_group;
+  // tile rows there can be at most: every group may end in a partly filled one
+  const int64_t groups_used = wgrad ? s.E : (s.E < s.R ? s.E : s.R);
+  const int64_t max_tiles_m = wgrad ? (s.M + tile_rows - 1) / tile_rows * s.E
+                                    : s.R / tile_rows + groups_used;
+  int acc_cols = sgl::kAccCols;
+  const int min_cols = swiglu ? 128 : 64;
+  if (cta_group == 1 && !wgrad) {
+    while (acc_cols > min_cols) {
+      const int64_t cols = swiglu ? acc_cols / 2 : acc_cols;
+      if (max_tiles_m * ((s.N + cols - 1) / cols) >= 2 * info->sm_count) break;
+      acc_cols /= 2;
+    }
+  }
+  const int tile_cols = swiglu ? acc_cols / 2 : acc_cols;
+  const int64_t tiles_n = (s.N + tile_cols - 1) / tile_cols;
+  if (max_tiles_m * tiles_n > 0x7fffffffll) return fail(SGL_ERR_BAD_SHAPE, "too many tiles");
+  int a_rows = sgl::kBlockM;
+  if (cta_group == 1 && !wgrad && s.R < sgl::kBlockM)
+    a_rows = static_cast<int>((s.R + 15) / 16 * 16);
+  const int stages = v.max_stages(static_cast<int>(s.E), a_rows, acc_cols);
+  const int smem = v.smem_bytes(static_cast<int>(s.E), a_rows, acc_cols, stages);
+
+  sgl::ExpertMaps maps;
+  std::memset(&maps, 0, sizeof(maps));
+  const PreactLayout pl = preact_layout(s.form == sgl::EXP_SAVE8 ? 8 : 16, s.N);
+  if (wgrad) {
+    if ((rc = make_expert_map(&maps.a, s.a, s.M, s.R, 0, s.lda * 2, 0, 64, kExpertBlockK, "a")) ||
+        (rc = make_expert_map(&maps.b, s.b, s.N, s.R, 0, s.ldb * 2, 0, 64, kExpertBlockK, "g")) ||
+        (rc = make_expert_map(&maps.out, s.out, s.N, s.M, s.E, s.ld_out * 2, s.out_stride * 2, 64,
+                              32, "out", false, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+      return rc;
+  } else {
+    const int64_t b_cols = s.b_transposed ? s.K : (swiglu ? 2 * s.N : s.N);
+    const int64_t b_rows = s.b_transposed ? s.N : s.K;
+    if ((rc = make_expert_map(&maps.a, s.a, s.K, s.R, 0, s.lda * 2, 0, 64, sgl::kBlockM, "a")) ||
+        (rc = make_expert_map(&maps.a16, s.a, s.K, s.R, 0, s.lda * 2, 0, 64, 16, "a")) ||
+        (rc = make_expert_map(&maps.b, s.b, b_cols, b_rows, s.E, s.ldb * 2, s.b_stride * 2, 64,
+                              s.b_transposed ? 64 : kExpertBlockK, "b")) ||
+        (rc = make_expert_map(&maps.out, s.out, s.N, s.R, 0, s.ld_out * 2, 0, 64, 32, "out", false,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+      return rc;
+    if (s.form == sgl::EXP_SAVE16 || s.form == sgl::EXP_SAVE8) {
+      const bool bytes = s.form == sgl::EXP_SAVE8;
+      uint8_t* pre = static_cast<uint8_t*>(s.pre);
+      const CUtensorMapSwizzle sw = bytes ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
+      if ((rc = make_expert_map(&maps.up, pre, s.N, s.R, 0, pl.pitch, 0, 64, 32, "up", bytes, sw,
+                                CU_TENSOR_MAP_L2_PROMOTION_NONE)) ||
+          (rc = make_expert_map(&maps.gate, pre + pl.gate_off, s.N, s.R, 0, pl.pitch, 0, 64, 32,
+                                "gate", bytes, sw, CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+        return rc;
+    }
+  }
+
+  sgl::ExpertParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.offsets = s.offsets;
+  p.groups = static_cast<int>(s.E);
+  p.R = static_cast<int>(s.R);
+  p.N = static_cast<int>(s.N);
+  p.K = static_cast<int>(s.K);
+  p.M = static_cast<int>(s.M);
+  p.tiles_n = static_cast<int>(tiles_n);
+  p.group_m = 8;
+  p.stages = stages;
+  p.acc_cols = acc_cols;
+  p.a_rows = a_rows;
+  p.b_kmajor = s.b_transposed;
+  p.out = static_cast<__nv_bfloat16*>(s.out);
+  p.ld_out = s.ld_out;
+  p.pre = static_cast<uint8_t*>(s.pre);
+  p.ld_pre = pl.pitch;
+  p.gate_off = pl.gate_off;
+  p.scales = static_cast<uint8_t*>(s.scales);
+  p.ld_scales = pl.scale_pitch;
+  p.gate_scale_off = pl.gate_scale_off;
+  p.l2_hints = 0;
+  p.wait_limit_ns = g_wait_limit_ns.load();
+
+  int64_t grid = clusters;
+  if (max_tiles_m * tiles_n < grid) grid = max_tiles_m * tiles_n;
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = dim3(static_cast<unsigned>(grid * cta_group), 1, 1);
+  lc.blockDim = dim3(sgl::kExpThreads, 1, 1);
+  lc.dynamicSmemBytes = static_cast<size_t>(smem);
+  lc.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = static_cast<unsigned>(cta_group);
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  lc.attrs = attrs;
+  lc.numAttrs = 2;
+  if (log_enabled())
+    fprintf(stderr,
+            "[libswiglu_b200] launch sgl %s R=%lld N=%lld K=%lld M=%lld E=%lld cta_group=%d "
+            "acc_cols=%d a_rows=%d stages=%d grid=%lld smem=%d\n",
+            s.name, static_cast<long long>(s.R), static_cast<long long>(s.N),
+            static_cast<long long>(s.K), static_cast<long long>(s.M), static_cast<long long>(s.E),
+            cta_group, acc_cols, a_rows, stages, static_cast<long long>(grid * cta_group), smem);
+  if (nvtx_enabled()) nvtxRangePushA(s.name);
+  cudaError_t e = cudaLaunchKernelEx(&lc, v.fn, maps, p);
+  if (nvtx_enabled()) nvtxRangePop();
+  if (e != cudaSuccess) return fail_cuda(e, "experts_kernel launch");
+  g_launches.fetch_add(1);
+  return SGL_OK;
+}
+
+// A launch whose grid may be set up while its predecessor in the stream still runs (the kernels
+// wait with griddepcontrol.wait before they touch memory).
+template <class... Args, class... Given>
+int launch_after(const char* what, void (*fn)(Args...), dim3 grid, dim3 block, int smem,
+                 unsigned cluster, void* stream, Given... args) {
+  cudaLaunchConfig_t lc = {};
+  lc.gridDim = grid;
+  lc.blockDim = block;
+  lc.dynamicSmemBytes = static_cast<size_t>(smem);
+  lc.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = cluster;
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
+  lc.attrs = attrs;
+  lc.numAttrs = cluster > 1 ? 2 : 1;
+  if (log_enabled()) fprintf(stderr, "[libswiglu_b200] launch sgl %s grid=%u\n", what, grid.x);
+  cudaError_t e = cudaLaunchKernelEx(&lc, fn, args...);
+  if (e != cudaSuccess) return fail_cuda(e, what);
+  g_launches.fetch_add(1);
+  return SGL_OK;
+}
+
+int validate_routing(int64_t T, int64_t k, int64_t E) {
+  if (T < 1 || k < 1 || k > 64 || E < 1 || E > sgl::kOrderMaxExperts)
+    return fail(SGL_ERR_BAD_SHAPE, "T=%lld >= 1 tokens, k=%lld in [1, 64], E=%lld in [1, %d] needed",
+                static_cast<long long>(T), static_cast<long long>(k), static_cast<long long>(E),
+                sgl::kOrderMaxExperts);
+  if (T > 0x7fffff00ll / k)
+    return fail(SGL_ERR_BAD_SHAPE, "T * k = %lld * %lld does not fit 31 bits",
+                static_cast<long long>(T), static_cast<long long>(k));
+  return SGL_OK;
+}
+
+int validate_words(const void* p, const char* name, unsigned align) {
+  if (!p) return fail(SGL_ERR_NULL_POINTER, "%s is NULL", name);
+  if (reinterpret_cast<uintptr_t>(p) & (align - 1))
+    return fail(SGL_ERR_MISALIGNED, "%s is not %u-byte aligned", name, align);
+  return SGL_OK;
+}
+
+int validate_row_call(int64_t T, int64_t k, int64_t D, int64_t R) {
+  int rc = validate_routing(T, k, 1);
+  if (rc) return rc;
+  if (D < 8 || D % 8 != 0 || D > 0x7fffff00ll)
+    return fail(SGL_ERR_BAD_SHAPE, "D=%lld must be a positive multiple of 8",
+                static_cast<long long>(D));
+  if (R < 1 || R > 0x7fffff00ll)
+    return fail(SGL_ERR_BAD_SHAPE, "R=%lld rows must be in [1, 2^31)", static_cast<long long>(R));
+  return SGL_OK;
+}
+
+// Threads of a token (a power of two of warps, at most 256) and CTAs for `T` tokens.
+void row_geometry(int64_t T, int nvec, const DeviceInfo* info, dim3* grid, dim3* block) {
+  unsigned tx = 32;
+  while (tx < 256 && tx < static_cast<unsigned>(nvec)) tx *= 2;
+  *block = dim3(tx, 256 / tx, 1);
+  int64_t ctas = (T + block->y - 1) / block->y;
+  const int64_t cap = static_cast<int64_t>(info->sm_count) * 8;
+  *grid = dim3(static_cast<unsigned>(ctas < cap ? ctas : cap), 1, 1);
+}
+
+int check_bits(int bits) {
+  if (bits != 8 && bits != 16) return fail(SGL_ERR_BAD_ARGUMENT, "bits=%d must be 8 or 16", bits);
+  return SGL_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, int64_t ld_ids,
+                     int64_t E, void* offsets, void* slots, void* rows, void* stream) {
+  int rc;
+  if ((rc = validate_routing(T, k, E))) return rc;
+  if ((rc = validate_words(ids, "ids", ids_are_int64 ? 8 : 4)) ||
+      (rc = validate_words(offsets, "offsets", 4)) || (rc = validate_words(slots, "slots", 4)) ||
+      (rc = validate_words(rows, "rows", 4)))
+    return rc;
+  if (ld_ids < k)
+    return fail(SGL_ERR_BAD_STRIDE, "ld_ids=%lld is smaller than k=%lld",
+                static_cast<long long>(ld_ids), static_cast<long long>(k));
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info))) return rc;
+  const int smem = sgl::order_smem_bytes(static_cast<int>(E));
+  {
+    int dev = 0;
+    if ((rc = current_device(&dev))) return rc;
+    std::lock_guard<std::mutex> lock(g_dev_mutex);
+    ExpertDevice& d = g_expert_devices[dev];
+    if (!d.order_ready) {
+      cudaError_t e = cudaFuncSetAttribute(
+          reinterpret_cast<const void*>(sgl::expert_order_kernel),
+          cudaFuncAttributeMaxDynamicSharedMemorySize,
+          sgl::order_smem_bytes(sgl::kOrderMaxExperts));
+      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(expert_order)");
+      d.order_ready = true;
+    }
+  }
+  sgl::OrderParams p;
+  p.ids = ids;
+  p.ld_ids = ld_ids;
+  p.total = T * k;
+  p.k = static_cast<int>(k);
+  p.E = static_cast<int>(E);
+  p.ids64 = ids_are_int64 != 0;
+  p.offsets = static_cast<int*>(offsets);
+  p.slots = static_cast<int*>(slots);
+  p.rows = static_cast<int*>(rows);
+  const unsigned ctas = p.total > 4 * sgl::kOrderThreads ? sgl::kOrderCluster : 1;
+  return launch_after("expert_order", sgl::expert_order_kernel, dim3(ctas), dim3(sgl::kOrderThreads),
+                      smem, ctas, stream, p);
+}
+
+int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
+                        int64_t R, int64_t ldx, int64_t ldo, void* stream) {
+  int rc;
+  if ((rc = validate_row_call(T, k, D, R))) return rc;
+  if ((rc = validate_ptr(x, "x")) || (rc = validate_words(rows, "rows", 4)) ||
+      (rc = validate_ptr(out, "out")))
+    return rc;
+  if ((rc = validate_ld(ldx, D, "ldx")) || (rc = validate_ld(ldo, D, "ldo"))) return rc;
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info))) return rc;
+  sgl::RowParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.in = static_cast<const __nv_bfloat16*>(x);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.rows = static_cast<const int*>(rows);
+  p.ld_in = ldx;
+  p.ld_out = ldo;
+  p.T = T;
+  p.k = static_cast<int>(k);
+  p.nvec = static_cast<int>(D / 8);
+  p.R = R;
+  dim3 grid, block;
+  row_geometry(T, p.nvec, info, &grid, &block);
+  return launch_after("expert_dispatch", sgl::expert_dispatch_kernel, grid, block, 0, 1, stream, p);
+}
+
+int sgl_expert_combine(const void* in, const void* rows, const void* weights, int weights_bf16,
+                       void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
+                       int64_t ld_w, int64_t ldo, void* stream) {
+  int rc;
+  if ((rc = validate_row_call(T, k, D, R))) return rc;
+  if ((rc = validate_ptr(in, "in")) || (rc = validate_words(rows, "rows", 4)) ||
+      (rc = validate_ptr(out, "out")))
+    return rc;
+  if (weights) {
+    if ((rc = validate_words(weights, "weights", weights_bf16 ? 2 : 4))) return rc;
+    if (ld_w < k)
+      return fail(SGL_ERR_BAD_STRIDE, "ld_w=%lld is smaller than k=%lld",
+                  static_cast<long long>(ld_w), static_cast<long long>(k));
+  }
+  if ((rc = validate_ld(ld_in, D, "ld_in")) || (rc = validate_ld(ldo, D, "ldo"))) return rc;
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info))) return rc;
+  sgl::RowParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.in = static_cast<const __nv_bfloat16*>(in);
+  p.out = static_cast<__nv_bfloat16*>(out);
+  p.rows = static_cast<const int*>(rows);
+  p.weights = weights;
+  p.w_bf16 = weights_bf16 != 0;
+  p.ld_in = ld_in;
+  p.ld_out = ldo;
+  p.ld_w = ld_w;
+  p.T = T;
+  p.k = static_cast<int>(k);
+  p.nvec = static_cast<int>(D / 8);
+  p.R = R;
+  dim3 grid, block;
+  row_geometry(T, p.nvec, info, &grid, &block);
+  return launch_after("expert_combine", sgl::expert_combine_kernel, grid, block, 0, 1, stream, p);
+}
+
+int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* rows,
+                            const void* weights, int weights_bf16, void* grad_rows,
+                            void* grad_weights, int64_t T, int64_t k, int64_t D, int64_t R,
+                            int64_t ld_go, int64_t ld_in, int64_t ld_w, int64_t ld_gr,
+                            void* stream) {
+  int rc;
+  if ((rc = validate_row_call(T, k, D, R))) return rc;
+  const unsigned wa = weights_bf16 ? 2 : 4;
+  if ((rc = validate_ptr(grad_out, "grad_out")) || (rc = validate_words(rows, "rows", 4)) ||
+      (rc = validate_words(weights, "weights", wa)) || (rc = validate_ptr(grad_rows, "grad_rows")))
+    return rc;
+  if ((in != nullptr || grad_weights != nullptr) &&
+      ((rc = validate_ptr(in, "in")) || (rc = validate_words(grad_weights, "grad_weights", wa))))
+    return rc;
+  if (ld_w < k)
+    return fail(SGL_ERR_BAD_STRIDE, "ld_w=%lld is smaller than k=%lld",
+                static_cast<long long>(ld_w), static_cast<long long>(k));
+  if ((rc = validate_ld(ld_go, D, "ld_go")) || (in && (rc = validate_ld(ld_in, D, "ld_in"))) ||
+      (rc = validate_ld(ld_gr, D, "ld_gr")))
+    return rc;
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info))) return rc;
+  sgl::RowParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.in = static_cast<const __nv_bfloat16*>(grad_out);
+  p.in2 = static_cast<const __nv_bfloat16*>(in);
+  p.out = static_cast<__nv_bfloat16*>(grad_rows);
+  p.rows = static_cast<const int*>(rows);
+  p.weights = weights;
+  p.w_bf16 = weights_bf16 != 0;
+  p.grad_weights = grad_weights;
+  p.ld_in = ld_go;
+  p.ld_in2 = ld_in;
+  p.ld_out = ld_gr;
+  p.ld_w = ld_w;
+  p.T = T;
+  p.k = static_cast<int>(k);
+  p.nvec = static_cast<int>(D / 8);
+  p.R = R;
+  dim3 grid, block;
+  row_geometry(T, p.nvec, info, &grid, &block);
+  return launch_after("expert_combine_grad", sgl::expert_combine_grad_kernel, grid, block, 0, 1,
+                      stream, p);
+}
+
+int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int64_t* scale_bytes,
+                         int64_t* scale_pitch) {
+  int rc;
+  if ((rc = check_bits(bits))) return rc;
+  if ((rc = validate_shape(rows < 1 ? 1 : rows, N, 8))) return rc;
+  const PreactLayout l = preact_layout(bits, N);
+  if (pitch) *pitch = l.pitch;
+  if (scale_pitch) *scale_pitch = l.scale_pitch;
+  if (scale_bytes) *scale_bytes = l.scale_pitch * rows;
+  return l.pitch * rows;
+}
+
+static int grouped_swiglu(const char* name, const void* x, const void* w, const void* offsets,
+                          void* h, void* pre, void* scales, int bits, int64_t R, int64_t N,
+                          int64_t K, int64_t E, int64_t ldx, int64_t ldw, int64_t w_stride,
+                          int64_t ldh, void* stream) {
+  int rc;
+  if ((rc = validate_groups(R, E, offsets, E > 1))) return rc;
+  if ((rc = validate_ptr(x, "x")) || (rc = validate_ptr(w, "w")) || (rc = validate_ptr(h, "h")))
+    return rc;
+  if ((rc = validate_shape(R, N, K))) return rc;
+  if ((rc = validate_ld(ldx, K, "ldx")) || (rc = validate_ld(ldw, 2 * N, "ldw")) ||
+      (rc = validate_ld(ldh, N, "ldh")) ||
+      (rc = validate_expert_stride(w_stride, K, ldw, E, "w_stride")))
+    return rc;
+  ExpertLaunch s;
+  s.form = bits == 0 ? sgl::EXP_SWIGLU : (bits == 8 ? sgl::EXP_SAVE8 : sgl::EXP_SAVE16);
+  if (bits != 0) {
+    if ((rc = validate_ptr(pre, "pre"))) return rc;
+    if (bits == 8 && (rc = validate_words(scales, "scales", 2))) return rc;
+  }
+  s.name = name;
+  s.a = x;
+  s.b = w;
+  s.out = h;
+  s.offsets = static_cast<const int*>(offsets);
+  s.R = R;
+  s.N = N;
+  s.K = K;
+  s.E = E;
+  s.lda = ldx;
+  s.ldb = ldw;
+  s.b_stride = E > 1 ? w_stride : K * ldw;
+  s.ld_out = ldh;
+  s.pre = pre;
+  s.scales = scales;
+  return launch_experts(s, stream);
+}
+
+int sgl_grouped_fused_swiglu(const void* x, const void* w, const void* offsets, void* h, int64_t R,
+                             int64_t N, int64_t K, int64_t E, int64_t ldx, int64_t ldw,
+                             int64_t w_stride, int64_t ldh, void* stream) {
+  int rc = validate_groups(R, E, offsets, true);
+  if (rc) return rc;
+  return grouped_swiglu("grouped_fused_swiglu", x, w, offsets, h, nullptr, nullptr, 0, R, N, K, E,
+                        ldx, ldw, w_stride, ldh, stream);
+}
+
+int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offsets, void* h,
+                                  void* pre, void* scales, int bits, int64_t R, int64_t N,
+                                  int64_t K, int64_t E, int64_t ldx, int64_t ldw, int64_t w_stride,
+                                  int64_t ldh, void* stream) {
+  int rc = check_bits(bits);
+  if (rc) return rc;
+  return grouped_swiglu("grouped_fused_swiglu_save", x, w, offsets, h, pre, scales, bits, R, N, K,
+                        E, ldx, ldw, w_stride, ldh, stream);
+}
+
+int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
+                       int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
+                       int64_t ldc, int b_transposed, void* stream) {
+  int rc;
+  if ((rc = validate_groups(R, E, offsets, true))) return rc;
+  if ((rc = validate_ptr(a, "a")) || (rc = validate_ptr(b, "b")) || (rc = validate_ptr(c, "c")))
+    return rc;
+  if ((rc = validate_shape(R, N, K))) return rc;
+  const int64_t b_rows = b_transposed ? N : K;
+  if ((rc = validate_ld(lda, K, "lda")) || (rc = validate_ld(ldb, b_transposed ? K : N, "ldb")) ||
+      (rc = validate_ld(ldc, N, "ldc")) ||
+      (rc = validate_expert_stride(b_stride, b_rows, ldb, E, "b_stride")))
+    return rc;
+  ExpertLaunch s;
+  s.form = sgl::EXP_GEMM;
+  s.name = "grouped_matmul";
+  s.a = a;
+  s.b = b;
+  s.out = c;
+  s.offsets = static_cast<const int*>(offsets);
+  s.R = R;
+  s.N = N;
+  s.K = K;
+  s.E = E;
+  s.lda = lda;
+  s.ldb = ldb;
+  s.b_stride = E > 1 ? b_stride : b_rows * ldb;
+  s.ld_out = ldc;
+  s.b_transposed = b_transposed != 0;
+  return launch_experts(s, stream);
+}
+
+int sgl_grouped_weight_grad(const void* a, const void* g, const void* offsets, void* c, int64_t R,
+                            int64_t M, int64_t N, int64_t E, int64_t lda, int64_t ldg, int64_t ldc,
+                            int64_t c_stride, void* stream) {
+  int rc;
+  if ((rc = validate_groups(R, E, offsets, true))) return rc;
+  if ((rc = validate_ptr(a, "a")) || (rc = validate_ptr(g, "g")) || (rc = validate_ptr(c, "c")))
+    return rc;
+  if ((rc = validate_shape(R, N, M))) return rc;
+  if ((rc = validate_ld(lda, M, "lda")) || (rc = validate_ld(ldg, N, "ldg")) ||
+      (rc = validate_ld(ldc, N, "ldc")) ||
+      (rc = validate_expert_stride(c_stride, M, ldc, E, "c_stride")))
+    return rc;
+  ExpertLaunch s;
+  s.form = sgl::EXP_WGRAD;
+  s.name = "grouped_weight_grad";
+  s.a = a;
+  s.b = g;
+  s.out = c;
+  s.offsets = static_cast<const int*>(offsets);
+  s.R = R;
+  s.N = N;
+  s.K = R;
+  s.M = M;
+  s.E = E;
+  s.lda = lda;
+  s.ldb = ldg;
+  s.ld_out = ldc;
+  s.out_stride = E > 1 ? c_stride : M * ldc;
+  return launch_experts(s, stream);
+}
+
+int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* scales, int bits,
+                                 void* grad_preact, void* h, const void* end, int64_t rows,
+                                 int64_t N, int64_t lddy, int64_t ldo, int64_t ldh, void* stream) {
+  int rc;
+  if ((rc = check_bits(bits))) return rc;
+  if ((rc = validate_ptr(dy, "dy")) || (rc = validate_ptr(pre, "pre")) ||
+      (rc = validate_ptr(grad_preact, "grad_preact")))
+    return rc;
+  if (bits == 8 && (rc = validate_words(scales, "scales", 2))) return rc;
+  if (h && (rc = validate_ptr(h, "h"))) return rc;
+  if (end && (rc = validate_words(end, "end", 4))) return rc;
+  if ((rc = validate_shape(rows, N, 8))) return rc;
+  if ((rc = validate_ld(lddy, N, "lddy")) || (rc = validate_ld(ldo, 2 * N, "ldo"))) return rc;
+  if (h && (rc = validate_ld(ldh, N, "ldh"))) return rc;
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info))) return rc;
+  const PreactLayout l = preact_layout(bits, N);
+  sgl::PreactParams p;
+  p.dy = static_cast<const __nv_bfloat16*>(dy);
+  p.pre = static_cast<const uint8_t*>(pre);
+  p.scales = static_cast<const uint8_t*>(scales);
+  p.grad = static_cast<__nv_bfloat16*>(grad_preact);
+  p.h = static_cast<__nv_bfloat16*>(h);
+  p.end = static_cast<const int*>(end);
+  p.lddy = lddy;
+  p.ld_pre = l.pitch;
+  p.gate_off = l.gate_off;
+  p.ld_scales = l.scale_pitch;
+  p.gate_scale_off = l.gate_scale_off;
+  p.ld_grad = ldo;
+  p.ldh = ldh;
+  p.rows = rows;
+  p.nvec = static_cast<int>(N / 8);
+  const int64_t vecs = rows * p.nvec;
+  int64_t blocks = (vecs + 255) / 256;
+  const int64_t cap = static_cast<int64_t>(info->sm_count) * 8;
+  if (blocks > cap) blocks = cap;
+  return launch_after("grad_preact_saved",
+                      bits == 8 ? sgl::grad_preact_saved_kernel<8> : sgl::grad_preact_saved_kernel<16>,
+                      dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, stream, p);
+}
+
+// ---- the expert layer at inference, one call ----
+
+static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
+
+struct ExpertsWorkspace {
+  int64_t offsets, slots, rows, xs, h, ys, total;
+};
+
+static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
+                             ExpertsWorkspace* w) {
+  int rc;
+  if ((rc = validate_routing(T, k, E)) || (rc = validate_shape(T * k, N, D)) ||
+      (rc = validate_shape(T * k, D_out, 8)))
+    return rc;
+  const int64_t R = T * k;
+  int64_t at = 0;
+  w->offsets = at;
+  at += align256((E + 1) * 4);
+  w->slots = at;
+  at += align256(R * 4);
+  w->rows = at;
+  at += align256(R * 4);
+  w->xs = at;
+  at += align256(R * D * 2);
+  w->h = at;
+  at += align256(R * N * 2);
+  w->ys = at;
+  at += align256(R * D_out * 2);
+  w->total = at;
+  return SGL_OK;
+}
+
+int64_t sgl_experts_swiglu_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N,
+                                           int64_t D_out) {
+  ExpertsWorkspace w;
+  int rc = experts_workspace(T, k, E, D, N, D_out, &w);
+  return rc ? rc : w.total;
+}
+
+int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const void* weights,
+                       int weights_bf16, const void* w, const void* w_down, void* y,
+                       void* workspace, int64_t workspace_bytes, int64_t T, int64_t k, int64_t E,
+                       int64_t D, int64_t N, int64_t D_out, int64_t ldx, int64_t ld_ids,
+                       int64_t ld_weights, int64_t ldw, int64_t w_stride, int64_t ldd,
+                       int64_t d_stride, int64_t ldy, void* stream) {
+  ExpertsWorkspace l;
+  int rc;
+  if ((rc = experts_workspace(T, k, E, D, N, D_out, &l))) return rc;
+  if ((rc = validate_ptr(x, "x")) || (rc = validate_words(ids, "ids", ids_are_int64 ? 8 : 4)) ||
+      (rc = validate_words(weights, "weights", weights_bf16 ? 2 : 4)) ||
+      (rc = validate_ptr(w, "w")) || (rc = validate_ptr(w_down, "w_down")) ||
+      (rc = validate_ptr(y, "y")) || (rc = validate_ptr(workspace, "workspace")))
+    return rc;
+  if (workspace_bytes < l.total)
+    return fail(SGL_ERR_BAD_ARGUMENT, "workspace holds %lld bytes, %lld needed",
+                static_cast<long long>(workspace_bytes), static_cast<long long>(l.total));
+  // everything the launches below would refuse is refused before the first of them
+  if (ld_ids < k || ld_weights < k)
+    return fail(SGL_ERR_BAD_STRIDE, "ld_ids=%lld and ld_weights=%lld must be at least k=%lld",
+                static_cast<long long>(ld_ids), static_cast<long long>(ld_weights),
+                static_cast<long long>(k));
+  if ((rc = validate_ld(ldx, D, "ldx")) || (rc = validate_ld(ldw, 2 * N, "ldw")) ||
+      (rc = validate_ld(ldd, D_out, "ldd")) || (rc = validate_ld(ldy, D_out, "ldy")) ||
+      (rc = validate_expert_stride(w_stride, D, ldw, E, "w_stride")) ||
+      (rc = validate_expert_stride(d_stride, N, ldd, E, "d_stride")))
+    return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t R = T * k;
+  if ((rc = sgl_expert_order(ids, ids_are_int64, T, k, ld_ids, E, ws + l.offsets, ws + l.slots,
+                             ws + l.rows, stream)) ||
+      (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream)) ||
+      (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
+                                     w_stride, N, stream)) ||
+      (rc = sgl_grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
+                               d_stride, D_out, 0, stream)))
+    return rc;
+  return sgl_expert_combine(ws + l.ys, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
+                            ld_weights, ldy, stream);
+}
+
+}  // extern "C"

@@ -1,0 +1,802 @@
+// Products over rows that are grouped by expert, on the tensor cores (tcgen05 + TMA).
+//
+// Row group e is [offsets[e], offsets[e+1]) of the row tensors (device memory: the host never
+// learns the sizes); groups may be empty or of any length, so their borders fall inside tiles.
+//   EXP_SWIGLU   h[r]  = silu(x[r] @ Wgate[e]) * (x[r] @ Wup[e]),   W[E, K, 2N] = [W_up | W_gate]
+//   EXP_SAVE16   the same, and the pre-activations [up | gate] in bf16
+//   EXP_SAVE8    the same, and the pre-activations in e4m3 with a power-of-two scale per row
+//                and 32 columns (1 + 1/32 bytes for each value)
+//   EXP_GEMM     c[r]  = a[r] @ B[e] or a[r] @ B[e]^T
+//   EXP_WGRAD    C[e]  = a_e^T @ g_e   (the sum runs over the rows of the group; 0 if it is empty)
+// With offsets == NULL there is one group of all rows (the dense stage's 8-bit checkpoints).
+//
+// Structure as the dense kernel's (swiglu_kernel.cuh): persistent CTAs (or CTA pairs on 256-row
+// tiles, tcgen05 cta_group::2), warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-5 = epilogue,
+// a 256-column fp32 accumulator in two TMEM stages.  What the groups change:
+//   * every CTA turns the offsets into a table of first tile rows once, and finds the expert
+//     of a tile by bisection in it;
+//   * an A tile whose rows run past its group takes them along in the operand (their
+//     accumulator rows are not stored), but in steps of 16 rows: one TMA box for a full tile,
+//     else ceil(rows / 16) small ones, so a group of one token does not fetch 128 rows;
+//   * the epilogue stores 32 whole rows with TMA; a warp whose rows end inside its 32 copies
+//     the rows that exist with plain stores, so that no row of another group is touched;
+//   * EXP_WGRAD sums over rows, so rows past the group must not reach the MMA: warp 6 waits
+//     for such a block of operands to land, overwrites them with zeros (TMA cannot clip at a
+//     border inside the tensor) and only then hands the block to the MMA issuer.
+// Every wait is bounded, as everywhere in this library.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+#include "ptx_sm100.cuh"
+#include "swiglu_kernel.cuh"
+
+namespace sgl {
+
+enum : int { EXP_SWIGLU = 0, EXP_SAVE16 = 1, EXP_SAVE8 = 2, EXP_GEMM = 3, EXP_WGRAD = 4 };
+
+constexpr int kExpThreads = 224;       // producer, MMA issuer, 4 epilogue warps, tail warp
+constexpr int kExpMaxStages = 16;
+constexpr int kExpBarrierBytes = 8 * (3 * kExpMaxStages + 2 * kAccStages) + 32;
+constexpr int kExpMaxGroups = 1024;
+
+enum : unsigned {
+  kErrExpProducerWait = 0x111,
+  kErrExpMmaFullWait = 0x112,
+  kErrExpMmaTmemWait = 0x113,
+  kErrExpEpilogueWait = 0x114,
+  kErrExpTailWait = 0x115,
+};
+
+struct ExpertMaps {
+  CUtensorMap a;        // A operand, whole-tile box
+  CUtensorMap a16;      // A operand, boxes of 16 rows (forward forms)
+  CUtensorMap b;        // B operand
+  CUtensorMap out;      // h / c / C
+  CUtensorMap up;       // pre-activations: up half
+  CUtensorMap gate;     // pre-activations: gate half
+};
+
+struct ExpertParams {
+  const int* offsets;   // [groups + 1] or NULL (one group of R rows)
+  int groups;
+  int R;                // rows of the row tensors
+  int N, K;             // columns of the result; extent of the sum (forward forms)
+  int M;                // EXP_WGRAD: rows of each C[e]
+  int tiles_n;
+  int group_m;          // tile rows walked together inside a group
+  int stages;
+  int acc_cols;         // accumulator columns of a tile (256; single-CTA tiles also 128, 64)
+  int a_rows;           // rows of an A slot: 128, or a multiple of 16 below it when R is small
+  int b_kmajor;         // B[e] is stored [n, k] (multiplied transposed)
+  __nv_bfloat16* out;   // forward forms: raw pointers for rows that end inside a warp's 32
+  int64_t ld_out;
+  uint8_t* pre;         // pre-activations, bytes; gate half at + gate_off
+  int64_t ld_pre;       // row pitch, bytes
+  int64_t gate_off;     // bytes from the up half to the gate half of a row
+  uint8_t* scales;      // EXP_SAVE8: [R][2][n_blocks] exponents + 127
+  int64_t ld_scales;    // row pitch, bytes
+  int64_t gate_scale_off;
+  int l2_hints;
+  unsigned long long wait_limit_ns;
+};
+
+template <int kForm, int kCtaGroup, int kBlockK>
+struct ExpertTraits {
+  static constexpr bool kSwiglu = kForm == EXP_SWIGLU || kForm == EXP_SAVE16 || kForm == EXP_SAVE8;
+  // staging of one epilogue warp: two 64-column chunks, or one chunk with its pre-activations
+  static constexpr int kStagingPerWarp =
+      kForm == EXP_SAVE16 ? 3 * kChunkBytes : 2 * kChunkBytes;
+  static constexpr int kStagingBytes = kEpiWarps * kStagingPerWarp;
+  static constexpr int kBSlabsMax = kAccCols / kCtaGroup / 64;
+  static constexpr int kBSlabBytes = kBlockK * 128;
+
+  __host__ __device__ static constexpr int a_stage_bytes(int a_rows) { return a_rows * kBlockK * 2; }
+  __host__ __device__ static constexpr int b_stage_bytes(int acc_cols) {
+    return acc_cols / kCtaGroup * kBlockK * 2;
+  }
+  __host__ __device__ static constexpr int table_bytes(int groups) {
+    return (2 * (groups + 1) * 4 + 15) / 16 * 16;
+  }
+  __host__ __device__ static constexpr int fixed_bytes(int groups) {
+    return 1024 + kStagingBytes + kExpBarrierBytes + table_bytes(groups);
+  }
+  // An MMA reads 128 A rows whatever the slot holds: past the last A slot it reads B slots.
+  __host__ __device__ static int max_stages(int groups, int a_rows, int acc_cols) {
+    const int s = (227 * 1024 - fixed_bytes(groups)) / (a_stage_bytes(a_rows) + b_stage_bytes(acc_cols));
+    return s > kExpMaxStages ? kExpMaxStages : s;
+  }
+  __host__ __device__ static int smem_bytes(int groups, int a_rows, int acc_cols, int stages) {
+    return fixed_bytes(groups) + stages * (a_stage_bytes(a_rows) + b_stage_bytes(acc_cols));
+  }
+};
+
+// ---------------------------------------------------------------- 8-bit blocks
+//
+// 32 values v share the scale 2^e, e the smallest integer (>= -127) with max|v| <= 448 * 2^e,
+// 448 being the largest e4m3 value: nothing saturates, and a value keeps a relative error of at
+// most 2^-4 down to 2^-15 of the block's largest.  From the bits of the maximum m * 2^x
+// (1 <= m < 2): e = x - 8, or x - 7 when m > 1.75; adding 0x1fffff to the bits carries into the
+// exponent field exactly then.  The stored byte is e + 127; 255 stands for a block that holds an
+// infinity or a NaN, and every value of it reads as NaN.
+__device__ __forceinline__ int block_exponent_code(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  if (bits >= 0x7f800000u) return 255;
+  const int field = static_cast<int>((bits + 0x1fffffu) >> 23) - 8;
+  return field < 0 ? 0 : field;
+}
+// 2^(127 - code), the factor a value is multiplied by before it is rounded to e4m3.
+__device__ __forceinline__ float block_inverse_scale(int code) {
+  return __uint_as_float(static_cast<uint32_t>(254 - code) << 23);   // code <= 247: normal
+}
+// 2^(code - 127) (NaN for 255): code 0 is the subnormal 2^-127.
+__device__ __forceinline__ float block_scale(int code) {
+  if (code == 255) return __uint_as_float(0x7fc00000u);
+  return __uint_as_float(code == 0 ? 0x00400000u : static_cast<uint32_t>(code) << 23);
+}
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  uint16_t lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b), "f"(a));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
+  return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+}
+// Rounds 32 values; returns the scale code.
+__device__ __forceinline__ int round_block_e4m3(const float (&v)[32], uint32_t (&codes)[8]) {
+  // (the bits of |v| order like the values, and a NaN's lie above every number's)
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const uint32_t b = __float_as_uint(v[i]) & 0x7fffffffu;
+    top = b > top ? b : top;
+  }
+  const int code = block_exponent_code(__uint_as_float(top));
+  const float inv = block_inverse_scale(code == 255 ? 127 : code);
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    codes[i] = pack_e4m3x4(v[4 * i] * inv, v[4 * i + 1] * inv, v[4 * i + 2] * inv,
+                           v[4 * i + 3] * inv);
+  return code;
+}
+
+// ---------------------------------------------------------------- extra PTX
+
+__device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap* map, int x,
+                                            int y, int z, uint32_t bar, uint64_t policy,
+                                            bool peer_barrier) {
+  if (peer_barrier) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes.cta_group::2"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
+        ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+  }
+}
+
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int y, int z,
+                                             uint32_t smem_src, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.global.shared::cta.bulk_group.L2::cache_hint"
+      " [%0, {%1, %2, %3}], [%4], %5;" ::"l"(reinterpret_cast<uint64_t>(map)),
+      "r"(x), "r"(y), "r"(z), "r"(smem_src), "l"(policy)
+      : "memory");
+}
+
+__device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                             uint32_t d) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+// Copies the first `rows` of 32 staged rows (row_bytes = 128 or 64 each, in the swizzle of a TMA
+// box of that width) to global memory, `cols16` pieces of 16 bytes per row at most (the last may
+// be cut: `bytes` valid bytes per row, a multiple of 8).  One warp.
+template <int kRowBytes>
+__device__ __forceinline__ void copy_rows(uint32_t buf, uint8_t* dst, int64_t ld, int rows,
+                                          int bytes, int lane) {
+  constexpr int kPieces = kRowBytes / 16;
+  for (int i = lane; i < rows * kPieces; i += 32) {
+    const int r = i / kPieces, piece = i % kPieces;
+    if (piece * 16 >= bytes) continue;
+    const int sw = kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
+    const uint4 v = ld_shared_v4(buf + static_cast<uint32_t>(r * kRowBytes + ((piece ^ sw) << 4)));
+    uint8_t* at = dst + r * ld + piece * 16;
+    if (bytes - piece * 16 >= 16) {
+      *reinterpret_cast<uint4*>(at) = v;
+    } else {
+      *reinterpret_cast<uint2*>(at) = make_uint2(v.x, v.y);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- the kernel
+
+template <int kForm, int kCtaGroup, int kBlockK>
+__global__ void __launch_bounds__(kExpThreads, 1)
+experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
+  using T = ExpertTraits<kForm, kCtaGroup, kBlockK>;
+  constexpr bool kWgrad = kForm == EXP_WGRAD;
+  constexpr bool kSwiglu = T::kSwiglu;
+  constexpr int kTileRows = kBlockM * kCtaGroup;
+
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t rank = (kCtaGroup == 2) ? ptx::cluster_ctarank() : 0u;
+  const int cluster_id = blockIdx.x / kCtaGroup;
+  const int num_clusters = gridDim.x / kCtaGroup;
+  const int stages = p.stages;
+  const int a_stage = T::a_stage_bytes(p.a_rows);
+  const int b_stage = T::b_stage_bytes(p.acc_cols);
+  const int b_slabs = p.acc_cols / kCtaGroup / 64;
+  const int tile_cols = kSwiglu ? p.acc_cols / 2 : p.acc_cols;
+
+  // ---- shared memory ----
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const uint32_t sA = smem_base;
+  const uint32_t sB = sA + stages * a_stage;
+  const uint32_t sOut = sB + stages * b_stage;
+  const uint32_t sBar = sOut + T::kStagingBytes;
+  const uint32_t bar_full = sBar;
+  const uint32_t bar_empty = bar_full + 8 * kExpMaxStages;
+  const uint32_t bar_land = bar_empty + 8 * kExpMaxStages;     // EXP_WGRAD: partial blocks
+  const uint32_t bar_tfull = bar_land + 8 * kExpMaxStages;
+  const uint32_t bar_tempty = bar_tfull + 8 * kAccStages;
+  const uint32_t tmem_slot = bar_tempty + 8 * kAccStages;
+  const uint32_t abort_slot = tmem_slot + 8;
+  const uint32_t table = abort_slot + 24;
+  volatile uint32_t* tmem_slot_ptr =
+      reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - smem_base));
+  int* abort_flag = reinterpret_cast<int*>(smem_gen + (abort_slot - smem_base));
+  int* row_lo = reinterpret_cast<int*>(smem_gen + (table - smem_base));   // [groups + 1]
+  int* tile_lo = row_lo + p.groups + 1;                                   // [groups + 1]
+
+  if (threadIdx.x == 0) {
+    abort_flag[0] = 0;
+    abort_flag[1] = 0;
+    for (int s = 0; s < stages; ++s) {
+      ptx::mbar_init(bar_full + 8 * s, kCtaGroup);
+      ptx::mbar_init(bar_empty + 8 * s, 1);
+      ptx::mbar_init(bar_land + 8 * s, 1);
+    }
+    for (int s = 0; s < kAccStages; ++s) {
+      ptx::mbar_init(bar_tfull + 8 * s, 1);
+      ptx::mbar_init(bar_tempty + 8 * s, kEpiWarps * kCtaGroup);
+    }
+    ptx::fence_mbar_init();
+    ptx::prefetch_tensormap(&maps.a);
+    ptx::prefetch_tensormap(&maps.b);
+    ptx::prefetch_tensormap(&maps.out);
+  }
+  if (warp == 1) ptx::tmem_alloc<kCtaGroup>(tmem_slot, kTmemCols);
+
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  // ---- the groups: first row and first tile row of each (clamped: rows that do not exist in
+  // the row tensors are never addressed, whatever the offsets say) ----
+  const int G = p.groups;
+  for (int e = threadIdx.x; e <= G; e += kExpThreads) {
+    int lo = p.offsets ? p.offsets[e] : (e == 0 ? 0 : p.R);
+    lo = lo < 0 ? 0 : (lo > p.R ? p.R : lo);
+    row_lo[e] = lo;
+  }
+  __syncthreads();
+  if (warp == 0 && !kWgrad) {
+    const int per = (G + 31) / 32;
+    const int e0 = lane * per, e1 = (e0 + per < G) ? e0 + per : G;
+    int mine = 0;
+    for (int e = e0; e < e1; ++e) {
+      const int n = row_lo[e + 1] - row_lo[e];
+      mine += n > 0 ? (n + kTileRows - 1) / kTileRows : 0;
+    }
+    int inc = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, inc, d);
+      if (lane >= d) inc += v;
+    }
+    int at = inc - mine;
+    for (int e = e0; e < e1; ++e) {
+      tile_lo[e] = at;
+      const int n = row_lo[e + 1] - row_lo[e];
+      at += n > 0 ? (n + kTileRows - 1) / kTileRows : 0;
+    }
+    if (lane == 31) tile_lo[G] = inc;
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (kCtaGroup == 2) ptx::cluster_sync();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+
+  const int wgrad_tiles_m = kWgrad ? (p.M + kTileRows - 1) / kTileRows : 0;
+  const int total_units = (kWgrad ? wgrad_tiles_m * G : tile_lo[G]) * p.tiles_n;
+
+  struct Unit {
+    int e;          // group
+    int row;        // forward: first row of the tile; EXP_WGRAD: first row of the group
+    int rows;       // forward: rows from there to the group's end; EXP_WGRAD: rows of the group
+    int m, n;       // EXP_WGRAD: first row of C[e]; first column of the result
+  };
+  auto unit_of = [&](int u) {
+    Unit r;
+    const int tm = u / p.tiles_n;
+    if constexpr (kWgrad) {
+      r.e = tm / wgrad_tiles_m;
+      const TileCoord tc = tile_coord(u - r.e * wgrad_tiles_m * p.tiles_n, wgrad_tiles_m,
+                                      p.tiles_n, p.group_m);
+      r.row = row_lo[r.e];
+      r.rows = row_lo[r.e + 1] - r.row;
+      if (r.rows < 0) r.rows = 0;
+      r.m = tc.m * kTileRows;
+      r.n = tc.n * tile_cols;
+    } else {
+      int lo = 0, hi = G;    // the group whose tile rows contain tm
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (tile_lo[mid] <= tm) lo = mid; else hi = mid;
+      }
+      r.e = lo;
+      const TileCoord tc = tile_coord(u - tile_lo[lo] * p.tiles_n, tile_lo[lo + 1] - tile_lo[lo],
+                                      p.tiles_n, p.group_m);
+      r.row = row_lo[lo] + tc.m * kTileRows;
+      r.rows = row_lo[lo + 1] - r.row;
+      r.m = 0;
+      r.n = tc.n * tile_cols;
+    }
+    return r;
+  };
+  // k-blocks of a unit
+  auto unit_kb = [&](const Unit& un) {
+    return ((kWgrad ? un.rows : p.K) + kBlockK - 1) / kBlockK;
+  };
+
+  const uint64_t limit = p.wait_limit_ns;
+
+  if (warp == 0) {
+    // =========================== TMA producer ===========================
+    if (lane == 0) {
+      const uint64_t pol_a = ptx::make_l2_policy(p.l2_hints & 3);
+      const uint64_t pol_b = ptx::make_l2_policy((p.l2_hints >> 2) & 3);
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+        const Unit un = unit_of(u);
+        const int num_kb = unit_kb(un);
+        // forward: rows of this CTA's half of the tile, and the boxes that cover them
+        int left = un.rows - static_cast<int>(rank) * kBlockM;
+        left = left < 0 ? 0 : (left > kBlockM ? kBlockM : left);
+        const int my_row = un.row + static_cast<int>(rank) * kBlockM;
+        const int boxes16 = (left + 15) / 16;
+        const bool whole = !kWgrad && boxes16 * 16 == p.a_rows && p.a_rows == kBlockM;
+        const uint32_t b_bytes = static_cast<uint32_t>(b_slabs * T::kBSlabBytes);
+        const uint32_t stage_tx =
+            b_bytes + static_cast<uint32_t>(kWgrad ? kBlockM * kBlockK * 2
+                                                   : boxes16 * 16 * kBlockK * 2);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          if (!ptx::mbar_wait(bar_empty + 8 * s, ph ^ 1u, limit, abort_flag)) {
+            report_error(kErrExpProducerWait, kb, abort_flag);
+            ok = false;
+            break;
+          }
+          const int k0 = kb * kBlockK;
+          const uint32_t full_local = bar_full + 8 * s;
+          uint32_t bar = (kCtaGroup == 2) ? ptx::mapa(full_local, 0) : full_local;
+          bool peer = kCtaGroup == 2;
+          if (SGL_DBG_COORD_BAD(un.row >= 0 && un.row < p.R && un.e >= 0 && un.e < G &&
+                                    (un.n & 7) == 0 && un.n < p.N && un.m >= 0,
+                                kb)) {
+            *reinterpret_cast<volatile int*>(abort_flag) = 1;
+            ok = false;
+            break;
+          }
+          if constexpr (kWgrad) {
+            // a block that the group ends in reports to this CTA's own barrier: the tail warp
+            // clears the rows behind the group and passes the block on
+            if (un.rows - k0 < kBlockK) {
+              bar = bar_land + 8 * s;
+              peer = false;
+            }
+          }
+          ptx::mbar_arrive_expect_tx_cluster(bar, stage_tx);
+          const uint32_t a_dst = sA + s * a_stage;
+          const uint32_t b_dst = sB + s * b_stage;
+          if constexpr (kWgrad) {
+#pragma unroll
+            for (int j = 0; j < kBlockM / 64; ++j) {
+              const int x = un.m + static_cast<int>(rank) * kBlockM + j * 64;
+              if (peer) {
+                ptx::tma_load_2d<true>(a_dst + j * (kBlockK * 128), &maps.a, x, un.row + k0, bar,
+                                       pol_a);
+              } else {
+                ptx::tma_load_2d<false>(a_dst + j * (kBlockK * 128), &maps.a, x, un.row + k0, bar,
+                                        pol_a);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < T::kBSlabsMax; ++j) {
+              if (j >= b_slabs) break;
+              const int x = un.n + (static_cast<int>(rank) * b_slabs + j) * 64;
+              if (peer) {
+                ptx::tma_load_2d<true>(b_dst + j * T::kBSlabBytes, &maps.b, x, un.row + k0, bar,
+                                       pol_b);
+              } else {
+                ptx::tma_load_2d<false>(b_dst + j * T::kBSlabBytes, &maps.b, x, un.row + k0, bar,
+                                        pol_b);
+              }
+            }
+          } else {
+#pragma unroll
+            for (int j = 0; j < kBlockK / 64; ++j) {
+              const uint32_t dst = a_dst + j * (p.a_rows * 128);
+              if (whole) {
+                ptx::tma_load_2d<kCtaGroup == 2>(dst, &maps.a, k0 + j * 64, my_row, bar, pol_a);
+              } else {
+                for (int i = 0; i < boxes16; ++i)
+                  ptx::tma_load_2d<kCtaGroup == 2>(dst + i * (16 * 128), &maps.a16, k0 + j * 64,
+                                                   my_row + i * 16, bar, pol_a);
+              }
+            }
+            if (p.b_kmajor) {
+              // B[e] stored [n, k]: boxes of 64 n-rows x 64 k, one 64-k slice of all this CTA's
+              // rows contiguous
+#pragma unroll
+              for (int j = 0; j < kBlockK / 64; ++j) {
+                for (int i = 0; i < b_slabs; ++i) {
+                  const int row = un.n + (static_cast<int>(rank) * b_slabs + i) * 64;
+                  tma_load_3d(b_dst + j * (b_slabs * 64 * 128) + i * (64 * 128), &maps.b,
+                              k0 + j * 64, row, un.e, bar, pol_b, peer);
+                }
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < T::kBSlabsMax; ++j) {
+                if (j >= b_slabs) break;
+                const int g = static_cast<int>(rank) * b_slabs + j;   // slab of the tile
+                int col = un.n + g * 64;
+                if constexpr (kSwiglu) {
+                  // the first half of the accumulator is up, the second gate
+                  const int half = p.acc_cols / 128;
+                  col = g < half ? un.n + g * 64 : p.N + un.n + (g - half) * 64;
+                }
+                tma_load_3d(b_dst + j * T::kBSlabBytes, &maps.b, col, k0, un.e, bar, pol_b, peer);
+              }
+            }
+          }
+          if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+      }
+      if (!ok) {
+        // loads in flight land before the CTA exits
+        const uint64_t t0 = ptx::globaltimer_ns();
+        while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+      }
+    }
+  } else if (warp == 1) {
+    // =========================== MMA issuer ===========================
+    if (rank == 0 && lane == 0) {
+      const uint32_t idesc =
+          ptx::make_idesc_bf16(kTileRows, p.acc_cols, /*a_mn_major=*/kWgrad,
+                               /*b_mn_major=*/p.b_kmajor == 0);
+      const bool b_kmajor = p.b_kmajor != 0;
+      constexpr uint16_t mask = (kCtaGroup == 2) ? 0x3 : 0x1;
+      int s = 0;
+      uint32_t ph = 0;
+      bool ok = true;
+      int i = 0;
+      for (int u = cluster_id; u < total_units && ok; u += num_clusters, ++i) {
+        const Unit un = unit_of(u);
+        const int as = i % kAccStages;
+        const uint32_t aph = (i / kAccStages) & 1u;
+        if (!ptx::mbar_wait(bar_tempty + 8 * as, aph ^ 1u, limit, abort_flag)) {
+          report_error(kErrExpMmaTmemWait, i, abort_flag);
+          break;
+        }
+        ptx::tc_fence_after_sync();
+        const uint32_t d_tmem = tmem_base + as * kAccCols;
+        const int num_kb = unit_kb(un);
+        for (int kb = 0; kb < num_kb; ++kb) {
+          // (a block that passed through the peer's tail warp carries its ordinary writes)
+          const bool tail = kWgrad && un.rows - kb * kBlockK < kBlockK;
+          const bool landed =
+              (kCtaGroup == 2 && tail)
+                  ? ptx::mbar_wait_acquire_cluster(bar_full + 8 * s, ph, limit, abort_flag)
+                  : ptx::mbar_wait(bar_full + 8 * s, ph, limit, abort_flag);
+          if (!landed) {
+            report_error(kErrExpMmaFullWait, kb, abort_flag);
+            ok = false;
+            break;
+          }
+          ptx::tc_fence_after_sync();
+          const uint32_t a_base = sA + s * a_stage;
+          const uint32_t b_base = sB + s * b_stage;
+#pragma unroll
+          for (int kk = 0; kk < kBlockK / 16; ++kk) {
+            const uint64_t a_desc =
+                kWgrad ? ptx::smem_desc_sw128(a_base + kk * 16 * 128, kBlockK * 128, 1024)
+                       : ptx::smem_desc_sw128(
+                             a_base + (kk >> 2) * (p.a_rows * 128) + (kk & 3) * 32, 16, 1024);
+            const uint64_t b_desc =
+                b_kmajor ? ptx::smem_desc_sw128(
+                               b_base + (kk >> 2) * (b_slabs * 64 * 128) + (kk & 3) * 32, 16, 1024)
+                         : ptx::smem_desc_sw128(b_base + kk * 16 * 128, T::kBSlabBytes, 1024);
+            ptx::umma_bf16<kCtaGroup>(d_tmem, a_desc, b_desc, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+          }
+          ptx::umma_commit<kCtaGroup>(bar_empty + 8 * s, mask);
+          if (++s == stages) {
+            s = 0;
+            ph ^= 1u;
+          }
+        }
+        if (ok) ptx::umma_commit<kCtaGroup>(bar_tfull + 8 * as, mask);
+      }
+    }
+  } else if (warp == 6) {
+    // =========================== tail warp (EXP_WGRAD) ===========================
+    if constexpr (kWgrad) {
+      // Walks the same sequence of blocks as the producer; acts on the ones a group ends in.
+      // The landing barrier of a slot completes a phase only for such blocks: its parity is
+      // counted (one bit per slot), not derived from the ring's.
+      uint32_t parities = 0;
+      int64_t block = 0;    // blocks before this unit's first
+      for (int u = cluster_id; u < total_units; u += num_clusters) {
+        const Unit un = unit_of(u);
+        const int num_kb = unit_kb(un);
+        const int valid = un.rows - (num_kb - 1) * kBlockK;    // rows of the last block
+        if (num_kb > 0 && valid < kBlockK) {
+          const int64_t b = block + num_kb - 1;
+          const int s = static_cast<int>(b % stages);
+          const bool landed =
+              ptx::mbar_wait(bar_land + 8 * s, (parities >> s) & 1u, limit, abort_flag);
+          if (!__all_sync(0xffffffffu, landed)) {
+            if (lane == 0) report_error(kErrExpTailWait, num_kb, abort_flag);
+            break;
+          }
+          parities ^= 1u << s;
+          // rows [valid, kBlockK) of every 64-column slab, whole 128-byte rows (the swizzle
+          // moves 16-byte pieces only inside a row)
+          const uint32_t a0 = sA + s * a_stage, b0 = sB + s * b_stage;
+          const int pieces = (kBlockK - valid) * 8;
+          for (int slab = 0; slab < kBlockM / 64 + b_slabs; ++slab) {
+            const uint32_t at = (slab < kBlockM / 64 ? a0 + slab * (kBlockK * 128)
+                                                     : b0 + (slab - kBlockM / 64) * T::kBSlabBytes) +
+                                static_cast<uint32_t>(valid) * 128u;
+            for (int i = lane; i < pieces; i += 32) st_shared_v4(at + i * 16, 0, 0, 0, 0);
+          }
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            const uint32_t full_local = bar_full + 8 * s;
+            if constexpr (kCtaGroup == 2) {
+              ptx::mbar_arrive_release_cluster(ptx::mapa(full_local, 0));
+            } else {
+              ptx::mbar_arrive(full_local);
+            }
+          }
+          __syncwarp();
+        }
+        block += num_kb;
+      }
+    }
+  } else {
+    // =========================== epilogue ===========================
+    const int q = warp & 3;
+    const uint32_t buf0 = sOut + q * T::kStagingPerWarp;
+    const uint32_t tempty = (kCtaGroup == 2) ? ptx::mapa(bar_tempty, 0) : bar_tempty;
+    const uint32_t row_sw = static_cast<uint32_t>(lane & 7);
+    const uint32_t row_off = static_cast<uint32_t>(lane) * 128u;
+    const uint64_t pol_out = ptx::make_l2_policy((p.l2_hints >> 4) & 3);
+    const int gate_col = p.acc_cols / 2;
+    int stores = 0;       // staging buffers filled so far
+    int i = 0;
+    for (int u = cluster_id; u < total_units; u += num_clusters, ++i) {
+      const Unit un = unit_of(u);
+      const int as = i % kAccStages;
+      const uint32_t aph = (i / kAccStages) & 1u;
+      const bool w = ptx::mbar_wait(bar_tfull + 8 * as, aph, limit, abort_flag);
+      if (!__all_sync(0xffffffffu, w)) {
+        if (lane == 0) report_error(kErrExpEpilogueWait, i, abort_flag);
+        break;
+      }
+      ptx::tc_fence_after_sync();
+      const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * kAccCols;
+      // this warp's 32 rows of the tile, and how many of them exist
+      const int in_tile = static_cast<int>(rank) * kBlockM + q * 32;
+      int valid = (kWgrad ? p.M - un.m : un.rows) - in_tile;
+      valid = valid < 0 ? 0 : (valid > 32 ? 32 : valid);
+      const bool empty_sum = kWgrad && un.rows == 0;
+      auto hand_back = [&]() {
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(tempty + 8 * as);
+      };
+      if (valid == 0) {
+        hand_back();
+        continue;
+      }
+      const int64_t grow = un.row + in_tile;       // forward forms: first row in the row tensors
+      const int chunks = tile_cols / 64;
+#pragma unroll 1
+      for (int c = 0; c < chunks; ++c) {
+        const int x = un.n + c * 64;
+        const bool last = c == chunks - 1;
+        // the staging buffer(s) of this chunk
+        uint32_t buf = buf0;
+        if constexpr (kForm == EXP_SAVE16 || kForm == EXP_SAVE8) {
+          if (lane == 0) ptx::bulk_wait_group_read<0>();
+        } else {
+          if (lane == 0) ptx::bulk_wait_group_read<1>();
+          buf = buf0 + (stores & 1) * kChunkBytes;
+        }
+        ++stores;
+        __syncwarp();
+        uint32_t up_scales = 0, gate_scales = 0;
+        if (x < p.N) {
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const int col = c * 64 + half * 32;
+            float v0[32];
+            ptx::tmem_ld_32x32b_x32(t_row + col, v0);
+            if constexpr (kSwiglu) {
+              float gate[32];
+              ptx::tmem_ld_32x32b_x32(t_row + gate_col + col, gate);
+              ptx::tmem_ld_wait();
+              if constexpr (kForm == EXP_SAVE16) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  const uint32_t off =
+                      row_off + ((static_cast<uint32_t>(half * 4 + j) ^ row_sw) << 4);
+                  st_shared_v4(buf + kChunkBytes + off, pack_bf16x2(v0[8 * j], v0[8 * j + 1]),
+                               pack_bf16x2(v0[8 * j + 2], v0[8 * j + 3]),
+                               pack_bf16x2(v0[8 * j + 4], v0[8 * j + 5]),
+                               pack_bf16x2(v0[8 * j + 6], v0[8 * j + 7]));
+                  st_shared_v4(buf + 2 * kChunkBytes + off,
+                               pack_bf16x2(gate[8 * j], gate[8 * j + 1]),
+                               pack_bf16x2(gate[8 * j + 2], gate[8 * j + 3]),
+                               pack_bf16x2(gate[8 * j + 4], gate[8 * j + 5]),
+                               pack_bf16x2(gate[8 * j + 6], gate[8 * j + 7]));
+                }
+              }
+              if constexpr (kForm == EXP_SAVE8) {
+                // columns at and past N hold sums over nothing (the operand reads as zero
+                // there, or as the gate half's weights): they do not belong to a block
+                const int n_left = p.N - (x + half * 32);
+                if (n_left < 32) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) {
+                    v0[j] = j < n_left ? v0[j] : 0.f;
+                    gate[j] = j < n_left ? gate[j] : 0.f;
+                  }
+                }
+                const uint32_t off64 = static_cast<uint32_t>(lane) * 64u;
+                const uint32_t sw64 = (static_cast<uint32_t>(lane) >> 1) & 3u;
+                uint32_t codes[8];
+                up_scales |= static_cast<uint32_t>(round_block_e4m3(v0, codes)) << (8 * half);
+                st_shared_v4(buf + kChunkBytes + off64 + (((half * 2) ^ sw64) << 4), codes[0],
+                             codes[1], codes[2], codes[3]);
+                st_shared_v4(buf + kChunkBytes + off64 + (((half * 2 + 1) ^ sw64) << 4), codes[4],
+                             codes[5], codes[6], codes[7]);
+                gate_scales |= static_cast<uint32_t>(round_block_e4m3(gate, codes)) << (8 * half);
+                const uint32_t gbuf = buf + kChunkBytes + kChunkBytes / 2;
+                st_shared_v4(gbuf + off64 + (((half * 2) ^ sw64) << 4), codes[0], codes[1],
+                             codes[2], codes[3]);
+                st_shared_v4(gbuf + off64 + (((half * 2 + 1) ^ sw64) << 4), codes[4], codes[5],
+                             codes[6], codes[7]);
+              }
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v0[j] = silu_mul(gate[j], v0[j]);
+            } else {
+              ptx::tmem_ld_wait();
+              if constexpr (kWgrad) {
+                if (empty_sum) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) v0[j] = 0.f;
+                }
+              }
+            }
+            if (last && half == 1) hand_back();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              st_shared_v4(buf + row_off + ((static_cast<uint32_t>(half * 4 + j) ^ row_sw) << 4),
+                           pack_bf16x2(v0[8 * j], v0[8 * j + 1]),
+                           pack_bf16x2(v0[8 * j + 2], v0[8 * j + 3]),
+                           pack_bf16x2(v0[8 * j + 4], v0[8 * j + 5]),
+                           pack_bf16x2(v0[8 * j + 6], v0[8 * j + 7]));
+            }
+          }
+        } else if (last) {
+          hand_back();
+        }
+        if constexpr (kForm == EXP_SAVE8) {
+          if (x < p.N && lane < valid) {
+            // two scale bytes of this row for each half (the pitch has room for a whole chunk)
+            uint8_t* at = p.scales + (grow + lane) * p.ld_scales + (x >> 5);
+            *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(up_scales);
+            *reinterpret_cast<uint16_t*>(at + p.gate_scale_off) =
+                static_cast<uint16_t>(gate_scales);
+          }
+        }
+        if (kWgrad || valid == 32) {
+          ptx::fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            if (x < p.N) {
+              if constexpr (kWgrad) {
+                tma_store_3d(&maps.out, x, un.m + in_tile, un.e, buf, pol_out);
+              } else {
+                const int y = static_cast<int>(grow);
+                ptx::tma_store_2d(&maps.out, x, y, buf, pol_out);
+                if constexpr (kForm == EXP_SAVE16) {
+                  ptx::tma_store_2d(&maps.up, x, y, buf + kChunkBytes, pol_out);
+                  ptx::tma_store_2d(&maps.gate, x, y, buf + 2 * kChunkBytes, pol_out);
+                }
+                if constexpr (kForm == EXP_SAVE8) {
+                  ptx::tma_store_2d(&maps.up, x, y, buf + kChunkBytes, pol_out);
+                  ptx::tma_store_2d(&maps.gate, x, y, buf + kChunkBytes + kChunkBytes / 2, pol_out);
+                }
+              }
+            }
+            ptx::bulk_commit_group();
+          }
+        } else {
+          // the group ends inside this warp's rows: store the rows it has, and no other
+          __syncwarp();
+          if (x < p.N) {
+            const int cols = p.N - x < 64 ? p.N - x : 64;
+            copy_rows<128>(buf, reinterpret_cast<uint8_t*>(p.out + grow * p.ld_out + x),
+                           p.ld_out * 2, valid, cols * 2, lane);
+            if constexpr (kForm == EXP_SAVE16) {
+              uint8_t* at = p.pre + grow * p.ld_pre + x * 2;
+              copy_rows<128>(buf + kChunkBytes, at, p.ld_pre, valid, cols * 2, lane);
+              copy_rows<128>(buf + 2 * kChunkBytes, at + p.gate_off, p.ld_pre, valid, cols * 2,
+                             lane);
+            }
+            if constexpr (kForm == EXP_SAVE8) {
+              uint8_t* at = p.pre + grow * p.ld_pre + x;
+              copy_rows<64>(buf + kChunkBytes, at, p.ld_pre, valid, cols, lane);
+              copy_rows<64>(buf + kChunkBytes + kChunkBytes / 2, at + p.gate_off, p.ld_pre, valid,
+                            cols, lane);
+            }
+          }
+          __syncwarp();
+          if (lane == 0) ptx::bulk_commit_group();    // keeps the buffers' turn-taking in step
+        }
+      }
+    }
+    if (lane == 0) ptx::bulk_wait_group_read<0>();
+  }
+
+  // ---- teardown ----
+  __syncwarp();
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (kCtaGroup == 2) ptx::cluster_sync();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc<kCtaGroup>(tmem_base, kTmemCols);
+  }
+}
+
+}  // namespace sgl

@@ -23,8 +23,11 @@
 #include <cuda_runtime.h>
 #include <nvtx3/nvToolsExt.h>   // header-only; a no-op unless a profiler is attached
 
+#include "experts_order.cuh"
+#include "experts_products.cuh"
 #include "swiglu_elementwise.cuh"
 #include "swiglu_kernel.cuh"
+#include "swiglu_preact.cuh"
 
 namespace {
 
@@ -1691,5 +1694,6 @@ int sgl_version(void) { return 100; }
 
 }  // extern "C"
 
+#include "experts_abi.cuh"
 #include "swiglu_host_pipeline.cuh"
 #include "swiglu_mgpu.cuh"

@@ -1,0 +1,536 @@
+"""Mixture-of-experts operators around the SwiGLU stage.
+
+A router gives every token ``k`` experts (``expert_ids[T, k]``) and weights (``weights[T, k]``);
+expert ``e`` owns ``W[e] = [W_up | W_gate]`` (``[K, 2N]``) and ``W_down[e]`` (``[N, D]``).
+
+``expert_order``          token slots sorted by expert (stable; ids outside ``[0, E)`` are dropped)
+``expert_dispatch``       rows of ``x`` copied to their experts' row groups
+``expert_combine``        rows summed back to tokens with the routing weights (without weights:
+                          the gradient of ``expert_dispatch``)
+``expert_combine_grad``   gradients of the weighted sum, for the rows and for the weights
+``grouped_fused_swiglu``  the gate/up stage over row groups (``_save`` keeps the pre-activations)
+``grouped_matmul``        the down projection over row groups, and its transposed form
+``grouped_weight_grad``   ``a_e^T @ g_e`` for every expert
+``experts_swiglu``        all of the forward in one call, for inference
+``swiglu_grad_preact_saved``  the backward's elementwise step from saved pre-activations
+
+The conventions are those of the other operators: bf16 tensors with unit column stride and 16-byte
+rows, checks before anything is launched, torch's current stream unless ``stream=`` is given,
+``out=`` for caller-owned results, no CPU path.  The row counts of the groups live on the device
+(``offsets``): no call here waits for the GPU.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple
+
+import torch
+
+from . import _lib
+from .ops import (DTYPE, _check_matrix, _ld, _on_device, _prep_out, _same_device, _stream_handle,
+                  stream_context)
+
+MAX_EXPERTS = 1024
+MAX_CHOICES = 64
+
+
+class ExpertOrder(NamedTuple):
+    """``offsets[E + 1]``: first row of every expert, then the number of kept slots;
+    ``slots[T * k]``: the slot ``t * k + j`` each row holds (-1 behind ``offsets[E]``);
+    ``rows[T, k]``: the row of each slot (-1 if dropped).  All int32, on the device."""
+
+    offsets: torch.Tensor
+    slots: torch.Tensor
+    rows: torch.Tensor
+
+
+class SavedPreact(NamedTuple):
+    """Pre-activations ``[up | gate]`` kept for the backward pass.  ``data``: bf16 values
+    (``bits == 16``) or e4m3 codes as uint8 (``bits == 8``), ``[rows, 2, padded columns]``;
+    ``scales``: for 8 bits the exponents + 127 of the blocks of 32 columns,
+    ``[rows, 2, blocks (even)]`` uint8.  ``hidden`` is the number of columns of either half."""
+
+    data: torch.Tensor
+    scales: torch.Tensor | None
+    bits: int
+    hidden: int
+
+
+_CHECKPOINT_BITS = {"bf16": 16, "e4m3": 8}
+
+
+def _checkpoint_bits(checkpoint: str) -> int:
+    if checkpoint not in _CHECKPOINT_BITS:
+        raise ValueError(f"checkpoint must be 'bf16' or 'e4m3', got {checkpoint!r}")
+    return _CHECKPOINT_BITS[checkpoint]
+
+
+def _check_choices(t: torch.Tensor, name: str, dtypes) -> None:
+    """A [T, k] tensor of the router, any row pitch."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must be [tokens, choices], got shape {tuple(t.shape)}")
+    if t.dtype not in dtypes:
+        raise TypeError(f"{name} must be one of {', '.join(map(str, dtypes))}, got {t.dtype}")
+    T, k = t.shape
+    if not 1 <= k <= MAX_CHOICES:
+        raise ValueError(f"{name} has {k} choices per token; 1 to {MAX_CHOICES} are supported")
+    if k > 1 and t.stride(1) != 1:
+        raise ValueError(f"{name} must have unit stride along the choices, got {t.stride()}")
+    if T > 1 and t.stride(0) < k:
+        raise ValueError(f"{name} has overlapping rows: strides {t.stride()}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
+
+
+def _choice_ld(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _check_experts(w: torch.Tensor, name: str) -> None:
+    if not isinstance(w, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(w).__name__}")
+    if w.dim() != 3:
+        raise ValueError(f"{name} must be [experts, rows, columns], got shape {tuple(w.shape)}")
+    if w.dtype != DTYPE:
+        raise TypeError(f"{name} must be torch.bfloat16, got {w.dtype}")
+    if not w.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
+    E, r, c = w.shape
+    if not 1 <= E <= MAX_EXPERTS or r < 1 or c < 1:
+        raise ValueError(f"{name} of shape {tuple(w.shape)}: 1 to {MAX_EXPERTS} experts with "
+                         "non-empty matrices are supported")
+    s0, s1, s2 = w.stride()
+    if s2 != 1 or (r > 1 and (s1 < c or s1 % 8)):
+        raise ValueError(f"{name} must be row-major with a row stride that is a multiple of 8, "
+                         f"got strides {(s0, s1, s2)}")
+    if E > 1 and (s0 % 8 or s0 < (r - 1) * s1 + c):
+        raise ValueError(f"{name}: the experts' matrices overlap or are not 16-byte apart: strides "
+                         f"{(s0, s1, s2)}")
+    if w.data_ptr() % 16 != 0:
+        raise ValueError(f"{name} must be 16-byte aligned")
+
+
+def _expert_ld(w: torch.Tensor) -> int:
+    return w.stride(1) if w.shape[1] > 1 else (w.shape[2] + 7) // 8 * 8
+
+
+def _check_ints(t: torch.Tensor, name: str, shape: tuple) -> None:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.dtype != torch.int32:
+        raise TypeError(f"{name} must be torch.int32, got {t.dtype}")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {shape}, got {tuple(t.shape)}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _check_order_rows(order: ExpertOrder) -> tuple[int, int]:
+    if not isinstance(order, ExpertOrder):
+        raise TypeError(f"order must be an ExpertOrder, got {type(order).__name__}")
+    if not isinstance(order.rows, torch.Tensor) or order.rows.dim() != 2:
+        raise ValueError("order.rows must be a [tokens, choices] tensor")
+    T, k = order.rows.shape
+    _check_ints(order.rows, "order.rows", (T, k))
+    if not 1 <= k <= MAX_CHOICES:
+        raise ValueError(f"order.rows has {k} choices per token; 1 to {MAX_CHOICES} are supported")
+    return T, k
+
+
+def _multiple_of_8(**sizes: int) -> None:
+    for name, n in sizes.items():
+        if n % 8:
+            raise ValueError(f"{name}={n} must be a multiple of 8")
+
+
+def expert_order(expert_ids, num_experts: int, *, stream=None) -> ExpertOrder:
+    """Sorts the slots of ``expert_ids[T, k]`` (int32 or int64) by expert, slot order kept inside
+    an expert.  Slots with an id outside ``[0, num_experts)`` are dropped."""
+    _check_choices(expert_ids, "expert_ids", (torch.int32, torch.int64))
+    T, k = expert_ids.shape
+    E = int(num_experts)
+    if not 1 <= E <= MAX_EXPERTS:
+        raise ValueError(f"num_experts={E} outside [1, {MAX_EXPERTS}]")
+    dev = expert_ids.device
+    with stream_context(stream, dev):
+        buf = torch.empty(E + 1 + 2 * T * k, dtype=torch.int32, device=dev)
+        offsets, slots, rows = buf.split((E + 1, T * k, T * k))
+        if T == 0:
+            offsets.zero_()
+            return ExpertOrder(offsets, slots, rows.view(0, k))
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_expert_order(
+            expert_ids.data_ptr(), int(expert_ids.dtype == torch.int64), T, k,
+            _choice_ld(expert_ids), E, offsets.data_ptr(), slots.data_ptr(), rows.data_ptr(),
+            _stream_handle(stream, dev)))
+    return ExpertOrder(offsets, slots, rows.view(T, k))
+
+
+def expert_dispatch(x, order: ExpertOrder, *, out=None, stream=None):
+    """``out[order.rows[t, j]] = x[t]``: ``[T, D]`` -> ``[T * k, D]``, rows grouped by expert.  Rows
+    behind the last expert's (there are some if slots were dropped) are left as they were."""
+    T, k = _check_order_rows(order)
+    _check_matrix(x, "x", allow_empty_rows=True)
+    if x.shape[0] != T:
+        raise ValueError(f"x has {x.shape[0]} rows, the order {T} tokens")
+    D = x.shape[1]
+    _multiple_of_8(D=D)
+    dev = _same_device(("x", x), ("order.rows", order.rows))
+    if T == 0:
+        return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
+    with stream_context(stream, dev):
+        o = _prep_out(out, T * k, D, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_expert_dispatch(
+            x.data_ptr(), order.rows.data_ptr(), o.data_ptr(), T, k, D, T * k, _ld(x), _ld(o),
+            _stream_handle(stream, dev)))
+    return o
+
+
+def _check_weights(weights, T: int, k: int) -> None:
+    _check_choices(weights, "weights", (torch.float32, torch.bfloat16))
+    if tuple(weights.shape) != (T, k):
+        raise ValueError(f"weights shape {tuple(weights.shape)} != {(T, k)}")
+
+
+def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=None):
+    """``out[t] = sum_j weights[t, j] * rows[order.rows[t, j]]``: ``[T * k, D]`` -> ``[T, D]``, fp32
+    sums in the order of ``j``.  ``weights`` is fp32 or bf16 ``[T, k]``; without weights the rows
+    are summed as they are.  Dropped slots add nothing."""
+    T, k = _check_order_rows(order)
+    _check_matrix(rows, "rows", allow_empty_rows=True)
+    if rows.shape[0] != T * k:
+        raise ValueError(f"rows has {rows.shape[0]} rows, the order {T * k} slots")
+    D = rows.shape[1]
+    _multiple_of_8(D=D)
+    named = [("rows", rows), ("order.rows", order.rows)]
+    if weights is not None:
+        _check_weights(weights, T, k)
+        named.append(("weights", weights))
+    dev = _same_device(*named)
+    if T == 0:
+        return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
+    with stream_context(stream, dev):
+        o = _prep_out(out, T, D, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_expert_combine(
+            rows.data_ptr(), order.rows.data_ptr(),
+            weights.data_ptr() if weights is not None else None,
+            int(weights is not None and weights.dtype == DTYPE), o.data_ptr(), T, k, D, T * k,
+            _ld(rows), _choice_ld(weights) if weights is not None else 0, _ld(o),
+            _stream_handle(stream, dev)))
+    return o
+
+
+def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, out=None, stream=None):
+    """Gradients of ``expert_combine(rows, order, weights)``: ``(grad_rows, grad_weights)`` with
+    ``grad_rows[r] = weight * grad_out[t]`` (rows behind the last expert's are left as they were)
+    and ``grad_weights[t, j] = <grad_out[t], rows[r]>`` in the weights' type, 0 for dropped slots.
+    ``out`` takes ``grad_rows``; it may be ``rows`` itself.  With ``rows=None`` only ``grad_rows`` is
+    computed (``grad_weights`` is None)."""
+    T, k = _check_order_rows(order)
+    _check_matrix(grad_out, "grad_out", allow_empty_rows=True)
+    D = grad_out.shape[1]
+    named = [("grad_out", grad_out), ("order.rows", order.rows), ("weights", weights)]
+    if rows is not None:
+        _check_matrix(rows, "rows", allow_empty_rows=True)
+        named.append(("rows", rows))
+    if grad_out.shape[0] != T or (rows is not None and tuple(rows.shape) != (T * k, D)):
+        raise ValueError(f"grad_out {tuple(grad_out.shape)} and rows "
+                         f"{tuple(rows.shape) if rows is not None else None} do not fit {T} tokens "
+                         f"of {k} choices")
+    _multiple_of_8(D=D)
+    _check_weights(weights, T, k)
+    dev = _same_device(*named)
+    with stream_context(stream, dev):
+        gw = torch.empty((T, k), dtype=weights.dtype, device=dev) if rows is not None else None
+        if T == 0:
+            return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev), gw
+        gr = _prep_out(out, T * k, D, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_expert_combine_grad(
+            grad_out.data_ptr(), rows.data_ptr() if rows is not None else None,
+            order.rows.data_ptr(), weights.data_ptr(), int(weights.dtype == DTYPE), gr.data_ptr(),
+            gw.data_ptr() if gw is not None else None, T, k, D, T * k, _ld(grad_out),
+            _ld(rows) if rows is not None else D, _choice_ld(weights), _ld(gr),
+            _stream_handle(stream, dev)))
+    return gr, gw
+
+
+def _swiglu_operands(x, W, offsets):
+    """Checks and sizes of the grouped gate/up stage: (R, K, N, E, device)."""
+    _check_matrix(x, "x", allow_empty_rows=True)
+    _check_experts(W, "W")
+    R, K = x.shape
+    E, K2, N2 = W.shape
+    if K2 != K:
+        raise ValueError(f"K mismatch: x.K={K} vs W.K={K2}")
+    if N2 % 2:
+        raise ValueError(f"W's last dim ({N2}) must be even")
+    _multiple_of_8(K=K, N=N2 // 2)
+    _check_ints(offsets, "offsets", (E + 1,))
+    return R, K, N2 // 2, E, _same_device(("x", x), ("W", W), ("offsets", offsets))
+
+
+def grouped_fused_swiglu(x, W, offsets, *, out=None, stream=None):
+    """``h[r] = silu(x[r] @ W_gate[e]) * (x[r] @ W_up[e])`` for the rows ``[offsets[e],
+    offsets[e + 1])`` of every expert.
+
+    x       : [R, K] bf16
+    W       : [E, K, 2N] bf16, ``[W_up | W_gate]`` per expert
+    offsets : [E + 1] int32 on the device, non-decreasing
+    returns : [R, N] bf16; rows behind ``offsets[E]`` are left as they were
+    """
+    R, K, N, E, dev = _swiglu_operands(x, W, offsets)
+    if R == 0:
+        return out if out is not None else torch.empty((0, N), dtype=DTYPE, device=dev)
+    with stream_context(stream, dev):
+        h = _prep_out(out, R, N, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_grouped_fused_swiglu(
+            x.data_ptr(), W.data_ptr(), offsets.data_ptr(), h.data_ptr(), R, N, K, E, _ld(x),
+            _expert_ld(W), W.stride(0), _ld(h), _stream_handle(stream, dev)))
+    return h
+
+
+def _preact_shapes(bits: int, rows: int, N: int):
+    """Shapes of ``SavedPreact.data`` and ``.scales`` (None for 16 bits)."""
+    pitch, scale_pitch = C.c_int64(), C.c_int64()
+    n = _lib.load().sgl_preact_bytes(bits, rows, N, C.byref(pitch), None, C.byref(scale_pitch))
+    if n < 0:
+        _lib.check(int(n))
+    return ((rows, 2, pitch.value // (2 * bits // 8)),
+            (rows, 2, scale_pitch.value // 2) if bits == 8 else None)
+
+
+def _empty_preact(bits: int, rows: int, N: int, dev) -> SavedPreact:
+    shape, scale_shape = _preact_shapes(bits, rows, N)
+    data = torch.empty(shape, dtype=torch.uint8 if bits == 8 else DTYPE, device=dev)
+    scales = torch.empty(scale_shape, dtype=torch.uint8, device=dev) if bits == 8 else None
+    return SavedPreact(data, scales, bits, N)
+
+
+def _check_preact(p: SavedPreact) -> None:
+    if p.bits not in (8, 16):
+        raise ValueError(f"preact.bits must be 8 or 16, got {p.bits}")
+    shape, scale_shape = _preact_shapes(p.bits, p.data.shape[0], p.hidden)
+    for name, t, want, dtype in (("data", p.data, shape, torch.uint8 if p.bits == 8 else DTYPE),
+                                 ("scales", p.scales, scale_shape, torch.uint8)):
+        if want is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != want \
+                or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"preact.{name} must be a contiguous {dtype} CUDA tensor of shape {want}")
+
+
+def _save(x, w_ptr, offsets, E, ldw, w_stride, R, K, N, bits, out, stream, dev):
+    with stream_context(stream, dev):
+        h = _prep_out(out, R, N, dev) if R else torch.empty((0, N), dtype=DTYPE, device=dev)
+        pre = _empty_preact(bits, R, N, dev)
+    if R:
+        with _on_device(dev):
+            _lib.check(_lib.load().sgl_grouped_fused_swiglu_save(
+                x.data_ptr(), w_ptr, offsets.data_ptr() if offsets is not None else None,
+                h.data_ptr(), pre.data.data_ptr(),
+                pre.scales.data_ptr() if pre.scales is not None else None, bits, R, N, K, E, _ld(x),
+                ldw, w_stride, _ld(h), _stream_handle(stream, dev)))
+    return h, pre
+
+
+def grouped_fused_swiglu_save(x, W, offsets, *, checkpoint: str = "bf16", out=None, stream=None):
+    """Training form of ``grouped_fused_swiglu``: ``(h, SavedPreact)``.  ``checkpoint="e4m3"`` keeps
+    the pre-activations in 8 bits (a power-of-two scale per row and 32 columns), ``"bf16"`` in 16."""
+    bits = _checkpoint_bits(checkpoint)
+    R, K, N, E, dev = _swiglu_operands(x, W, offsets)
+    return _save(x, W.data_ptr(), offsets, E, _expert_ld(W), W.stride(0), R, K, N, bits, out, stream,
+                 dev)
+
+
+def matmul_fused_swiglu_save_preact(A, W, *, checkpoint: str = "e4m3", out=None, stream=None):
+    """``matmul_fused_swiglu`` for training with an 8-bit checkpoint: ``(h, SavedPreact)``.
+
+    A : [M, K] bf16, W : [K, 2N] bf16 = [W_up | W_gate].  The checkpoint takes ``2N + N/16`` bytes
+    per row (``"bf16"``: ``4N``); ``matmul_fused_swiglu_save_factors`` keeps two bf16 factors."""
+    bits = _checkpoint_bits(checkpoint)
+    _check_matrix(A, "A", allow_empty_rows=True)
+    _check_matrix(W, "W")
+    M, K = A.shape
+    K2, N2 = W.shape
+    if K != K2:
+        raise ValueError(f"K mismatch: A.K={K} vs W.K={K2}")
+    if N2 % 2:
+        raise ValueError(f"W's 2nd dim ({N2}) must be even")
+    _multiple_of_8(K=K, N=N2 // 2)
+    dev = _same_device(("A", A), ("W", W))
+    return _save(A, W.data_ptr(), None, 1, _ld(W), 0, M, K, N2 // 2, bits, out, stream, dev)
+
+
+def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h: bool = False,
+                             out=None, stream=None):
+    """Backward elementwise step from saved pre-activations: ``[dy * silu(gate) |
+    dy * up * silu'(gate)]``, ``[R, 2N]``; with ``return_h`` also ``h = silu(gate) * up``.  With
+    ``offsets`` (of the experts' row groups) rows behind ``offsets[-1]`` are left as they were."""
+    if not isinstance(preact, SavedPreact):
+        raise TypeError(f"preact must be a SavedPreact, got {type(preact).__name__}")
+    _check_matrix(dy, "dy", allow_empty_rows=True)
+    R, N = dy.shape
+    _multiple_of_8(N=N)
+    if preact.hidden != N or preact.data.shape[0] != R:
+        raise ValueError(f"dy shape {tuple(dy.shape)} does not fit the saved pre-activations of "
+                         f"{preact.data.shape[0]} rows and {preact.hidden} columns")
+    _check_preact(preact)
+    named = [("dy", dy), ("preact.data", preact.data)]
+    if preact.scales is not None:
+        named.append(("preact.scales", preact.scales))
+    if offsets is not None:
+        if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or offsets.numel() < 1:
+            raise ValueError("offsets must be a 1-D tensor")
+        _check_ints(offsets, "offsets", (offsets.numel(),))
+        named.append(("offsets", offsets))
+    dev = _same_device(*named)
+    with stream_context(stream, dev):
+        h = torch.empty((R, N), dtype=DTYPE, device=dev) if return_h else None
+        if R == 0:
+            g = out if out is not None else torch.empty((0, 2 * N), dtype=DTYPE, device=dev)
+            return (g, h) if return_h else g
+        g = _prep_out(out, R, 2 * N, dev)
+    end = offsets.data_ptr() + 4 * (offsets.numel() - 1) if offsets is not None else None
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_swiglu_grad_preact_saved(
+            dy.data_ptr(), preact.data.data_ptr(),
+            preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
+            g.data_ptr(), h.data_ptr() if h is not None else None, end, R, N, _ld(dy), _ld(g),
+            _ld(h) if h is not None else 0, _stream_handle(stream, dev)))
+    return (g, h) if return_h else g
+
+
+def grouped_matmul(a, B, offsets, *, out=None, stream=None, transpose_b: bool = False):
+    """``c[r] = a[r] @ B[e]`` for the rows of every expert: the down projection.
+
+    a : [R, K] bf16;  B : [E, K, N] bf16, or [E, N, K] with ``transpose_b`` (read in place)
+    returns [R, N] bf16; rows behind ``offsets[E]`` are left as they were
+    """
+    _check_matrix(a, "a", allow_empty_rows=True)
+    _check_experts(B, "B")
+    R, K = a.shape
+    E = B.shape[0]
+    K2, N = (B.shape[2], B.shape[1]) if transpose_b else (B.shape[1], B.shape[2])
+    if K2 != K:
+        raise ValueError(f"K mismatch: a.K={K} vs op(B).K={K2}")
+    _multiple_of_8(K=K, N=N)
+    _check_ints(offsets, "offsets", (E + 1,))
+    dev = _same_device(("a", a), ("B", B), ("offsets", offsets))
+    if R == 0:
+        return out if out is not None else torch.empty((0, N), dtype=DTYPE, device=dev)
+    with stream_context(stream, dev):
+        c = _prep_out(out, R, N, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_grouped_matmul(
+            a.data_ptr(), B.data_ptr(), offsets.data_ptr(), c.data_ptr(), R, N, K, E, _ld(a),
+            _expert_ld(B), B.stride(0), _ld(c), int(transpose_b), _stream_handle(stream, dev)))
+    return c
+
+
+def grouped_weight_grad(a, g, offsets, *, out=None, stream=None):
+    """``C[e] = a_e^T @ g_e`` over the rows of every expert: ``a [R, M]``, ``g [R, N]`` ->
+    ``[E, M, N]`` bf16 (fp32 sums; zero for an expert without rows)."""
+    _check_matrix(a, "a", allow_empty_rows=True)
+    _check_matrix(g, "g", allow_empty_rows=True)
+    R, M = a.shape
+    if g.shape[0] != R:
+        raise ValueError(f"a has {R} rows, g {g.shape[0]}")
+    N = g.shape[1]
+    _multiple_of_8(M=M, N=N)
+    if not isinstance(offsets, torch.Tensor) or offsets.dim() != 1 or \
+            not 2 <= offsets.numel() <= MAX_EXPERTS + 1:
+        raise ValueError(f"offsets must be a 1-D tensor of 2 to {MAX_EXPERTS + 1} entries")
+    E = offsets.numel() - 1
+    _check_ints(offsets, "offsets", (E + 1,))
+    dev = _same_device(("a", a), ("g", g), ("offsets", offsets))
+    with stream_context(stream, dev):
+        if out is None:
+            c = torch.empty((E, M, N), dtype=DTYPE, device=dev)
+        else:
+            c = out
+            _check_experts(c, "out")
+            if tuple(c.shape) != (E, M, N):
+                raise ValueError(f"out shape {tuple(c.shape)} != {(E, M, N)}")
+            if c.device != dev:
+                raise ValueError(f"out is on {c.device}, expected {dev}")
+        if R == 0:
+            return c.zero_()
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_grouped_weight_grad(
+            a.data_ptr(), g.data_ptr(), offsets.data_ptr(), c.data_ptr(), R, M, N, E, _ld(a), _ld(g),
+            _expert_ld(c), c.stride(0), _stream_handle(stream, dev)))
+    return c
+
+
+def experts_swiglu_workspace_bytes(T: int, k: int, E: int, D: int, N: int, D_out: int) -> int:
+    """Bytes of device memory ``experts_swiglu`` works in for these sizes."""
+    n = _lib.load().sgl_experts_swiglu_workspace_bytes(T, k, E, D, N, D_out)
+    if n < 0:
+        _lib.check(int(n))
+    return int(n)
+
+
+def _layer_operands(x, expert_ids, weights, W, W_down):
+    _check_matrix(x, "x", allow_empty_rows=True)
+    _check_choices(expert_ids, "expert_ids", (torch.int32, torch.int64))
+    T, D = x.shape
+    if expert_ids.shape[0] != T:
+        raise ValueError(f"x has {T} rows, expert_ids {expert_ids.shape[0]}")
+    k = expert_ids.shape[1]
+    _check_weights(weights, T, k)
+    _check_experts(W, "W")
+    _check_experts(W_down, "W_down")
+    E, D2, N2 = W.shape
+    if D2 != D:
+        raise ValueError(f"K mismatch: x.K={D} vs W.K={D2}")
+    if N2 % 2:
+        raise ValueError(f"W's last dim ({N2}) must be even")
+    N = N2 // 2
+    if W_down.shape[0] != E or W_down.shape[1] != N:
+        raise ValueError(f"W_down shape {tuple(W_down.shape)} does not follow W's {tuple(W.shape)}")
+    D_out = W_down.shape[2]
+    _multiple_of_8(K=D, N=N, D=D_out)
+    dev = _same_device(("x", x), ("expert_ids", expert_ids), ("weights", weights), ("W", W),
+                       ("W_down", W_down))
+    return T, k, E, D, N, D_out, dev
+
+
+def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=None, stream=None):
+    """The expert layer at inference, one library call:
+    ``y[t] = sum_j weights[t, j] * (silu(x[t] @ W_gate[e]) * (x[t] @ W_up[e])) @ W_down[e]`` with
+    ``e = expert_ids[t, j]``.
+
+    x          : [T, D] bf16
+    expert_ids : [T, k] int32 or int64; a slot outside ``[0, E)`` is dropped
+    weights    : [T, k] fp32 or bf16
+    W, W_down  : [E, D, 2N] = [W_up | W_gate], [E, N, D_out] bf16
+    workspace  : uint8 CUDA tensor of ``experts_swiglu_workspace_bytes`` bytes (allocated if omitted);
+                 calls that overlap on the GPU must not share one
+    returns    : [T, D_out] bf16
+    """
+    T, k, E, D, N, D_out, dev = _layer_operands(x, expert_ids, weights, W, W_down)
+    if T == 0:
+        return out if out is not None else torch.empty((0, D_out), dtype=DTYPE, device=dev)
+    need = experts_swiglu_workspace_bytes(T, k, E, D, N, D_out)
+    with stream_context(stream, dev):
+        y = _prep_out(out, T, D_out, dev)
+        if workspace is None:
+            workspace = torch.empty(need, dtype=torch.uint8, device=dev)
+    if workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous uint8 CUDA tensor on the operands' device")
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_experts_swiglu(
+            x.data_ptr(), expert_ids.data_ptr(), int(expert_ids.dtype == torch.int64),
+            weights.data_ptr(), int(weights.dtype == DTYPE), W.data_ptr(), W_down.data_ptr(),
+            y.data_ptr(), workspace.data_ptr(), workspace.numel(), T, k, E, D, N, D_out, _ld(x),
+            _choice_ld(expert_ids), _choice_ld(weights), _expert_ld(W), W.stride(0),
+            _expert_ld(W_down), W_down.stride(0), _ld(y), _stream_handle(stream, dev)))
+    return y

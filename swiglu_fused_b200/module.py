@@ -23,7 +23,8 @@ import warnings
 
 import torch
 
-from .autograd import fused_swiglu
+from .autograd import fused_swiglu, fused_swiglu_experts
+from .experts import _checkpoint_bits, experts_swiglu
 from .ops import matmul_fused_swiglu
 from .weights import pack_swiglu_linear_weight, unpack_swiglu_linear_weight
 
@@ -37,12 +38,18 @@ class PackedSwiGLULinear(torch.nn.Module):
     constructor's tuning switches (``swiglu/triton/impls.py:3388-3408``); they are accepted,
     checked against the same sets and otherwise unused: there is one native forward/backward
     path and one parameter layout here (asking for the ``"packed"`` layout warns and
-    ``parameter_layout`` reads ``"normal"`` afterwards)."""
+    ``parameter_layout`` reads ``"normal"`` afterwards).
+
+    ``checkpoint`` (this implementation's own switch) is what the training forward keeps for the
+    backward, see ``autograd.fused_swiglu``: ``None``, ``"bf16"`` or ``"e4m3"``."""
 
     def __init__(self, in_features: int, hidden_features: int, *, block_n_half=None,
                  backward_mode: str = "save_factors_normal", parameter_layout: str = "normal",
-                 device=None, dtype=torch.bfloat16) -> None:
+                 checkpoint: str | None = None, device=None, dtype=torch.bfloat16) -> None:
         super().__init__()
+        if checkpoint is not None:
+            _checkpoint_bits(checkpoint)
+        self.checkpoint = checkpoint
         if backward_mode not in _BACKWARD_MODES:
             raise ValueError(f"unknown backward_mode {backward_mode!r}")
         if parameter_layout not in ("packed", "normal"):
@@ -129,8 +136,81 @@ class PackedSwiGLULinear(torch.nn.Module):
         if not x2.is_contiguous():
             x2 = x2.contiguous()
         needs_grad = torch.is_grad_enabled() and (x2.requires_grad or self.weight.requires_grad)
-        out = fused_swiglu(x2, self.weight) if needs_grad else matmul_fused_swiglu(x2, self.weight)
+        out = (fused_swiglu(x2, self.weight, checkpoint=self.checkpoint) if needs_grad
+               else matmul_fused_swiglu(x2, self.weight))
         return out.view(*lead, self.hidden_features)
 
     def extra_repr(self) -> str:
         return f"in_features={self.in_features}, hidden_features={self.hidden_features}"
+
+
+class PackedSwiGLUExperts(torch.nn.Module):
+    """The experts of a mixture-of-experts layer: ``num_experts`` SwiGLU feed-forward networks.
+
+    Parameters: ``weight [num_experts, in_features, 2 * hidden_features] = [W_up | W_gate]`` and
+    ``weight_down [num_experts, hidden_features, out_features]``.  ``forward(x, expert_ids, weights)``
+    takes the router's choices, ``[..., k]`` beside ``x [..., in_features]``; ids outside
+    ``[0, num_experts)`` are dropped.  With gradients the pre-activations are kept as
+    ``checkpoint`` says (``"bf16"`` or ``"e4m3"``); without, the layer is one library call."""
+
+    def __init__(self, in_features: int, hidden_features: int, num_experts: int, *,
+                 out_features: int | None = None, checkpoint: str = "bf16", device=None,
+                 dtype=torch.bfloat16) -> None:
+        super().__init__()
+        out_features = in_features if out_features is None else out_features
+        if in_features % 8 or hidden_features % 8 or out_features % 8:
+            raise ValueError("in_features, hidden_features and out_features must be multiples of 8 "
+                             f"(16-byte rows), got {in_features}, {hidden_features}, {out_features}")
+        _checkpoint_bits(checkpoint)
+        self.in_features = in_features
+        self.hidden_features = hidden_features
+        self.out_features = out_features
+        self.num_experts = num_experts
+        self.checkpoint = checkpoint
+        self.weight = torch.nn.Parameter(
+            torch.empty(num_experts, in_features, 2 * hidden_features, device=device, dtype=dtype))
+        self.weight_down = torch.nn.Parameter(
+            torch.empty(num_experts, hidden_features, out_features, device=device, dtype=dtype))
+        self.reset_parameters()
+
+    @torch.no_grad()
+    def reset_parameters(self) -> None:
+        # expert by expert what PackedSwiGLULinear draws; down: N(0, 1/hidden_features)
+        n = self.hidden_features
+        torch.nn.init.normal_(self.weight[..., :n], std=1.0 / math.sqrt(self.in_features))
+        torch.nn.init.normal_(self.weight[..., n:], std=math.sqrt(2.0 / self.in_features))
+        torch.nn.init.normal_(self.weight_down, std=1.0 / math.sqrt(n))
+
+    @torch.no_grad()
+    def load_expert_(self, expert: int, gate_up: torch.Tensor, down: torch.Tensor) -> None:
+        """Copies one expert from ``nn.Linear`` layout: ``gate_up [2 * hidden_features, in_features]``
+        (rows: up, then gate) and ``down [out_features, hidden_features]``."""
+        for name, t, shape in (("gate_up", gate_up, (2 * self.hidden_features, self.in_features)),
+                               ("down", down, (self.out_features, self.hidden_features))):
+            if tuple(t.shape) != shape:
+                raise ValueError(f"expected {name} of shape {shape}, got {tuple(t.shape)}")
+        self.weight[expert].copy_(gate_up.detach().t())
+        self.weight_down[expert].copy_(down.detach().t())
+
+    def forward(self, x: torch.Tensor, expert_ids: torch.Tensor,
+                weights: torch.Tensor) -> torch.Tensor:
+        lead = x.shape[:-1]
+        if expert_ids.shape[:-1] != lead or weights.shape != expert_ids.shape:
+            raise ValueError(f"x {tuple(x.shape)}, expert_ids {tuple(expert_ids.shape)} and weights "
+                             f"{tuple(weights.shape)} do not belong together")
+        x2 = x.reshape(-1, x.shape[-1]).contiguous()
+        ids = expert_ids.reshape(-1, expert_ids.shape[-1]).contiguous()
+        rw = weights.reshape(-1, weights.shape[-1]).contiguous()
+        needs_grad = torch.is_grad_enabled() and any(
+            t.requires_grad for t in (x2, rw, self.weight, self.weight_down))
+        if needs_grad:
+            y = fused_swiglu_experts(x2, ids, rw, self.weight, self.weight_down,
+                                     checkpoint=self.checkpoint)
+        else:
+            y = experts_swiglu(x2, ids, rw, self.weight, self.weight_down)
+        return y.view(*lead, self.out_features)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, hidden_features={self.hidden_features}, "
+                f"out_features={self.out_features}, num_experts={self.num_experts}, "
+                f"checkpoint={self.checkpoint!r}")

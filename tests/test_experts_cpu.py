@@ -1,0 +1,152 @@
+"""Refusals and host arithmetic of the mixture-of-experts operators, without a GPU."""
+import ctypes as C
+
+import pytest
+import torch
+
+import experts_reference as ref
+import swiglu_fused_b200 as sg
+from swiglu_fused_b200 import _lib, experts
+
+BUF = (C.c_uint8 * 4096)()
+P = (C.addressof(BUF) + 15) // 16 * 16
+BF16 = torch.bfloat16
+
+
+def call(fn, code, needle, *args):
+    lib = _lib.load()
+    assert getattr(lib, fn)(*args) == code
+    assert needle in lib.sgl_last_error().decode()
+
+
+@pytest.mark.parametrize("change,code,needle", [
+    (dict(ids=0), -1, "ids is NULL"), (dict(ids=P + 4), -4, "8-byte"), (dict(T=0), -2, "T=0"),
+    (dict(k=0), -2, "k=0"), (dict(k=65, ld=65), -2, "k=65"), (dict(E=0), -2, "E=0"),
+    (dict(E=1025), -2, "E=1025"), (dict(T=2 ** 31), -2, "31 bits"), (dict(ld=1), -3, "ld_ids"),
+    (dict(offsets=0), -1, "offsets"), (dict(slots=P + 2), -4, "slots"), (dict(rows=0), -1, "rows")])
+def test_order_refusals(change, code, needle):
+    a = dict(ids=P, T=4, k=2, ld=2, E=8, offsets=P, slots=P, rows=P) | change
+    call("sgl_expert_order", code, needle, a["ids"], 1, a["T"], a["k"], a["ld"], a["E"],
+         a["offsets"], a["slots"], a["rows"], None)
+
+
+@pytest.mark.parametrize("change,code,needle", [
+    (dict(x=0), -1, "x is NULL"), (dict(out=P + 8), -4, "16-byte"), (dict(D=12), -2, "D=12"),
+    (dict(R=0), -2, "R=0"), (dict(ldx=8), -3, "ldx"), (dict(ldo=20), -3, "ldo"),
+    (dict(rows=P + 1), -4, "rows")])
+def test_dispatch_refusals(change, code, needle):
+    a = dict(x=P, rows=P, out=P, D=16, R=8, ldx=16, ldo=16) | change
+    call("sgl_expert_dispatch", code, needle, a["x"], a["rows"], a["out"], 4, 2, a["D"], a["R"],
+         a["ldx"], a["ldo"], None)
+
+
+@pytest.mark.parametrize("change,code,needle", [
+    (dict(inp=0), -1, "in is NULL"), (dict(w=P + 2), -4, "weights"), (dict(ldw=1), -3, "ld_w"),
+    (dict(ldi=8), -3, "ld_in")])
+def test_combine_refusals(change, code, needle):
+    a = dict(inp=P, w=P, ldw=2, ldi=16) | change
+    call("sgl_expert_combine", code, needle, a["inp"], P, a["w"], 0, P, 4, 2, 16, 8, a["ldi"],
+         a["ldw"], 16, None)
+    a.setdefault("gw", P)
+    call("sgl_expert_combine_grad", code, needle, P, a["inp"], P, a["w"], 0, P, a["gw"], 4, 2, 16, 8,
+         16, a["ldi"], a["ldw"], 16, None)
+
+
+@pytest.mark.parametrize("change,code,needle", [
+    (dict(off=0), -1, "offsets"), (dict(off=P + 2), -4, "offsets"), (dict(E=1025), -2, "E=1025"),
+    (dict(R=0), -2, "R=0"), (dict(K=20), -2, "multiples of 8"), (dict(ldw=16), -3, "ldw"),
+    (dict(stride=8), -3, "w_stride"), (dict(stride=516), -3, "w_stride"), (dict(h=0), -1, "h is NULL"),
+    (dict(R=2 ** 31), -2, "2^31")])
+def test_grouped_swiglu_refusals(change, code, needle):
+    a = dict(off=P, h=P, R=10, N=16, K=16, E=2, ldx=16, ldw=32, stride=512) | change
+    a["ldx"] = a["K"] if a["K"] % 8 == 0 else 24
+    call("sgl_grouped_fused_swiglu", code, needle, P, P, a["off"], a["h"], a["R"], a["N"], a["K"],
+         a["E"], a["ldx"], a["ldw"], a["stride"], 16, None)
+    call("sgl_grouped_fused_swiglu_save", code, needle, P, P, a["off"], a["h"], P, P, 8, a["R"],
+         a["N"], a["K"], a["E"], a["ldx"], a["ldw"], a["stride"], 16, None)
+
+
+def test_other_refusals():
+    call("sgl_grouped_fused_swiglu_save", -10, "bits=4", P, P, P, P, P, P, 4, 8, 16, 16, 2, 16, 32,
+         512, 16, None)
+    call("sgl_grouped_fused_swiglu_save", -1, "scales", P, P, P, P, P, 0, 8, 8, 16, 16, 2, 16, 32,
+         512, 16, None)
+    call("sgl_grouped_matmul", -3, "ldb", P, P, P, P, 8, 16, 32, 2, 32, 16, 512, 16, 1, None)
+    call("sgl_grouped_matmul", -3, "b_stride", P, P, P, P, 8, 16, 32, 2, 32, 16, 256, 16, 0, None)
+    call("sgl_grouped_weight_grad", -3, "c_stride", P, P, P, P, 8, 16, 16, 2, 16, 16, 16, 128, None)
+    call("sgl_swiglu_grad_preact_saved", -3, "ldo", P, P, P, 8, P, None, None, 8, 16, 16, 16, 0, None)
+    call("sgl_swiglu_grad_preact_saved", -4, "end", P, P, P, 8, P, None, P + 2, 8, 16, 16, 32, 0, None)
+    call("sgl_experts_swiglu", -10, "workspace", P, P, 1, P, 0, P, P, P, P, 64, 4, 2, 8, 16, 16, 16,
+         16, 2, 2, 32, 512, 16, 256, 16, None)
+    n = _lib.load().sgl_experts_swiglu_workspace_bytes(4, 2, 8, 16, 16, 16)
+    call("sgl_experts_swiglu", -3, "ldd", P, P, 1, P, 0, P, P, P, P, n, 4, 2, 8, 16, 16, 16,
+         16, 2, 2, 32, 512, 8, 256, 16, None)
+    assert _lib.load().sgl_experts_swiglu_workspace_bytes(0, 2, 8, 16, 16, 16) == -2
+    assert _lib.load().sgl_preact_bytes(8, 4, 12, None, None, None) == -2
+
+
+def test_workspace_holds_every_part():
+    T, k, E, D, N, Do = 5, 3, 7, 24, 40, 16
+    n = sg.experts_swiglu_workspace_bytes(T, k, E, D, N, Do)
+    assert n >= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + Do)
+    assert n <= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + Do) + 6 * 256
+    with pytest.raises(ValueError):
+        sg.experts_swiglu_workspace_bytes(1, 65, E, D, N, Do)
+
+
+@pytest.mark.parametrize("N,half,scale", [(8, 32, 2), (32, 32, 2), (40, 64, 2), (72, 96, 4),
+                                          (14336, 14336, 448)])
+def test_preact_shapes(N, half, scale):
+    assert experts._preact_shapes(8, 5, N) == ((5, 2, half), (5, 2, scale))
+    assert experts._preact_shapes(16, 5, N) == ((5, 2, half), None)
+
+
+def test_python_refusals():
+    ids = torch.zeros((4, 2), dtype=torch.int64)
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.expert_order(ids, 4)
+    with pytest.raises(TypeError, match="expert_ids"):
+        sg.expert_order(ids.float(), 4)
+    with pytest.raises(ValueError, match="tokens, choices"):
+        sg.expert_order(ids.view(-1), 4)
+    with pytest.raises(ValueError, match="choices per token"):
+        sg.expert_order(torch.zeros((4, 65), dtype=torch.int64), 4)
+    order = sg.ExpertOrder(torch.zeros(5, dtype=torch.int32), torch.zeros(8, dtype=torch.int32),
+                           torch.zeros((4, 2), dtype=torch.int32))
+    x = torch.zeros((4, 16), dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.expert_dispatch(x, order)
+    with pytest.raises(TypeError, match="ExpertOrder"):
+        sg.expert_combine(x, (order.offsets, order.slots, order.rows))
+    w = torch.zeros((4, 16, 32), dtype=BF16)
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.grouped_fused_swiglu(x, w, order.offsets)
+    with pytest.raises(ValueError, match="checkpoint"):
+        sg.fused_swiglu(x, w[0], checkpoint="int8")
+    with pytest.raises(ValueError, match="checkpoint"):
+        sg.PackedSwiGLUExperts(16, 16, 4, checkpoint="fp8")
+    with pytest.raises(ValueError, match="multiples of 8"):
+        sg.PackedSwiGLUExperts(16, 12, 4)
+    with pytest.raises(TypeError, match="SavedPreact"):
+        sg.swiglu_grad_preact_saved(x, x)
+
+
+def test_module_parameters_and_expert_loading():
+    mod = sg.PackedSwiGLUExperts(16, 24, 3, out_features=8)
+    assert mod.weight.shape == (3, 16, 48) and mod.weight_down.shape == (3, 24, 8)
+    gate_up, down = torch.randn(48, 16).to(BF16), torch.randn(8, 24).to(BF16)
+    mod.load_expert_(2, gate_up, down)
+    assert torch.equal(mod.weight[2].detach(), gate_up.t())
+    assert torch.equal(mod.weight_down[2].detach(), down.t())
+    with pytest.raises(ValueError, match="gate_up"):
+        mod.load_expert_(0, gate_up.t(), down)
+    assert set(mod.state_dict()) == {"weight", "weight_down"}
+
+
+def test_reference_block_codes():
+    """The plain form itself: smallest power of two that holds the block, nearest e4m3 value."""
+    v = torch.tensor([[448.0] + [1.0] * 31, [449.0] + [0.0] * 31, [0.0] * 32])
+    codes, scales = ref.block_codes(v)
+    assert scales.view(-1).tolist() == [127, 128, 0]
+    assert codes[0, 0].item() == 0x7e and codes[0, 1].item() == 0x38
+    assert codes[1, 0].item() == 0x76              # 224.5 -> 224
