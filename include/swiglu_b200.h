@@ -516,11 +516,11 @@ int sgl_mgpu_destroy(sgl_mgpu* g);
  *   or at least every row named in `rows` (an index outside [0, R) is not followed).  Rows
  *   behind offsets[E] are left as they were.
  * sgl_expert_combine: out[t] = sum_j weights[t, j] * in[rows[t, j]], summed in fp32 in the order
- *   of j.  weights: fp32 or bf16 [T, k], row pitch ld_w, or NULL for ones (which is dispatch's
- *   gradient).  Dropped slots add nothing; a token without any gets zeros.
+ *   of j.  in: bf16, or fp32 (in_is_f32; its pitch a multiple of 8 elements too).  weights: fp32
+ *   or bf16 [T, k], row pitch ld_w, or NULL for ones (which is dispatch's gradient).  Dropped slots add nothing; a token without any gets zeros.
  * sgl_expert_combine_grad: grad_rows[rows[t, j]] = weights[t, j] * grad_out[t] (other rows are left
- *   as they were) and grad_weights[t, j] = <grad_out[t], in[rows[t, j]]> (fp32 sums, stored in the
- *   weights' type, dense [T, k]; 0 for dropped slots).  in and grad_weights may both be NULL:
+ *   as they were; weights NULL: ones) and grad_weights[t, j] = <grad_out[t], in[rows[t, j]]>
+ *   (fp32 sums, stored dense [T, k] in fp32 or, weights_bf16, bf16; 0 for dropped slots).  in and grad_weights may both be NULL:
  *   grad_rows alone.  grad_rows may be `in` itself.
  * D must be a multiple of 8; the bf16 tensors follow the conventions above.
  */
@@ -528,10 +528,10 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
                      int64_t E, void* offsets, void* slots, void* rows, void* stream);
 int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
                         int64_t R, int64_t ldx, int64_t ldo, void* stream);
-int sgl_expert_combine(const void* in, const void* rows, const void* weights, int weights_bf16,
-                       void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
+int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
+                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
                        int64_t ld_w, int64_t ldo, void* stream);
-int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* rows,
+int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32, const void* rows,
                             const void* weights, int weights_bf16, void* grad_rows,
                             void* grad_weights, int64_t T, int64_t k, int64_t D, int64_t R,
                             int64_t ld_go, int64_t ld_in, int64_t ld_w, int64_t ld_gr,
@@ -550,7 +550,14 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* ro
  *   (the smallest 2^e, e >= -127, with max|v| <= 448 * 2^e; a block that holds an infinity or
  *   a NaN reads as NaN).  `pre` takes sgl_preact_bytes() bytes, `scales` *scale_bytes (bits = 8).
  *   E = 1 with offsets == NULL is the dense stage over all R rows.
- * sgl_grouped_matmul: c[r] = a[r] @ b_e, or a[r] @ b_e^T with b_e stored [N, K] (b_transposed).
+ * sgl_grouped_matmul: c[r] = a[r] @ b_e, or a[r] @ b_e^T with b_e stored [N, K] (b_transposed);
+ *   c in bf16, or in fp32 (c_is_f32).
+ * sgl_grouped_grad_preact: the backward of the stage behind the down projection, in one launch.
+ *   With t = dy[r] @ w_down_e^T (dy[R, D], w_down_e [N, D] as in the forward) and the saved
+ *   pre-activations up, gate of row r: grad_preact[r] = [w t silu(gate) | w t up silu'(gate)]
+ *   ([R, 2N]) and h[r] = w silu(gate) up ([R, N]), w the weight of slot slots[r], weights[T, k] with
+ *   R = T * k; slots and weights NULL: w = 1.  t stays in fp32; with the weight on this side
+ *   w_down's gradient is h_e^T @ dy_e.
  * sgl_grouped_weight_grad: c[e] = a_e^T @ g_e, a[R, M], g[R, N], c[E, M, N]; an empty group's
  *   matrix is zero.  M and N are multiples of 8, the groups' row counts are arbitrary.
  */
@@ -563,7 +570,13 @@ int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offs
                                   int64_t ldh, void* stream);
 int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
                        int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
-                       int64_t ldc, int b_transposed, void* stream);
+                       int64_t ldc, int b_transposed, int c_is_f32, void* stream);
+int sgl_grouped_grad_preact(const void* dy, const void* w_down, const void* offsets,
+                            const void* slots, const void* weights, int weights_bf16,
+                            const void* pre, const void* scales, int bits, void* grad_preact,
+                            void* h, int64_t R, int64_t N, int64_t D, int64_t E, int64_t k,
+                            int64_t lddy, int64_t ldw, int64_t w_stride, int64_t ld_weights,
+                            int64_t ld_grad, int64_t ldh, void* stream);
 int sgl_grouped_weight_grad(const void* a, const void* g, const void* offsets, void* c, int64_t R,
                             int64_t M, int64_t N, int64_t E, int64_t lda, int64_t ldg, int64_t ldc,
                             int64_t c_stride, void* stream);

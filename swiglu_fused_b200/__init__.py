@@ -12,8 +12,8 @@ from ._lib import TileConfig, SglError
 from .autograd import fused_swiglu, fused_swiglu_experts
 from .experts import (ExpertOrder, SavedPreact, expert_combine, expert_combine_grad, expert_dispatch,
                       expert_order, experts_swiglu, experts_swiglu_workspace_bytes,
-                      grouped_fused_swiglu, grouped_fused_swiglu_save, grouped_matmul,
-                      grouped_weight_grad, matmul_fused_swiglu_save_preact,
+                      grouped_fused_swiglu, grouped_fused_swiglu_save, grouped_grad_preact,
+                      grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
                       swiglu_grad_preact_saved)
 from .module import PackedSwiGLUExperts, PackedSwiGLULinear
 from .ops import (matmul_bf16, matmul_fused_swiglu, matmul_silu_mul, tune_matmul_fused_swiglu,
@@ -34,6 +34,7 @@ __all__ = [
     "grouped_fused_swiglu",
     "grouped_fused_swiglu_save",
     "grouped_matmul",
+    "grouped_grad_preact",
     "grouped_weight_grad",
     "experts_swiglu",
     "experts_swiglu_workspace_bytes",

@@ -82,6 +82,7 @@ EXPORTED_SYMBOLS = (
     "sgl_grouped_fused_swiglu",
     "sgl_grouped_fused_swiglu_save",
     "sgl_grouped_matmul",
+    "sgl_grouped_grad_preact",
     "sgl_grouped_weight_grad",
     "sgl_preact_bytes",
     "sgl_swiglu_grad_preact_saved",
@@ -284,15 +285,17 @@ def load() -> C.CDLL:
         lib.sgl_expert_dispatch.restype = ip
         lib.sgl_expert_dispatch.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]
         lib.sgl_expert_combine.restype = ip
-        lib.sgl_expert_combine.argtypes = [vp, vp, vp, ip, vp] + [i64] * 7 + [vp]
+        lib.sgl_expert_combine.argtypes = [vp, ip, vp, vp, ip, vp] + [i64] * 7 + [vp]
         lib.sgl_expert_combine_grad.restype = ip
-        lib.sgl_expert_combine_grad.argtypes = [vp, vp, vp, vp, ip, vp, vp] + [i64] * 8 + [vp]
+        lib.sgl_expert_combine_grad.argtypes = [vp, vp, ip, vp, vp, ip, vp, vp] + [i64] * 8 + [vp]
         lib.sgl_grouped_fused_swiglu.restype = ip
         lib.sgl_grouped_fused_swiglu.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [vp]
         lib.sgl_grouped_fused_swiglu_save.restype = ip
         lib.sgl_grouped_fused_swiglu_save.argtypes = [vp] * 6 + [ip] + [i64] * 8 + [vp]
         lib.sgl_grouped_matmul.restype = ip
-        lib.sgl_grouped_matmul.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [ip, vp]
+        lib.sgl_grouped_matmul.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [ip, ip, vp]
+        lib.sgl_grouped_grad_preact.restype = ip
+        lib.sgl_grouped_grad_preact.argtypes = [vp] * 5 + [ip, vp, vp, ip, vp, vp] + [i64] * 11 + [vp]
         lib.sgl_grouped_weight_grad.restype = ip
         lib.sgl_grouped_weight_grad.argtypes = [vp, vp, vp, vp] + [i64] * 8 + [vp]
         lib.sgl_preact_bytes.restype = i64

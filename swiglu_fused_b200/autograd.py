@@ -13,7 +13,7 @@ import torch
 
 from .experts import (ExpertOrder, SavedPreact, _checkpoint_bits, _layer_operands, expert_combine,
                       expert_combine_grad, expert_dispatch, expert_order, grouped_fused_swiglu_save,
-                      grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
+                      grouped_grad_preact, grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
                       swiglu_grad_preact_saved)
 from .ops import matmul_bf16, matmul_fused_swiglu_save_factors, swiglu_grad_preact
 
@@ -83,14 +83,21 @@ def fused_swiglu(x: torch.Tensor, w: torch.Tensor, *, checkpoint: str | None = N
 class FusedSwiGLUExpertsFunction(torch.autograd.Function):
     """The expert layer.  Kept for the backward: the inputs, the order, the pre-activations and,
     if the routing weights need a gradient, the experts' outputs.  The grouped copy of x and h
-    are made again."""
+    are made again.
+
+    Rounding to bf16 happens where a value becomes an operand of a product (h, the pre-activations'
+    gradients) and once for each result; the experts' outputs and the rows of x's gradient, which
+    are summed over a token's choices, stay in fp32, and the routing weight is applied to fp32
+    values (``grouped_grad_preact``).  Each result then carries two roundings on its way."""
 
     @staticmethod
     def forward(ctx, x, expert_ids, weights, w, w_down, checkpoint):
         order = expert_order(expert_ids, w.shape[0])
         xs = expert_dispatch(x, order)
         h, pre = grouped_fused_swiglu_save(xs, w, order.offsets, checkpoint=checkpoint)
-        ys = grouped_matmul(h, w_down, order.offsets)
+        del xs
+        ys = grouped_matmul(h, w_down, order.offsets, out_dtype=torch.float32)
+        del h
         y = expert_combine(ys, order, weights)
         ctx.save_for_backward(x, weights, w, w_down, *order, pre.data, pre.scales,
                               ys if ctx.needs_input_grad[2] else None)
@@ -105,21 +112,22 @@ class FusedSwiGLUExpertsFunction(torch.autograd.Function):
             return (torch.zeros_like(x), None, torch.zeros_like(weights), torch.zeros_like(w),
                     torch.zeros_like(w_down), None)
         order = ExpertOrder(offsets, slots, rows)
-        grad_ys, grad_weights = expert_combine_grad(grad_y.contiguous(), ys, order, weights)
+        # the rows' gradients without the routing weights, and the weights' own
+        grad_rows, grad_weights = expert_combine_grad(grad_y.contiguous(), ys, order, weights,
+                                                      weighted=False)
         grad_x = grad_w = grad_down = None
         if need_x or need_w or need_down:
             pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
-            grad_h = grouped_matmul(grad_ys, w_down, offsets, transpose_b=True)
-            grad_preact, h = swiglu_grad_preact_saved(grad_h, pre, offsets=offsets, return_h=True)
-            del grad_h
+            grad_preact, h = grouped_grad_preact(grad_rows, w_down, pre, order, weights)
             if need_down:
-                grad_down = grouped_weight_grad(h, grad_ys, offsets)
-            del h, grad_ys
+                grad_down = grouped_weight_grad(h, grad_rows, offsets)
+            del h, grad_rows
             if need_w:
                 grad_w = grouped_weight_grad(expert_dispatch(x, order), grad_preact, offsets)
             if need_x:
-                grad_x = expert_combine(grouped_matmul(grad_preact, w, offsets, transpose_b=True),
-                                        order)
+                grad_x = expert_combine(
+                    grouped_matmul(grad_preact, w, offsets, transpose_b=True,
+                                   out_dtype=torch.float32), order)
         return grad_x, None, grad_weights if need_weights else None, grad_w, grad_down, None
 
 

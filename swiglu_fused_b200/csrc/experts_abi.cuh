@@ -22,23 +22,31 @@ ExpertVariant make_expert_variant() {
   return v;
 }
 
-constexpr int kExpertVariants = 10;   // form * 2 + (cta_group - 1)
-constexpr int kExpertBlockK = 64;
+constexpr int kExpertVariants = sgl::EXP_FORMS * 2;   // form * 2 + (cta_group - 1)
+constexpr int kExpertBlockK = 128;
+
+template <int F>
+void fill_expert_form(ExpertVariant* table) {
+  table[F * 2] = make_expert_variant<F, 1, kExpertBlockK>();
+  table[F * 2 + 1] = make_expert_variant<F, 2, kExpertBlockK>();
+}
 
 const ExpertVariant& expert_variant(int form, int cta_group) {
-  static const ExpertVariant table[kExpertVariants] = {
-      make_expert_variant<sgl::EXP_SWIGLU, 1, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_SWIGLU, 2, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_SAVE16, 1, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_SAVE16, 2, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_SAVE8, 1, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_SAVE8, 2, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_GEMM, 1, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_GEMM, 2, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_WGRAD, 1, kExpertBlockK>(),
-      make_expert_variant<sgl::EXP_WGRAD, 2, kExpertBlockK>(),
+  struct Table {
+    ExpertVariant v[kExpertVariants];
+    Table() {
+      fill_expert_form<sgl::EXP_SWIGLU>(v);
+      fill_expert_form<sgl::EXP_SAVE16>(v);
+      fill_expert_form<sgl::EXP_SAVE8>(v);
+      fill_expert_form<sgl::EXP_GEMM>(v);
+      fill_expert_form<sgl::EXP_GEMM32>(v);
+      fill_expert_form<sgl::EXP_GRAD16>(v);
+      fill_expert_form<sgl::EXP_GRAD8>(v);
+      fill_expert_form<sgl::EXP_WGRAD>(v);
+    }
   };
-  return table[form * 2 + cta_group - 1];
+  static const Table table;
+  return table.v[form * 2 + cta_group - 1];
 }
 
 struct ExpertDevice {
@@ -94,10 +102,11 @@ int prepare_expert_variant(int form, int cta_group, const DeviceInfo* info, int*
   return SGL_OK;
 }
 
-// Tensor map over bf16 (or bytes) [outer][rows][cols]; rank 2 when outer == 0.
+// Tensor map over [outer][rows][cols] elements (bf16 unless said); rank 2 when outer == 0.
 int make_expert_map(CUtensorMap* out, const void* base, int64_t cols, int64_t rows, int64_t outer,
                     int64_t ld_bytes, int64_t outer_bytes, int box_cols, int box_rows,
-                    const char* name, bool bytes = false,
+                    const char* name,
+                    CUtensorMapDataType type = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
                     CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B,
                     CUtensorMapL2promotion promo = CU_TENSOR_MAP_L2_PROMOTION_L2_256B) {
   EncodeTiledFn fn = encode_tiled_fn();
@@ -108,8 +117,7 @@ int make_expert_map(CUtensorMap* out, const void* base, int64_t cols, int64_t ro
   cuuint64_t strides[2] = {static_cast<cuuint64_t>(ld_bytes), static_cast<cuuint64_t>(outer_bytes)};
   cuuint32_t box[3] = {static_cast<cuuint32_t>(box_cols), static_cast<cuuint32_t>(box_rows), 1};
   cuuint32_t estr[3] = {1, 1, 1};
-  CUresult r = fn(out, bytes ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
-                  rank, const_cast<void*>(base), dims, strides, box, estr,
+  CUresult r = fn(out, type, rank, const_cast<void*>(base), dims, strides, box, estr,
                   CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, promo, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(SGL_ERR_TENSOR_MAP,
@@ -154,8 +162,15 @@ struct ExpertLaunch {
   int64_t R = 0, N = 0, K = 0, M = 0, E = 0;
   int64_t lda = 0, ldb = 0, b_stride = 0, ld_out = 0, out_stride = 0;
   int b_transposed = 0;
-  void* pre = nullptr;       // saved pre-activations (see preact_layout)
-  void* scales = nullptr;
+  void* pre = nullptr;       // EXP_SAVE*: pre-activations (see preact_layout); EXP_GRAD*: their
+                             // gradients, [R, 2N] bf16
+  int64_t ld_pre = 0;        // EXP_GRAD*: row pitch of the gradients, elements
+  const void* saved = nullptr;   // EXP_GRAD*: saved pre-activations
+  void* scales = nullptr;    // 8-bit forms
+  const int* slots = nullptr;    // EXP_GRAD*: the routing weight of each row, or NULL (ones)
+  const void* weights = nullptr;
+  int64_t ld_w = 0, k = 1;
+  int w_bf16 = 0;
 };
 
 // Byte layout of saved pre-activations: rows of [up | gate], each half padded to whole blocks.
@@ -178,7 +193,9 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   int rc = check_device(&info);
   if (rc) return rc;
   const bool wgrad = s.form == sgl::EXP_WGRAD;
-  const bool swiglu = s.form != sgl::EXP_GEMM && !wgrad;
+  const bool save = s.form == sgl::EXP_SAVE16 || s.form == sgl::EXP_SAVE8;
+  const bool grad = s.form == sgl::EXP_GRAD16 || s.form == sgl::EXP_GRAD8;
+  const bool swiglu = s.form == sgl::EXP_SWIGLU || save;
 
   // CTA pairs (256-row tiles) once the groups fill them on average; single CTAs (128 rows) else.
   int cta_group = 1;
@@ -205,24 +222,33 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
       acc_cols /= 2;
     }
   }
+  int a_rows = sgl::kBlockM;
+  if (cta_group == 1 && !wgrad && s.R <= 32) a_rows = static_cast<int>((s.R + 15) / 16 * 16);
+  int stages = v.max_stages(static_cast<int>(s.E), a_rows, acc_cols);
+  while (stages < 2 && acc_cols > min_cols) {   // several hundred groups: their table needs room
+    acc_cols /= 2;
+    stages = v.max_stages(static_cast<int>(s.E), a_rows, acc_cols);
+  }
   const int tile_cols = swiglu ? acc_cols / 2 : acc_cols;
   const int64_t tiles_n = (s.N + tile_cols - 1) / tile_cols;
   if (max_tiles_m * tiles_n > 0x7fffffffll) return fail(SGL_ERR_BAD_SHAPE, "too many tiles");
-  int a_rows = sgl::kBlockM;
-  if (cta_group == 1 && !wgrad && s.R < sgl::kBlockM)
-    a_rows = static_cast<int>((s.R + 15) / 16 * 16);
-  const int stages = v.max_stages(static_cast<int>(s.E), a_rows, acc_cols);
   const int smem = v.smem_bytes(static_cast<int>(s.E), a_rows, acc_cols, stages);
 
   sgl::ExpertMaps maps;
   std::memset(&maps, 0, sizeof(maps));
-  const PreactLayout pl = preact_layout(s.form == sgl::EXP_SAVE8 ? 8 : 16, s.N);
+  const int bits = s.form == sgl::EXP_SAVE8 || s.form == sgl::EXP_GRAD8 ? 8 : 16;
+  const PreactLayout pl = preact_layout(bits, s.N);
+  constexpr CUtensorMapDataType kBf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  constexpr CUtensorMapSwizzle kSw128 = CU_TENSOR_MAP_SWIZZLE_128B, kSw64 = CU_TENSOR_MAP_SWIZZLE_64B;
+  constexpr CUtensorMapL2promotion kNoPromo = CU_TENSOR_MAP_L2_PROMOTION_NONE;
+  // pitch of `pre` and distance of its halves, bytes
+  const int64_t pre_pitch = grad ? s.ld_pre * 2 : pl.pitch;
+  const int64_t pre_gate = grad ? s.N * 2 : pl.gate_off;
   if (wgrad) {
     if ((rc = make_expert_map(&maps.a, s.a, s.M, s.R, 0, s.lda * 2, 0, 64, kExpertBlockK, "a")) ||
         (rc = make_expert_map(&maps.b, s.b, s.N, s.R, 0, s.ldb * 2, 0, 64, kExpertBlockK, "g")) ||
         (rc = make_expert_map(&maps.out, s.out, s.N, s.M, s.E, s.ld_out * 2, s.out_stride * 2, 64,
-                              32, "out", false, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+                              32, "out", kBf16, kSw128, kNoPromo)))
       return rc;
   } else {
     const int64_t b_cols = s.b_transposed ? s.K : (swiglu ? 2 * s.N : s.N);
@@ -230,18 +256,25 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
     if ((rc = make_expert_map(&maps.a, s.a, s.K, s.R, 0, s.lda * 2, 0, 64, sgl::kBlockM, "a")) ||
         (rc = make_expert_map(&maps.a16, s.a, s.K, s.R, 0, s.lda * 2, 0, 64, 16, "a")) ||
         (rc = make_expert_map(&maps.b, s.b, b_cols, b_rows, s.E, s.ldb * 2, s.b_stride * 2, 64,
-                              s.b_transposed ? 64 : kExpertBlockK, "b")) ||
-        (rc = make_expert_map(&maps.out, s.out, s.N, s.R, 0, s.ld_out * 2, 0, 64, 32, "out", false,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+                              s.b_transposed ? 64 : kExpertBlockK, "b")))
       return rc;
-    if (s.form == sgl::EXP_SAVE16 || s.form == sgl::EXP_SAVE8) {
-      const bool bytes = s.form == sgl::EXP_SAVE8;
+    // boxes of the results, as the epilogue stages them: 32 rows x 128 bytes, x 64 bytes where
+    // three results (or the 8-bit halves) share the staging
+    const bool triple = s.form == sgl::EXP_SAVE16 || grad;
+    const bool f32 = s.form == sgl::EXP_GEMM32;
+    rc = make_expert_map(&maps.out, s.out, s.N, s.R, 0, s.ld_out * (f32 ? 4 : 2), 0,
+                         triple || f32 ? 32 : 64, 32, "out",
+                         f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kBf16, triple ? kSw64 : kSw128,
+                         kNoPromo);
+    if (rc) return rc;
+    if (triple || s.form == sgl::EXP_SAVE8) {
       uint8_t* pre = static_cast<uint8_t*>(s.pre);
-      const CUtensorMapSwizzle sw = bytes ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B;
-      if ((rc = make_expert_map(&maps.up, pre, s.N, s.R, 0, pl.pitch, 0, 64, 32, "up", bytes, sw,
-                                CU_TENSOR_MAP_L2_PROMOTION_NONE)) ||
-          (rc = make_expert_map(&maps.gate, pre + pl.gate_off, s.N, s.R, 0, pl.pitch, 0, 64, 32,
-                                "gate", bytes, sw, CU_TENSOR_MAP_L2_PROMOTION_NONE)))
+      const CUtensorMapDataType type = triple ? kBf16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+      const int cols = triple ? 32 : 64;
+      if ((rc = make_expert_map(&maps.up, pre, s.N, s.R, 0, pre_pitch, 0, cols, 32, "up", type,
+                                kSw64, kNoPromo)) ||
+          (rc = make_expert_map(&maps.gate, pre + pre_gate, s.N, s.R, 0, pre_pitch, 0, cols, 32,
+                                "gate", type, kSw64, kNoPromo)))
         return rc;
     }
   }
@@ -255,7 +288,7 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.K = static_cast<int>(s.K);
   p.M = static_cast<int>(s.M);
   p.tiles_n = static_cast<int>(tiles_n);
-  p.group_m = 8;
+  p.group_m = 16;
   p.stages = stages;
   p.acc_cols = acc_cols;
   p.a_rows = a_rows;
@@ -263,12 +296,22 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.out = static_cast<__nv_bfloat16*>(s.out);
   p.ld_out = s.ld_out;
   p.pre = static_cast<uint8_t*>(s.pre);
-  p.ld_pre = pl.pitch;
-  p.gate_off = pl.gate_off;
+  p.ld_pre = pre_pitch;
+  p.gate_off = pre_gate;
   p.scales = static_cast<uint8_t*>(s.scales);
   p.ld_scales = pl.scale_pitch;
   p.gate_scale_off = pl.gate_scale_off;
-  p.l2_hints = 0;
+  p.saved = static_cast<const uint8_t*>(s.saved);
+  p.ld_saved = pl.pitch;
+  p.saved_gate_off = pl.gate_off;
+  p.slots = s.slots;
+  p.weights = s.weights;
+  p.ld_w = s.ld_w;
+  p.num_slots = s.R;
+  p.k = static_cast<int>(s.k);
+  p.w_bf16 = s.w_bf16;
+  // operands evict-last, results evict-first, as for the dense stage
+  p.l2_hints = 2 | (2 << 2) | (1 << 4);
   p.wait_limit_ns = g_wait_limit_ns.load();
 
   int64_t grid = clusters;
@@ -431,7 +474,7 @@ int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, i
   if ((rc = check_device(&info))) return rc;
   sgl::RowParams p;
   std::memset(&p, 0, sizeof(p));
-  p.in = static_cast<const __nv_bfloat16*>(x);
+  p.in = x;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.rows = static_cast<const int*>(rows);
   p.ld_in = ldx;
@@ -445,8 +488,8 @@ int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, i
   return launch_after("expert_dispatch", sgl::expert_dispatch_kernel, grid, block, 0, 1, stream, p);
 }
 
-int sgl_expert_combine(const void* in, const void* rows, const void* weights, int weights_bf16,
-                       void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
+int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
+                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
                        int64_t ld_w, int64_t ldo, void* stream) {
   int rc;
   if ((rc = validate_row_call(T, k, D, R))) return rc;
@@ -464,7 +507,7 @@ int sgl_expert_combine(const void* in, const void* rows, const void* weights, in
   if ((rc = check_device(&info))) return rc;
   sgl::RowParams p;
   std::memset(&p, 0, sizeof(p));
-  p.in = static_cast<const __nv_bfloat16*>(in);
+  p.in = in;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.rows = static_cast<const int*>(rows);
   p.weights = weights;
@@ -478,10 +521,12 @@ int sgl_expert_combine(const void* in, const void* rows, const void* weights, in
   p.R = R;
   dim3 grid, block;
   row_geometry(T, p.nvec, info, &grid, &block);
-  return launch_after("expert_combine", sgl::expert_combine_kernel, grid, block, 0, 1, stream, p);
+  return launch_after("expert_combine",
+                      in_is_f32 ? sgl::expert_combine_kernel<true> : sgl::expert_combine_kernel<false>,
+                      grid, block, 0, 1, stream, p);
 }
 
-int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* rows,
+int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32, const void* rows,
                             const void* weights, int weights_bf16, void* grad_rows,
                             void* grad_weights, int64_t T, int64_t k, int64_t D, int64_t R,
                             int64_t ld_go, int64_t ld_in, int64_t ld_w, int64_t ld_gr,
@@ -490,12 +535,13 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* ro
   if ((rc = validate_row_call(T, k, D, R))) return rc;
   const unsigned wa = weights_bf16 ? 2 : 4;
   if ((rc = validate_ptr(grad_out, "grad_out")) || (rc = validate_words(rows, "rows", 4)) ||
-      (rc = validate_words(weights, "weights", wa)) || (rc = validate_ptr(grad_rows, "grad_rows")))
+      (rc = validate_ptr(grad_rows, "grad_rows")))
     return rc;
+  if (weights && (rc = validate_words(weights, "weights", wa))) return rc;
   if ((in != nullptr || grad_weights != nullptr) &&
       ((rc = validate_ptr(in, "in")) || (rc = validate_words(grad_weights, "grad_weights", wa))))
     return rc;
-  if (ld_w < k)
+  if (weights && ld_w < k)
     return fail(SGL_ERR_BAD_STRIDE, "ld_w=%lld is smaller than k=%lld",
                 static_cast<long long>(ld_w), static_cast<long long>(k));
   if ((rc = validate_ld(ld_go, D, "ld_go")) || (in && (rc = validate_ld(ld_in, D, "ld_in"))) ||
@@ -505,8 +551,8 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* ro
   if ((rc = check_device(&info))) return rc;
   sgl::RowParams p;
   std::memset(&p, 0, sizeof(p));
-  p.in = static_cast<const __nv_bfloat16*>(grad_out);
-  p.in2 = static_cast<const __nv_bfloat16*>(in);
+  p.in = grad_out;
+  p.in2 = in;
   p.out = static_cast<__nv_bfloat16*>(grad_rows);
   p.rows = static_cast<const int*>(rows);
   p.weights = weights;
@@ -522,8 +568,10 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, const void* ro
   p.R = R;
   dim3 grid, block;
   row_geometry(T, p.nvec, info, &grid, &block);
-  return launch_after("expert_combine_grad", sgl::expert_combine_grad_kernel, grid, block, 0, 1,
-                      stream, p);
+  return launch_after("expert_combine_grad",
+                      in_is_f32 ? sgl::expert_combine_grad_kernel<true>
+                                : sgl::expert_combine_grad_kernel<false>,
+                      grid, block, 0, 1, stream, p);
 }
 
 int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int64_t* scale_bytes,
@@ -596,7 +644,7 @@ int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offs
 
 int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
                        int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
-                       int64_t ldc, int b_transposed, void* stream) {
+                       int64_t ldc, int b_transposed, int c_is_f32, void* stream) {
   int rc;
   if ((rc = validate_groups(R, E, offsets, true))) return rc;
   if ((rc = validate_ptr(a, "a")) || (rc = validate_ptr(b, "b")) || (rc = validate_ptr(c, "c")))
@@ -608,7 +656,7 @@ int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* 
       (rc = validate_expert_stride(b_stride, b_rows, ldb, E, "b_stride")))
     return rc;
   ExpertLaunch s;
-  s.form = sgl::EXP_GEMM;
+  s.form = c_is_f32 ? sgl::EXP_GEMM32 : sgl::EXP_GEMM;
   s.name = "grouped_matmul";
   s.a = a;
   s.b = b;
@@ -623,6 +671,63 @@ int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* 
   s.b_stride = E > 1 ? b_stride : b_rows * ldb;
   s.ld_out = ldc;
   s.b_transposed = b_transposed != 0;
+  return launch_experts(s, stream);
+}
+
+int sgl_grouped_grad_preact(const void* dy, const void* w_down, const void* offsets,
+                            const void* slots, const void* weights, int weights_bf16,
+                            const void* pre, const void* scales, int bits, void* grad_preact,
+                            void* h, int64_t R, int64_t N, int64_t D, int64_t E, int64_t k,
+                            int64_t lddy, int64_t ldw, int64_t w_stride, int64_t ld_weights,
+                            int64_t ld_grad, int64_t ldh, void* stream) {
+  int rc;
+  if ((rc = check_bits(bits)) || (rc = validate_groups(R, E, offsets, true))) return rc;
+  if ((rc = validate_ptr(dy, "dy")) || (rc = validate_ptr(w_down, "w_down")) ||
+      (rc = validate_ptr(pre, "pre")) || (rc = validate_ptr(grad_preact, "grad_preact")) ||
+      (rc = validate_ptr(h, "h")))
+    return rc;
+  if (bits == 8 && (rc = validate_words(scales, "scales", 2))) return rc;
+  if (slots || weights) {
+    if ((rc = validate_words(slots, "slots", 4)) ||
+        (rc = validate_words(weights, "weights", weights_bf16 ? 2 : 4)))
+      return rc;
+    if (k < 1 || k > 64 || R % k != 0)
+      return fail(SGL_ERR_BAD_SHAPE, "k=%lld outside [1, 64] or not a divisor of R=%lld",
+                  static_cast<long long>(k), static_cast<long long>(R));
+    if (ld_weights < k)
+      return fail(SGL_ERR_BAD_STRIDE, "ld_weights=%lld is smaller than k=%lld",
+                  static_cast<long long>(ld_weights), static_cast<long long>(k));
+  }
+  if ((rc = validate_shape(R, N, D))) return rc;
+  if ((rc = validate_ld(lddy, D, "lddy")) || (rc = validate_ld(ldw, D, "ldw")) ||
+      (rc = validate_ld(ld_grad, 2 * N, "ld_grad")) || (rc = validate_ld(ldh, N, "ldh")) ||
+      (rc = validate_expert_stride(w_stride, N, ldw, E, "w_stride")))
+    return rc;
+  ExpertLaunch s;
+  s.form = bits == 8 ? sgl::EXP_GRAD8 : sgl::EXP_GRAD16;
+  s.name = "grouped_grad_preact";
+  s.a = dy;
+  s.b = w_down;
+  s.out = h;
+  s.offsets = static_cast<const int*>(offsets);
+  s.R = R;
+  s.N = N;
+  s.K = D;
+  s.E = E;
+  s.lda = lddy;
+  s.ldb = ldw;
+  s.b_stride = E > 1 ? w_stride : N * ldw;
+  s.b_transposed = 1;
+  s.ld_out = ldh;
+  s.pre = grad_preact;
+  s.ld_pre = ld_grad;
+  s.saved = pre;
+  s.scales = const_cast<void*>(scales);
+  s.slots = static_cast<const int*>(slots);
+  s.weights = weights;
+  s.ld_w = ld_weights;
+  s.k = slots ? k : 1;
+  s.w_bf16 = weights_bf16 != 0;
   return launch_experts(s, stream);
 }
 
@@ -726,7 +831,7 @@ static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t
   w->h = at;
   at += align256(R * N * 2);
   w->ys = at;
-  at += align256(R * D_out * 2);
+  at += align256(R * D_out * 4);
   w->total = at;
   return SGL_OK;
 }
@@ -773,9 +878,9 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
       (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
                                      w_stride, N, stream)) ||
       (rc = sgl_grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
-                               d_stride, D_out, 0, stream)))
+                               d_stride, D_out, 0, 1, stream)))
     return rc;
-  return sgl_expert_combine(ws + l.ys, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
+  return sgl_expert_combine(ws + l.ys, 1, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
                             ld_weights, ldy, stream);
 }
 

@@ -195,12 +195,12 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
 // and let each thread move 16 bytes (8 columns) of the row at a time.  HBM bound.
 
 struct RowParams {
-  const __nv_bfloat16* in;     // x [T, D] | rows [R, D] | grad_out [T, D]
-  const __nv_bfloat16* in2;    // combine_grad: rows [R, D]
+  const void* in;              // x [T, D] | rows [R, D] | grad_out [T, D]; bf16, rows also fp32
+  const void* in2;             // combine_grad: rows [R, D] or NULL
   __nv_bfloat16* out;          // rows [R, D] | y [T, D] | grad_rows [R, D]
   const int* rows;             // [T, k]
   const void* weights;         // fp32 or bf16 [T, k], or NULL (all ones)
-  void* grad_weights;          // combine_grad: like weights, dense [T, k]
+  void* grad_weights;          // combine_grad: dense [T, k], fp32 or bf16 (w_bf16), or NULL
   int64_t ld_in, ld_in2, ld_out, ld_w;
   int64_t T;
   int k, nvec;                 // nvec = D / 8
@@ -234,6 +234,34 @@ __device__ __forceinline__ uint4 f32_to_bf16x8(const float (&f)[8]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
+// 8 columns of a row of bf16 or fp32, kept as loaded until they are used.
+template <bool kF32>
+struct Vec8 {
+  uint4 v[kF32 ? 2 : 1];
+  __device__ __forceinline__ void load(const void* base, int64_t row, int64_t ld, int vec) {
+    if constexpr (kF32) {
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(base) + row * ld);
+      v[0] = src[2 * vec];
+      v[1] = src[2 * vec + 1];
+    } else {
+      v[0] = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(base) + row * ld)[vec];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (kF32) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f[4 * i] = __uint_as_float(v[i].x);
+        f[4 * i + 1] = __uint_as_float(v[i].y);
+        f[4 * i + 2] = __uint_as_float(v[i].z);
+        f[4 * i + 3] = __uint_as_float(v[i].w);
+      }
+    } else {
+      bf16x8_to_f32(v[0], f);
+    }
+  }
+};
+
 // The row of choice j of token t, or -1 (dropped).
 __device__ __forceinline__ int row_of(const RowParams& p, int64_t t, int j) {
   const int r = p.rows[t * p.k + j];
@@ -246,7 +274,8 @@ __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p)
   asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
        t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    const uint4* src = reinterpret_cast<const uint4*>(p.in + t * p.ld_in);
+    const uint4* src = reinterpret_cast<const uint4*>(
+        static_cast<const __nv_bfloat16*>(p.in) + t * p.ld_in);
     for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
       const uint4 val = src[v];
       for (int j = 0; j < p.k; ++j) {
@@ -259,6 +288,7 @@ __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p)
 
 // out[t] = sum_j weights[t, j] * rows[rows[t, j]], fp32 in the order of j, rounded once.  A
 // dropped choice adds nothing (its weight is not read either); a token without any is zero.
+template <bool kF32>
 __global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -268,7 +298,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) 
     for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
       float acc[8] = {};
       for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-        uint4 val[kBatch];
+        Vec8<kF32> val[kBatch];
         float w[kBatch];
         bool on[kBatch];
 #pragma unroll
@@ -277,7 +307,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) 
           const int r = j < p.k ? row_of(p, t, j) : -1;
           on[u] = r >= 0;
           if (on[u]) {
-            val[u] = reinterpret_cast<const uint4*>(p.in + r * p.ld_in)[v];
+            val[u].load(p.in, r, p.ld_in, v);
             w[u] = load_weight(p, t, j);
           }
         }
@@ -285,7 +315,7 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) 
         for (int u = 0; u < kBatch; ++u) {
           if (on[u]) {
             float f[8];
-            bf16x8_to_f32(val[u], f);
+            val[u].get(f);
 #pragma unroll
             for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[u], f[i], acc[i]);
           }
@@ -296,9 +326,10 @@ __global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) 
   }
 }
 
-// Gradients of the weighted sum: grad_rows[r] = w * grad_out[t], grad_weights[t, j] =
-// <grad_out[t], rows[r]> (0 for a dropped choice), in one pass over the rows.  The dot product is
+// Gradients of the weighted sum: grad_rows[r] = w * grad_out[t] (w = 1 without weights),
+// grad_weights[t, j] = <grad_out[t], rows[r]> (0 for a dropped choice), in one pass over the rows.  The dot product is
 // summed in fp32: by thread over its columns, then over the threads in a fixed tree.
+template <bool kF32>
 __global__ void __launch_bounds__(256) expert_combine_grad_kernel(const RowParams p) {
   __shared__ float part[8];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -310,21 +341,22 @@ __global__ void __launch_bounds__(256) expert_combine_grad_kernel(const RowParam
        t0 += static_cast<int64_t>(gridDim.x) * blockDim.y) {
     const int64_t t = t0 + threadIdx.y;
     const bool live = t < p.T;
-    const uint4* dy = reinterpret_cast<const uint4*>(p.in + (live ? t : 0) * p.ld_in);
+    const uint4* dy = reinterpret_cast<const uint4*>(
+        static_cast<const __nv_bfloat16*>(p.in) + (live ? t : 0) * p.ld_in);
     for (int j = 0; j < p.k; ++j) {
       const int r = live ? row_of(p, t, j) : -1;
       float dot = 0.f;
       if (r >= 0) {
         const float w = load_weight(p, t, j);
-        const uint4* src =
-            p.in2 ? reinterpret_cast<const uint4*>(p.in2 + r * p.ld_in2) : nullptr;
         uint4* dst = reinterpret_cast<uint4*>(p.out + r * p.ld_out);
         for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
           float g[8];
           bf16x8_to_f32(dy[v], g);
-          if (src) {
+          if (p.in2) {
+            Vec8<kF32> val;
             float y[8];
-            bf16x8_to_f32(src[v], y);
+            val.load(p.in2, r, p.ld_in2, v);
+            val.get(y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) dot = fmaf(g[i], y[i], dot);
           }

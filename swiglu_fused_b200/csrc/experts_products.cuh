@@ -6,7 +6,11 @@
 //   EXP_SAVE16   the same, and the pre-activations [up | gate] in bf16
 //   EXP_SAVE8    the same, and the pre-activations in e4m3 with a power-of-two scale per row
 //                and 32 columns (1 + 1/32 bytes for each value)
-//   EXP_GEMM     c[r]  = a[r] @ B[e] or a[r] @ B[e]^T
+//   EXP_GEMM     c[r]  = a[r] @ B[e] or a[r] @ B[e]^T, stored in bf16 (EXP_GEMM32: in fp32)
+//   EXP_GRAD16, EXP_GRAD8   the backward of the gate/up stage behind the down projection: the
+//                product t = dy[r] @ Wdown[e]^T stays in the accumulator; the epilogue reads the
+//                saved pre-activations and writes g = [w t silu(gate) | w t up silu'(gate)] and
+//                w silu(gate) up, w the routing weight of the row's slot
 //   EXP_WGRAD    C[e]  = a_e^T @ g_e   (the sum runs over the rows of the group; 0 if it is empty)
 // With offsets == NULL there is one group of all rows (the dense stage's 8-bit checkpoints).
 //
@@ -16,8 +20,10 @@
 //   * every CTA turns the offsets into a table of first tile rows once, and finds the expert
 //     of a tile by bisection in it;
 //   * an A tile whose rows run past its group takes them along in the operand (their
-//     accumulator rows are not stored), but in steps of 16 rows: one TMA box for a full tile,
-//     else ceil(rows / 16) small ones, so a group of one token does not fetch 128 rows;
+//     accumulator rows are not stored).  Up to 32 rows come in one or two boxes of 16, so a
+//     group of one token does not fetch 128 rows; more come in one box of 128, because many
+//     small boxes hold up the one thread that issues them (16384 rows over 8 uneven experts,
+//     14336 -> 4096: 1.76 ms with boxes of 16 throughout, 1.38 ms so);
 //   * the epilogue stores 32 whole rows with TMA; a warp whose rows end inside its 32 copies
 //     the rows that exist with plain stores, so that no row of another group is touched;
 //   * EXP_WGRAD sums over rows, so rows past the group must not reach the MMA: warp 6 waits
@@ -29,6 +35,7 @@
 #include <cstdint>
 #include <cuda.h>
 #include <cuda_bf16.h>
+#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "ptx_sm100.cuh"
@@ -36,7 +43,10 @@
 
 namespace sgl {
 
-enum : int { EXP_SWIGLU = 0, EXP_SAVE16 = 1, EXP_SAVE8 = 2, EXP_GEMM = 3, EXP_WGRAD = 4 };
+enum : int {
+  EXP_SWIGLU = 0, EXP_SAVE16 = 1, EXP_SAVE8 = 2, EXP_GEMM = 3, EXP_GEMM32 = 4, EXP_GRAD16 = 5,
+  EXP_GRAD8 = 6, EXP_WGRAD = 7, EXP_FORMS = 8
+};
 
 constexpr int kExpThreads = 224;       // producer, MMA issuer, 4 epilogue warps, tail warp
 constexpr int kExpMaxStages = 16;
@@ -53,11 +63,11 @@ enum : unsigned {
 
 struct ExpertMaps {
   CUtensorMap a;        // A operand, whole-tile box
-  CUtensorMap a16;      // A operand, boxes of 16 rows (forward forms)
+  CUtensorMap a16;      // A operand, boxes of 16 rows (forward forms, few rows)
   CUtensorMap b;        // B operand
-  CUtensorMap out;      // h / c / C
-  CUtensorMap up;       // pre-activations: up half
-  CUtensorMap gate;     // pre-activations: gate half
+  CUtensorMap out;      // h / c / C / w h
+  CUtensorMap up;       // pre-activations or their gradients: up half
+  CUtensorMap gate;     // the same, gate half
 };
 
 struct ExpertParams {
@@ -74,12 +84,18 @@ struct ExpertParams {
   int b_kmajor;         // B[e] is stored [n, k] (multiplied transposed)
   __nv_bfloat16* out;   // forward forms: raw pointers for rows that end inside a warp's 32
   int64_t ld_out;
-  uint8_t* pre;         // pre-activations, bytes; gate half at + gate_off
+  uint8_t* pre;         // pre-activations or their gradients (written), gate half at + gate_off
   int64_t ld_pre;       // row pitch, bytes
   int64_t gate_off;     // bytes from the up half to the gate half of a row
-  uint8_t* scales;      // EXP_SAVE8: [R][2][n_blocks] exponents + 127
+  uint8_t* scales;      // 8-bit forms: [R][2][n_blocks] exponents + 127
   int64_t ld_scales;    // row pitch, bytes
   int64_t gate_scale_off;
+  const uint8_t* saved; // EXP_GRAD*: the saved pre-activations, pitch and gate half as for pre
+  int64_t ld_saved, saved_gate_off;
+  const int* slots;     // EXP_GRAD*: slot of each row, for its routing weight; NULL: weights of 1
+  const void* weights;  // fp32 or bf16 [T, k], row pitch ld_w
+  int64_t ld_w, num_slots;
+  int k, w_bf16;
   int l2_hints;
   unsigned long long wait_limit_ns;
 };
@@ -87,9 +103,15 @@ struct ExpertParams {
 template <int kForm, int kCtaGroup, int kBlockK>
 struct ExpertTraits {
   static constexpr bool kSwiglu = kForm == EXP_SWIGLU || kForm == EXP_SAVE16 || kForm == EXP_SAVE8;
-  // staging of one epilogue warp: two 64-column chunks, or one chunk with its pre-activations
+  static constexpr bool kGrad = kForm == EXP_GRAD16 || kForm == EXP_GRAD8;
+  // Three bf16 results of the same shape: staged 32 columns at a time (64-byte rows), so that a
+  // ring of three 128-deep stages still fits (at 64 columns only two do: save16 took 3.8 ms
+  // instead of 2.8 at 16384 x 4096 x 14336 over 8 experts).
+  static constexpr bool kTriple = kForm == EXP_SAVE16 || kGrad;
+  // staging of one epilogue warp: two 64-column chunks (of fp32: 32 columns), or one chunk
+  // with its 8-bit pre-activations, or three of 32 columns
   static constexpr int kStagingPerWarp =
-      kForm == EXP_SAVE16 ? 3 * kChunkBytes : 2 * kChunkBytes;
+      kTriple ? 3 * kChunkBytes / 2 : 2 * kChunkBytes;
   static constexpr int kStagingBytes = kEpiWarps * kStagingPerWarp;
   static constexpr int kBSlabsMax = kAccCols / kCtaGroup / 64;
   static constexpr int kBSlabBytes = kBlockK * 128;
@@ -99,7 +121,7 @@ struct ExpertTraits {
     return acc_cols / kCtaGroup * kBlockK * 2;
   }
   __host__ __device__ static constexpr int table_bytes(int groups) {
-    return (2 * (groups + 1) * 4 + 15) / 16 * 16;
+    return kForm == EXP_WGRAD ? 0 : ((groups + 1) * 4 + 15) / 16 * 16;
   }
   __host__ __device__ static constexpr int fixed_bytes(int groups) {
     return 1024 + kStagingBytes + kExpBarrierBytes + table_bytes(groups);
@@ -225,6 +247,63 @@ __device__ __forceinline__ void copy_rows(uint32_t buf, uint8_t* dst, int64_t ld
   }
 }
 
+// Two e4m3 values (16 bits) as fp32.
+__device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
+  uint32_t h2;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(static_cast<uint16_t>(two)));
+  return __half22float2(*reinterpret_cast<__half2*>(&h2));
+}
+
+// 32 saved up and gate values of one row, columns x .. x + 31 (a block; the halves are padded to
+// whole blocks, so the last one may be read past N).  Rows that do not exist are not read.
+template <int kBits>
+__device__ __forceinline__ void load_saved(const ExpertParams& p, int64_t row, int x, bool live,
+                                           float (&up)[32], float (&gate)[32]) {
+  const uint8_t* at = p.saved + row * p.ld_saved + x * (kBits / 8);
+  constexpr int kVecs = 32 * kBits / 8 / 16;
+  uint4 u[kVecs], g[kVecs];
+  int su = 0, sg = 0;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    u[i] = make_uint4(0, 0, 0, 0);
+    g[i] = u[i];
+  }
+  if (live) {
+#pragma unroll
+    for (int i = 0; i < kVecs; ++i) {
+      u[i] = reinterpret_cast<const uint4*>(at)[i];
+      g[i] = reinterpret_cast<const uint4*>(at + p.saved_gate_off)[i];
+    }
+    if constexpr (kBits == 8) {
+      const uint8_t* sc = p.scales + row * p.ld_scales + (x >> 5);
+      su = sc[0];
+      sg = sc[p.gate_scale_off];
+    }
+  }
+  const float fu = kBits == 8 ? block_scale(su) : 1.f, fg = kBits == 8 ? block_scale(sg) : 1.f;
+#pragma unroll
+  for (int i = 0; i < kVecs; ++i) {
+    const uint32_t wu[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+    const uint32_t wg[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if constexpr (kBits == 8) {
+        const int o = i * 16 + j * 4;
+        const float2 u0 = e4m3x2_to_f32(wu[j]), u1 = e4m3x2_to_f32(wu[j] >> 16);
+        const float2 g0 = e4m3x2_to_f32(wg[j]), g1 = e4m3x2_to_f32(wg[j] >> 16);
+        up[o] = u0.x * fu; up[o + 1] = u0.y * fu; up[o + 2] = u1.x * fu; up[o + 3] = u1.y * fu;
+        gate[o] = g0.x * fg; gate[o + 1] = g0.y * fg; gate[o + 2] = g1.x * fg; gate[o + 3] = g1.y * fg;
+      } else {
+        const int o = i * 8 + j * 2;
+        up[o] = __uint_as_float(wu[j] << 16);
+        up[o + 1] = __uint_as_float(wu[j] & 0xffff0000u);
+        gate[o] = __uint_as_float(wg[j] << 16);
+        gate[o + 1] = __uint_as_float(wg[j] & 0xffff0000u);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------- the kernel
 
 template <int kForm, int kCtaGroup, int kBlockK>
@@ -265,8 +344,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   volatile uint32_t* tmem_slot_ptr =
       reinterpret_cast<volatile uint32_t*>(smem_gen + (tmem_slot - smem_base));
   int* abort_flag = reinterpret_cast<int*>(smem_gen + (abort_slot - smem_base));
-  int* row_lo = reinterpret_cast<int*>(smem_gen + (table - smem_base));   // [groups + 1]
-  int* tile_lo = row_lo + p.groups + 1;                                   // [groups + 1]
+  int* tile_lo = reinterpret_cast<int*>(smem_gen + (table - smem_base));   // [groups + 1]
 
   if (threadIdx.x == 0) {
     abort_flag[0] = 0;
@@ -290,36 +368,40 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  // ---- the groups: first row and first tile row of each (clamped: rows that do not exist in
-  // the row tensors are never addressed, whatever the offsets say) ----
+  // ---- the groups: first row (clamped: rows that do not exist in the row tensors are never
+  // addressed, whatever the offsets say), and a table of first tile rows ----
   const int G = p.groups;
-  for (int e = threadIdx.x; e <= G; e += kExpThreads) {
-    int lo = p.offsets ? p.offsets[e] : (e == 0 ? 0 : p.R);
-    lo = lo < 0 ? 0 : (lo > p.R ? p.R : lo);
-    row_lo[e] = lo;
-  }
-  __syncthreads();
-  if (warp == 0 && !kWgrad) {
-    const int per = (G + 31) / 32;
-    const int e0 = lane * per, e1 = (e0 + per < G) ? e0 + per : G;
-    int mine = 0;
-    for (int e = e0; e < e1; ++e) {
-      const int n = row_lo[e + 1] - row_lo[e];
-      mine += n > 0 ? (n + kTileRows - 1) / kTileRows : 0;
+  auto row_lo = [&](int e) {
+    if (p.offsets == nullptr) return e == 0 ? 0 : p.R;
+    const int lo = __ldg(p.offsets + e);
+    return lo < 0 ? 0 : (lo > p.R ? p.R : lo);
+  };
+  if constexpr (!kWgrad) {
+    for (int e = threadIdx.x; e < G; e += kExpThreads) {
+      const int n = row_lo(e + 1) - row_lo(e);
+      tile_lo[e] = n > 0 ? (n + kTileRows - 1) / kTileRows : 0;
     }
-    int inc = mine;
+    __syncthreads();
+    if (warp == 0) {
+      // exclusive sums in place: each lane a run of groups, then over the lanes
+      const int per = (G + 31) / 32;
+      const int e0 = lane * per, e1 = (e0 + per < G) ? e0 + per : G;
+      int mine = 0;
+      for (int e = e0; e < e1; ++e) mine += tile_lo[e];
+      int inc = mine;
 #pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, d);
-      if (lane >= d) inc += v;
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, d);
+        if (lane >= d) inc += v;
+      }
+      int at = inc - mine;
+      for (int e = e0; e < e1; ++e) {
+        const int n = tile_lo[e];
+        tile_lo[e] = at;
+        at += n;
+      }
+      if (lane == 31) tile_lo[G] = inc;
     }
-    int at = inc - mine;
-    for (int e = e0; e < e1; ++e) {
-      tile_lo[e] = at;
-      const int n = row_lo[e + 1] - row_lo[e];
-      at += n > 0 ? (n + kTileRows - 1) / kTileRows : 0;
-    }
-    if (lane == 31) tile_lo[G] = inc;
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
@@ -343,8 +425,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       r.e = tm / wgrad_tiles_m;
       const TileCoord tc = tile_coord(u - r.e * wgrad_tiles_m * p.tiles_n, wgrad_tiles_m,
                                       p.tiles_n, p.group_m);
-      r.row = row_lo[r.e];
-      r.rows = row_lo[r.e + 1] - r.row;
+      r.row = row_lo(r.e);
+      r.rows = row_lo(r.e + 1) - r.row;
       if (r.rows < 0) r.rows = 0;
       r.m = tc.m * kTileRows;
       r.n = tc.n * tile_cols;
@@ -357,8 +439,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       r.e = lo;
       const TileCoord tc = tile_coord(u - tile_lo[lo] * p.tiles_n, tile_lo[lo + 1] - tile_lo[lo],
                                       p.tiles_n, p.group_m);
-      r.row = row_lo[lo] + tc.m * kTileRows;
-      r.rows = row_lo[lo + 1] - r.row;
+      r.row = row_lo(lo) + tc.m * kTileRows;
+      r.rows = row_lo(lo + 1) - r.row;
       r.m = 0;
       r.n = tc.n * tile_cols;
     }
@@ -379,19 +461,21 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       int s = 0;
       uint32_t ph = 0;
       bool ok = true;
+      Unit next;
+      if (cluster_id < total_units) next = unit_of(cluster_id);
       for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
-        const Unit un = unit_of(u);
+        const Unit un = next;
         const int num_kb = unit_kb(un);
+        if (num_kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
         // forward: rows of this CTA's half of the tile, and the boxes that cover them
         int left = un.rows - static_cast<int>(rank) * kBlockM;
         left = left < 0 ? 0 : (left > kBlockM ? kBlockM : left);
         const int my_row = un.row + static_cast<int>(rank) * kBlockM;
+        const bool whole = left > 32 && p.a_rows == kBlockM;
         const int boxes16 = (left + 15) / 16;
-        const bool whole = !kWgrad && boxes16 * 16 == p.a_rows && p.a_rows == kBlockM;
         const uint32_t b_bytes = static_cast<uint32_t>(b_slabs * T::kBSlabBytes);
         const uint32_t stage_tx =
-            b_bytes + static_cast<uint32_t>(kWgrad ? kBlockM * kBlockK * 2
-                                                   : boxes16 * 16 * kBlockK * 2);
+            b_bytes + static_cast<uint32_t>((kWgrad || whole ? kBlockM : boxes16 * 16) * kBlockK * 2);
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!ptx::mbar_wait(bar_empty + 8 * s, ph ^ 1u, limit, abort_flag)) {
             report_error(kErrExpProducerWait, kb, abort_flag);
@@ -486,6 +570,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             s = 0;
             ph ^= 1u;
           }
+          // the next tile is looked up while this one's loads are under way
+          if (kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
         }
       }
       if (!ok) {
@@ -506,8 +592,11 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       uint32_t ph = 0;
       bool ok = true;
       int i = 0;
+      Unit next;
+      if (cluster_id < total_units) next = unit_of(cluster_id);
       for (int u = cluster_id; u < total_units && ok; u += num_clusters, ++i) {
-        const Unit un = unit_of(u);
+        const Unit un = next;
+        if (unit_kb(un) == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
         const int as = i % kAccStages;
         const uint32_t aph = (i / kAccStages) & 1u;
         if (!ptx::mbar_wait(bar_tempty + 8 * as, aph ^ 1u, limit, abort_flag)) {
@@ -549,6 +638,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             s = 0;
             ph ^= 1u;
           }
+          if (kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
         }
         if (ok) ptx::umma_commit<kCtaGroup>(bar_tfull + 8 * as, mask);
       }
@@ -637,6 +727,136 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         continue;
       }
       const int64_t grow = un.row + in_tile;       // forward forms: first row in the row tensors
+      if constexpr (T::kTriple) {
+        // ---- three bf16 results, 32 columns at a time ----
+        constexpr uint32_t kSB = kChunkBytes / 2;
+        const uint32_t off_row = static_cast<uint32_t>(lane) * 64u;
+        const uint32_t sw64 = (static_cast<uint32_t>(lane) >> 1) & 3u;
+        const int units = tile_cols / 32;
+        const bool live = lane < valid;
+        float weight = 1.0f;
+        if constexpr (T::kGrad) {
+          if (p.slots != nullptr && live) {
+            const int64_t slot = p.slots[grow + lane];
+            weight = 0.f;
+            if (slot >= 0 && slot < p.num_slots) {
+              const int64_t at = slot / p.k * p.ld_w + slot % p.k;
+              weight = p.w_bf16
+                           ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.weights)[at])
+                           : reinterpret_cast<const float*>(p.weights)[at];
+            }
+          }
+        }
+        for (int c = 0; c < units; ++c) {
+          const int x = un.n + c * 32;
+          const bool last = c == units - 1;
+          if (x < p.N) {
+            float a[32], b[32], h[32];
+            if constexpr (kForm == EXP_SAVE16) {
+              ptx::tmem_ld_32x32b_x32(t_row + c * 32, a);
+              ptx::tmem_ld_32x32b_x32(t_row + gate_col + c * 32, b);
+              ptx::tmem_ld_wait();
+              if (last) hand_back();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) h[j] = silu_mul(b[j], a[j]);
+            } else {
+              // this row's 32 saved up and gate values, then the gradients in their place
+              load_saved<kForm == EXP_GRAD8 ? 8 : 16>(p, grow + lane, x, live, a, b);
+              ptx::tmem_ld_32x32b_x32(t_row + c * 32, h);
+              ptx::tmem_ld_wait();
+              if (last) hand_back();
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                float hv, sv, dv;
+                silu_factors(b[j], a[j], hv, sv, dv);
+                const float t = weight * h[j];
+                a[j] = t * sv;
+                b[j] = t * dv;
+                h[j] = weight * hv;
+              }
+            }
+            if (lane == 0) ptx::bulk_wait_group_read<0>();
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const uint32_t off = buf0 + off_row + ((static_cast<uint32_t>(j) ^ sw64) << 4);
+              st_shared_v4(off, pack_bf16x2(h[8 * j], h[8 * j + 1]),
+                           pack_bf16x2(h[8 * j + 2], h[8 * j + 3]),
+                           pack_bf16x2(h[8 * j + 4], h[8 * j + 5]),
+                           pack_bf16x2(h[8 * j + 6], h[8 * j + 7]));
+              st_shared_v4(off + kSB, pack_bf16x2(a[8 * j], a[8 * j + 1]),
+                           pack_bf16x2(a[8 * j + 2], a[8 * j + 3]),
+                           pack_bf16x2(a[8 * j + 4], a[8 * j + 5]),
+                           pack_bf16x2(a[8 * j + 6], a[8 * j + 7]));
+              st_shared_v4(off + 2 * kSB, pack_bf16x2(b[8 * j], b[8 * j + 1]),
+                           pack_bf16x2(b[8 * j + 2], b[8 * j + 3]),
+                           pack_bf16x2(b[8 * j + 4], b[8 * j + 5]),
+                           pack_bf16x2(b[8 * j + 6], b[8 * j + 7]));
+            }
+            if (valid == 32) {
+              ptx::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                const int y = static_cast<int>(grow);
+                ptx::tma_store_2d(&maps.out, x, y, buf0, pol_out);
+                ptx::tma_store_2d(&maps.up, x, y, buf0 + kSB, pol_out);
+                ptx::tma_store_2d(&maps.gate, x, y, buf0 + 2 * kSB, pol_out);
+                ptx::bulk_commit_group();
+              }
+            } else {
+              // the group ends inside this warp's rows: store the rows it has, and no other
+              __syncwarp();
+              const int bytes = (p.N - x < 32 ? p.N - x : 32) * 2;
+              copy_rows<64>(buf0, reinterpret_cast<uint8_t*>(p.out + grow * p.ld_out + x),
+                            p.ld_out * 2, valid, bytes, lane);
+              uint8_t* at = p.pre + grow * p.ld_pre + x * 2;
+              copy_rows<64>(buf0 + kSB, at, p.ld_pre, valid, bytes, lane);
+              copy_rows<64>(buf0 + 2 * kSB, at + p.gate_off, p.ld_pre, valid, bytes, lane);
+              __syncwarp();
+            }
+          } else if (last) {
+            hand_back();
+          }
+        }
+      } else if constexpr (kForm == EXP_GEMM32) {
+        // ---- fp32 result, 32 columns at a time, two buffers ----
+        const int units = tile_cols / 32;
+        for (int c = 0; c < units; ++c) {
+          const int x = un.n + c * 32;
+          const bool last = c == units - 1;
+          if (x < p.N) {
+            const uint32_t buf = buf0 + (stores & 1) * kChunkBytes;
+            ++stores;
+            if (lane == 0) ptx::bulk_wait_group_read<1>();
+            __syncwarp();
+            float v[32];
+            ptx::tmem_ld_32x32b_x32(t_row + c * 32, v);
+            ptx::tmem_ld_wait();
+            if (last) hand_back();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              st_shared_v4(buf + row_off + ((static_cast<uint32_t>(j) ^ row_sw) << 4),
+                           __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                           __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+            if (valid == 32) {
+              ptx::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) ptx::tma_store_2d(&maps.out, x, static_cast<int>(grow), buf, pol_out);
+            } else {
+              __syncwarp();
+              copy_rows<128>(buf,
+                             reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) +
+                                                        grow * p.ld_out + x),
+                             p.ld_out * 4, valid, (p.N - x < 32 ? p.N - x : 32) * 4, lane);
+              __syncwarp();
+            }
+            if (lane == 0) ptx::bulk_commit_group();   // keeps the buffers' turn-taking in step
+          } else if (last) {
+            hand_back();
+          }
+        }
+      } else {
+      // ---- one bf16 result, 64 columns at a time (EXP_SAVE8: with its 8-bit pre-activations) ----
       const int chunks = tile_cols / 64;
 #pragma unroll 1
       for (int c = 0; c < chunks; ++c) {
@@ -644,7 +864,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         const bool last = c == chunks - 1;
         // the staging buffer(s) of this chunk
         uint32_t buf = buf0;
-        if constexpr (kForm == EXP_SAVE16 || kForm == EXP_SAVE8) {
+        if constexpr (kForm == EXP_SAVE8) {
           if (lane == 0) ptx::bulk_wait_group_read<0>();
         } else {
           if (lane == 0) ptx::bulk_wait_group_read<1>();
@@ -663,22 +883,6 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
               float gate[32];
               ptx::tmem_ld_32x32b_x32(t_row + gate_col + col, gate);
               ptx::tmem_ld_wait();
-              if constexpr (kForm == EXP_SAVE16) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                  const uint32_t off =
-                      row_off + ((static_cast<uint32_t>(half * 4 + j) ^ row_sw) << 4);
-                  st_shared_v4(buf + kChunkBytes + off, pack_bf16x2(v0[8 * j], v0[8 * j + 1]),
-                               pack_bf16x2(v0[8 * j + 2], v0[8 * j + 3]),
-                               pack_bf16x2(v0[8 * j + 4], v0[8 * j + 5]),
-                               pack_bf16x2(v0[8 * j + 6], v0[8 * j + 7]));
-                  st_shared_v4(buf + 2 * kChunkBytes + off,
-                               pack_bf16x2(gate[8 * j], gate[8 * j + 1]),
-                               pack_bf16x2(gate[8 * j + 2], gate[8 * j + 3]),
-                               pack_bf16x2(gate[8 * j + 4], gate[8 * j + 5]),
-                               pack_bf16x2(gate[8 * j + 6], gate[8 * j + 7]));
-                }
-              }
               if constexpr (kForm == EXP_SAVE8) {
                 // columns at and past N hold sums over nothing (the operand reads as zero
                 // there, or as the gate half's weights): they do not belong to a block
@@ -748,10 +952,6 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
               } else {
                 const int y = static_cast<int>(grow);
                 ptx::tma_store_2d(&maps.out, x, y, buf, pol_out);
-                if constexpr (kForm == EXP_SAVE16) {
-                  ptx::tma_store_2d(&maps.up, x, y, buf + kChunkBytes, pol_out);
-                  ptx::tma_store_2d(&maps.gate, x, y, buf + 2 * kChunkBytes, pol_out);
-                }
                 if constexpr (kForm == EXP_SAVE8) {
                   ptx::tma_store_2d(&maps.up, x, y, buf + kChunkBytes, pol_out);
                   ptx::tma_store_2d(&maps.gate, x, y, buf + kChunkBytes + kChunkBytes / 2, pol_out);
@@ -761,18 +961,11 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             ptx::bulk_commit_group();
           }
         } else {
-          // the group ends inside this warp's rows: store the rows it has, and no other
           __syncwarp();
           if (x < p.N) {
             const int cols = p.N - x < 64 ? p.N - x : 64;
             copy_rows<128>(buf, reinterpret_cast<uint8_t*>(p.out + grow * p.ld_out + x),
                            p.ld_out * 2, valid, cols * 2, lane);
-            if constexpr (kForm == EXP_SAVE16) {
-              uint8_t* at = p.pre + grow * p.ld_pre + x * 2;
-              copy_rows<128>(buf + kChunkBytes, at, p.ld_pre, valid, cols * 2, lane);
-              copy_rows<128>(buf + 2 * kChunkBytes, at + p.gate_off, p.ld_pre, valid, cols * 2,
-                             lane);
-            }
             if constexpr (kForm == EXP_SAVE8) {
               uint8_t* at = p.pre + grow * p.ld_pre + x;
               copy_rows<64>(buf + kChunkBytes, at, p.ld_pre, valid, cols, lane);
@@ -783,6 +976,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
           __syncwarp();
           if (lane == 0) ptx::bulk_commit_group();    // keeps the buffers' turn-taking in step
         }
+      }
       }
     }
     if (lane == 0) ptx::bulk_wait_group_read<0>();

@@ -10,7 +10,6 @@
 
 #include <cstdint>
 #include <cuda_bf16.h>
-#include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
 #include "experts_order.cuh"
@@ -34,10 +33,7 @@ __device__ __forceinline__ void e4m3x8_to_f32(uint2 c, float scale, float (&f)[8
   const uint32_t w[2] = {c.x, c.y};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint16_t two = static_cast<uint16_t>(w[i >> 1] >> (16 * (i & 1)));
-    uint32_t h2;
-    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h2) : "h"(two));
-    const float2 v = __half22float2(*reinterpret_cast<__half2*>(&h2));
+    const float2 v = e4m3x2_to_f32(w[i >> 1] >> (16 * (i & 1)));
     f[2 * i] = v.x * scale;
     f[2 * i + 1] = v.y * scale;
   }

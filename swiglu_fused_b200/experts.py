@@ -10,6 +10,7 @@ expert ``e`` owns ``W[e] = [W_up | W_gate]`` (``[K, 2N]``) and ``W_down[e]`` (``
 ``expert_combine_grad``   gradients of the weighted sum, for the rows and for the weights
 ``grouped_fused_swiglu``  the gate/up stage over row groups (``_save`` keeps the pre-activations)
 ``grouped_matmul``        the down projection over row groups, and its transposed form
+``grouped_grad_preact``   the gate/up stage's backward behind the down projection, one launch
 ``grouped_weight_grad``   ``a_e^T @ g_e`` for every expert
 ``experts_swiglu``        all of the forward in one call, for inference
 ``swiglu_grad_preact_saved``  the backward's elementwise step from saved pre-activations
@@ -141,6 +142,39 @@ def _check_order_rows(order: ExpertOrder) -> tuple[int, int]:
     return T, k
 
 
+def _check_rows(t: torch.Tensor, name: str) -> None:
+    """Rows of the experts' outputs: a bf16 matrix as everywhere, or the same in fp32."""
+    if isinstance(t, torch.Tensor) and t.dtype == torch.float32:
+        if t.dim() != 2:
+            raise ValueError(f"{name} must be 2-D, got shape {tuple(t.shape)}")
+        rows, cols = t.shape
+        if not t.is_cuda:
+            raise ValueError(f"{name} must be a CUDA tensor (this operator has no CPU path)")
+        if cols < 1 or t.stride(1) != 1 or (rows > 1 and (t.stride(0) < cols or t.stride(0) % 8)):
+            raise ValueError(f"{name} must be row-major with a row stride that is a multiple of 8, "
+                             f"got shape {tuple(t.shape)}, strides {t.stride()}")
+        if t.data_ptr() % 16 != 0:
+            raise ValueError(f"{name} must be 16-byte aligned")
+        return
+    _check_matrix(t, name, allow_empty_rows=True)
+
+
+def _prep_rows(out, M: int, N: int, device, dtype):
+    """``out`` for a result in ``dtype`` (bf16 or fp32), allocated if omitted."""
+    if dtype == DTYPE:
+        return _prep_out(out, M, N, device)
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=device)
+    if not isinstance(out, torch.Tensor) or out.dtype != dtype:
+        raise TypeError(f"out must be a {dtype} tensor")
+    _check_rows(out, "out")
+    if tuple(out.shape) != (M, N):
+        raise ValueError(f"out shape {tuple(out.shape)} != {(M, N)}")
+    if out.device != device:
+        raise ValueError(f"out is on {out.device}, expected {device}")
+    return out
+
+
 def _multiple_of_8(**sizes: int) -> None:
     for name, n in sizes.items():
         if n % 8:
@@ -198,11 +232,11 @@ def _check_weights(weights, T: int, k: int) -> None:
 
 
 def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=None):
-    """``out[t] = sum_j weights[t, j] * rows[order.rows[t, j]]``: ``[T * k, D]`` -> ``[T, D]``, fp32
-    sums in the order of ``j``.  ``weights`` is fp32 or bf16 ``[T, k]``; without weights the rows
-    are summed as they are.  Dropped slots add nothing."""
+    """``out[t] = sum_j weights[t, j] * rows[order.rows[t, j]]``: ``[T * k, D]`` bf16 or fp32 ->
+    ``[T, D]`` bf16, fp32 sums in the order of ``j``.  ``weights`` is fp32 or bf16 ``[T, k]``;
+    without weights the rows are summed as they are.  Dropped slots add nothing."""
     T, k = _check_order_rows(order)
-    _check_matrix(rows, "rows", allow_empty_rows=True)
+    _check_rows(rows, "rows")
     if rows.shape[0] != T * k:
         raise ValueError(f"rows has {rows.shape[0]} rows, the order {T * k} slots")
     D = rows.shape[1]
@@ -218,7 +252,7 @@ def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=N
         o = _prep_out(out, T, D, dev)
     with _on_device(dev):
         _lib.check(_lib.load().sgl_expert_combine(
-            rows.data_ptr(), order.rows.data_ptr(),
+            rows.data_ptr(), int(rows.dtype == torch.float32), order.rows.data_ptr(),
             weights.data_ptr() if weights is not None else None,
             int(weights is not None and weights.dtype == DTYPE), o.data_ptr(), T, k, D, T * k,
             _ld(rows), _choice_ld(weights) if weights is not None else 0, _ld(o),
@@ -226,18 +260,21 @@ def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=N
     return o
 
 
-def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, out=None, stream=None):
+def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, weighted: bool = True,
+                        out=None, stream=None):
     """Gradients of ``expert_combine(rows, order, weights)``: ``(grad_rows, grad_weights)`` with
     ``grad_rows[r] = weight * grad_out[t]`` (rows behind the last expert's are left as they were)
     and ``grad_weights[t, j] = <grad_out[t], rows[r]>`` in the weights' type, 0 for dropped slots.
-    ``out`` takes ``grad_rows``; it may be ``rows`` itself.  With ``rows=None`` only ``grad_rows`` is
-    computed (``grad_weights`` is None)."""
+    ``rows`` may be bf16 or fp32.  ``out`` takes ``grad_rows``; it may be a bf16 ``rows`` itself.
+    With ``rows=None`` only ``grad_rows`` is computed (``grad_weights`` is None).  With
+    ``weighted=False`` the rows of ``grad_rows`` are ``grad_out[t]`` as it is, for a caller that
+    applies the weight further on (``grouped_grad_preact`` does)."""
     T, k = _check_order_rows(order)
     _check_matrix(grad_out, "grad_out", allow_empty_rows=True)
     D = grad_out.shape[1]
     named = [("grad_out", grad_out), ("order.rows", order.rows), ("weights", weights)]
     if rows is not None:
-        _check_matrix(rows, "rows", allow_empty_rows=True)
+        _check_rows(rows, "rows")
         named.append(("rows", rows))
     if grad_out.shape[0] != T or (rows is not None and tuple(rows.shape) != (T * k, D)):
         raise ValueError(f"grad_out {tuple(grad_out.shape)} and rows "
@@ -254,7 +291,8 @@ def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, out=None
     with _on_device(dev):
         _lib.check(_lib.load().sgl_expert_combine_grad(
             grad_out.data_ptr(), rows.data_ptr() if rows is not None else None,
-            order.rows.data_ptr(), weights.data_ptr(), int(weights.dtype == DTYPE), gr.data_ptr(),
+            int(rows is not None and rows.dtype == torch.float32), order.rows.data_ptr(),
+            weights.data_ptr() if weighted else None, int(weights.dtype == DTYPE), gr.data_ptr(),
             gw.data_ptr() if gw is not None else None, T, k, D, T * k, _ld(grad_out),
             _ld(rows) if rows is not None else D, _choice_ld(weights), _ld(gr),
             _stream_handle(stream, dev)))
@@ -408,12 +446,15 @@ def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h:
     return (g, h) if return_h else g
 
 
-def grouped_matmul(a, B, offsets, *, out=None, stream=None, transpose_b: bool = False):
+def grouped_matmul(a, B, offsets, *, out=None, stream=None, transpose_b: bool = False,
+                   out_dtype: torch.dtype = DTYPE):
     """``c[r] = a[r] @ B[e]`` for the rows of every expert: the down projection.
 
     a : [R, K] bf16;  B : [E, K, N] bf16, or [E, N, K] with ``transpose_b`` (read in place)
-    returns [R, N] bf16; rows behind ``offsets[E]`` are left as they were
+    returns [R, N] in ``out_dtype``, bf16 or fp32; rows behind ``offsets[E]`` are left as they were
     """
+    if out_dtype not in (DTYPE, torch.float32):
+        raise TypeError(f"out_dtype must be torch.bfloat16 or torch.float32, got {out_dtype}")
     _check_matrix(a, "a", allow_empty_rows=True)
     _check_experts(B, "B")
     R, K = a.shape
@@ -425,14 +466,71 @@ def grouped_matmul(a, B, offsets, *, out=None, stream=None, transpose_b: bool = 
     _check_ints(offsets, "offsets", (E + 1,))
     dev = _same_device(("a", a), ("B", B), ("offsets", offsets))
     if R == 0:
-        return out if out is not None else torch.empty((0, N), dtype=DTYPE, device=dev)
+        return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=dev)
     with stream_context(stream, dev):
-        c = _prep_out(out, R, N, dev)
+        c = _prep_rows(out, R, N, dev, out_dtype)
     with _on_device(dev):
         _lib.check(_lib.load().sgl_grouped_matmul(
             a.data_ptr(), B.data_ptr(), offsets.data_ptr(), c.data_ptr(), R, N, K, E, _ld(a),
-            _expert_ld(B), B.stride(0), _ld(c), int(transpose_b), _stream_handle(stream, dev)))
+            _expert_ld(B), B.stride(0), _ld(c), int(transpose_b), int(out_dtype == torch.float32),
+            _stream_handle(stream, dev)))
     return c
+
+
+def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrder, weights=None, *,
+                        out=None, stream=None):
+    """The gate/up stage's backward behind the down projection, one launch: with
+    ``t = grad_rows[r] @ W_down[e]^T`` and the saved pre-activations of row ``r``,
+    ``grad_preact[r] = [w t silu(gate) | w t up silu'(gate)]`` and ``h[r] = w silu(gate) up``, ``w`` the
+    routing weight of the row's slot (1 without ``weights``).  ``t`` is not rounded; ``W_down``'s
+    gradient is ``grouped_weight_grad(h, grad_rows, offsets)``, the weight being in ``h`` already.
+
+    grad_rows : [R, D] bf16, gradients of the rows' outputs without the routing weight
+    W_down    : [E, N, D] bf16
+    returns   : ``(grad_preact [R, 2N], h [R, N])``; rows behind the last expert's are left as they were
+    """
+    T, k = _check_order_rows(order)
+    _check_matrix(grad_rows, "grad_rows", allow_empty_rows=True)
+    _check_experts(W_down, "W_down")
+    if not isinstance(preact, SavedPreact):
+        raise TypeError(f"preact must be a SavedPreact, got {type(preact).__name__}")
+    R, D = grad_rows.shape
+    E, N, D2 = W_down.shape
+    if D2 != D or R != T * k:
+        raise ValueError(f"grad_rows {tuple(grad_rows.shape)} does not fit W_down "
+                         f"{tuple(W_down.shape)} and {T} tokens of {k} choices")
+    _multiple_of_8(D=D, N=N)
+    _check_preact(preact)
+    if preact.hidden != N or preact.data.shape[0] != R:
+        raise ValueError(f"the saved pre-activations are of {preact.data.shape[0]} rows and "
+                         f"{preact.hidden} columns, expected {R} and {N}")
+    _check_ints(order.offsets, "order.offsets", (E + 1,))
+    _check_ints(order.slots, "order.slots", (R,))
+    named = [("grad_rows", grad_rows), ("W_down", W_down), ("preact.data", preact.data),
+             ("order.rows", order.rows), ("order.offsets", order.offsets),
+             ("order.slots", order.slots)]
+    if preact.scales is not None:
+        named.append(("preact.scales", preact.scales))
+    if weights is not None:
+        _check_weights(weights, T, k)
+        named.append(("weights", weights))
+    dev = _same_device(*named)
+    with stream_context(stream, dev):
+        h = torch.empty((R, N), dtype=DTYPE, device=dev)
+        if R == 0:
+            return (out if out is not None else torch.empty((0, 2 * N), dtype=DTYPE, device=dev)), h
+        g = _prep_out(out, R, 2 * N, dev)
+    with _on_device(dev):
+        _lib.check(_lib.load().sgl_grouped_grad_preact(
+            grad_rows.data_ptr(), W_down.data_ptr(), order.offsets.data_ptr(),
+            order.slots.data_ptr() if weights is not None else None,
+            weights.data_ptr() if weights is not None else None,
+            int(weights is not None and weights.dtype == DTYPE), preact.data.data_ptr(),
+            preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
+            g.data_ptr(), h.data_ptr(), R, N, D, E, k, _ld(grad_rows), _expert_ld(W_down),
+            W_down.stride(0), _choice_ld(weights) if weights is not None else 0, _ld(g), _ld(h),
+            _stream_handle(stream, dev)))
+    return g, h
 
 
 def grouped_weight_grad(a, g, offsets, *, out=None, stream=None):

@@ -45,10 +45,10 @@ def test_dispatch_refusals(change, code, needle):
     (dict(ldi=8), -3, "ld_in")])
 def test_combine_refusals(change, code, needle):
     a = dict(inp=P, w=P, ldw=2, ldi=16) | change
-    call("sgl_expert_combine", code, needle, a["inp"], P, a["w"], 0, P, 4, 2, 16, 8, a["ldi"],
+    call("sgl_expert_combine", code, needle, a["inp"], 0, P, a["w"], 0, P, 4, 2, 16, 8, a["ldi"],
          a["ldw"], 16, None)
     a.setdefault("gw", P)
-    call("sgl_expert_combine_grad", code, needle, P, a["inp"], P, a["w"], 0, P, a["gw"], 4, 2, 16, 8,
+    call("sgl_expert_combine_grad", code, needle, P, a["inp"], 0, P, a["w"], 0, P, a["gw"], 4, 2, 16, 8,
          16, a["ldi"], a["ldw"], 16, None)
 
 
@@ -71,8 +71,25 @@ def test_other_refusals():
          512, 16, None)
     call("sgl_grouped_fused_swiglu_save", -1, "scales", P, P, P, P, P, 0, 8, 8, 16, 16, 2, 16, 32,
          512, 16, None)
-    call("sgl_grouped_matmul", -3, "ldb", P, P, P, P, 8, 16, 32, 2, 32, 16, 512, 16, 1, None)
-    call("sgl_grouped_matmul", -3, "b_stride", P, P, P, P, 8, 16, 32, 2, 32, 16, 256, 16, 0, None)
+    call("sgl_grouped_matmul", -3, "ldb", P, P, P, P, 8, 16, 32, 2, 32, 16, 512, 16, 1, 0, None)
+    call("sgl_grouped_matmul", -3, "b_stride", P, P, P, P, 8, 16, 32, 2, 32, 16, 256, 16, 0, 1, None)
+    def grad(code, needle, **change):
+        a = dict(dy=P, slots=P, weights=P, bits=8, R=8, k=2, ldw=16, stride=256, ldr=2, ldg=32,
+                 scales=P) | change
+        call("sgl_grouped_grad_preact", code, needle, a["dy"], P, P, a["slots"], a["weights"], 0, P,
+             a["scales"], a["bits"], P, P, a["R"], 16, 16, 2, a["k"], 16, a["ldw"], a["stride"],
+             a["ldr"], a["ldg"], 16, None)
+
+    grad(-1, "dy", dy=0)
+    grad(-1, "slots", slots=0)
+    grad(-1, "weights", weights=0)
+    grad(-1, "scales", scales=0)
+    grad(-10, "bits", bits=9)
+    grad(-2, "divisor", R=9)
+    grad(-3, "ldw", ldw=8)
+    grad(-3, "w_stride", stride=128)
+    grad(-3, "ld_weights", ldr=1)
+    grad(-3, "ld_grad", ldg=16)
     call("sgl_grouped_weight_grad", -3, "c_stride", P, P, P, P, 8, 16, 16, 2, 16, 16, 16, 128, None)
     call("sgl_swiglu_grad_preact_saved", -3, "ldo", P, P, P, 8, P, None, None, 8, 16, 16, 16, 0, None)
     call("sgl_swiglu_grad_preact_saved", -4, "end", P, P, P, 8, P, None, P + 2, 8, 16, 16, 32, 0, None)
@@ -88,8 +105,8 @@ def test_other_refusals():
 def test_workspace_holds_every_part():
     T, k, E, D, N, Do = 5, 3, 7, 24, 40, 16
     n = sg.experts_swiglu_workspace_bytes(T, k, E, D, N, Do)
-    assert n >= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + Do)
-    assert n <= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + Do) + 6 * 256
+    assert n >= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + 2 * Do)
+    assert n <= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + 2 * Do) + 6 * 256
     with pytest.raises(ValueError):
         sg.experts_swiglu_workspace_bytes(1, 65, E, D, N, Do)
 
