@@ -506,9 +506,10 @@ int sgl_mgpu_destroy(sgl_mgpu* g);
  * A slot is one (token, choice) pair s = t * k + j of a router's answer ids[T, k] (int32 or
  * int64, row pitch ld_ids elements).  A slot whose id lies outside [0, E) is dropped (padding
  * tokens carry -1).  k <= 64, E <= 1024, T * k < 2^31.  All of these enqueue only, allocate
- * nothing and use no atomics: results are fixed bit for bit.  No counterpart in the reference.
+ * nothing, and their results are fixed bit for bit.  No counterpart in the reference.
  *
- * sgl_expert_order: stable counting sort of the slots by expert, one launch.
+ * sgl_expert_order: stable counting sort of the slots by expert.  `scratch`: caller-owned device
+ *   memory of sgl_expert_order_scratch_bytes bytes (0 up to 2048 slots: NULL will do), overwritten.
  *   offsets[E + 1] int32  offsets[e] = kept slots with an id below e; offsets[E] = kept slots
  *   slots[T * k]   int32  slot held by row r, -1 at and behind offsets[E]
  *   rows[T, k]     int32  row of slot (t, j), -1 if dropped (dense)
@@ -524,8 +525,10 @@ int sgl_mgpu_destroy(sgl_mgpu* g);
  *   grad_rows alone.  grad_rows may be `in` itself.
  * D must be a multiple of 8; the bf16 tensors follow the conventions above.
  */
+int64_t sgl_expert_order_scratch_bytes(int64_t T, int64_t k, int64_t E);
 int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, int64_t ld_ids,
-                     int64_t E, void* offsets, void* slots, void* rows, void* stream);
+                     int64_t E, void* offsets, void* slots, void* rows, void* scratch,
+                     int64_t scratch_bytes, void* stream);
 int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
                         int64_t R, int64_t ldx, int64_t ldo, void* stream);
 int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,

@@ -75,6 +75,7 @@ EXPORTED_SYMBOLS = (
     "sgl_mgpu_fused_swiglu",
     "sgl_mgpu_size",
     "sgl_mgpu_destroy",
+    "sgl_expert_order_scratch_bytes",
     "sgl_expert_order",
     "sgl_expert_dispatch",
     "sgl_expert_combine",
@@ -281,7 +282,9 @@ def load() -> C.CDLL:
         lib.sgl_mgpu_destroy.restype = ip
         lib.sgl_mgpu_destroy.argtypes = [vp]
         lib.sgl_expert_order.restype = ip
-        lib.sgl_expert_order.argtypes = [vp, ip, i64, i64, i64, i64, vp, vp, vp, vp]
+        lib.sgl_expert_order.argtypes = [vp, ip, i64, i64, i64, i64, vp, vp, vp, vp, i64, vp]
+        lib.sgl_expert_order_scratch_bytes.restype = i64
+        lib.sgl_expert_order_scratch_bytes.argtypes = [i64, i64, i64]
         lib.sgl_expert_dispatch.restype = ip
         lib.sgl_expert_dispatch.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, i64, vp]
         lib.sgl_expert_combine.restype = ip

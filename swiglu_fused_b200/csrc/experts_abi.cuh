@@ -349,21 +349,17 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
 // wait with griddepcontrol.wait before they touch memory).
 template <class... Args, class... Given>
 int launch_after(const char* what, void (*fn)(Args...), dim3 grid, dim3 block, int smem,
-                 unsigned cluster, void* stream, Given... args) {
+                 void* stream, Given... args) {
   cudaLaunchConfig_t lc = {};
   lc.gridDim = grid;
   lc.blockDim = block;
   lc.dynamicSmemBytes = static_cast<size_t>(smem);
   lc.stream = static_cast<cudaStream_t>(stream);
-  cudaLaunchAttribute attrs[2];
+  cudaLaunchAttribute attrs[1];
   attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attrs[0].val.programmaticStreamSerializationAllowed = 1;
-  attrs[1].id = cudaLaunchAttributeClusterDimension;
-  attrs[1].val.clusterDim.x = cluster;
-  attrs[1].val.clusterDim.y = 1;
-  attrs[1].val.clusterDim.z = 1;
   lc.attrs = attrs;
-  lc.numAttrs = cluster > 1 ? 2 : 1;
+  lc.numAttrs = 1;
   if (log_enabled()) fprintf(stderr, "[libswiglu_b200] launch sgl %s grid=%u\n", what, grid.x);
   cudaError_t e = cudaLaunchKernelEx(&lc, fn, args...);
   if (e != cudaSuccess) return fail_cuda(e, what);
@@ -400,13 +396,16 @@ int validate_row_call(int64_t T, int64_t k, int64_t D, int64_t R) {
   return SGL_OK;
 }
 
-// Threads of a token (a power of two of warps, at most 256) and CTAs for `T` tokens.
-void row_geometry(int64_t T, int nvec, const DeviceInfo* info, dim3* grid, dim3* block) {
+// Threads of a token (a power of two of warps, at most 256) and CTAs for `T` tokens, at most
+// `per_sm` per SM (16384 x 4096: dispatch 61 us without a limit and 68 us with 8; combine 73 and
+// 64 us).
+void row_geometry(int64_t T, int nvec, int64_t per_sm, const DeviceInfo* info, dim3* grid,
+                  dim3* block) {
   unsigned tx = 32;
   while (tx < 256 && tx < static_cast<unsigned>(nvec)) tx *= 2;
   *block = dim3(tx, 256 / tx, 1);
   int64_t ctas = (T + block->y - 1) / block->y;
-  const int64_t cap = static_cast<int64_t>(info->sm_count) * 8;
+  const int64_t cap = static_cast<int64_t>(info->sm_count) * per_sm;
   *grid = dim3(static_cast<unsigned>(ctas < cap ? ctas : cap), 1, 1);
 }
 
@@ -419,8 +418,35 @@ int check_bits(int bits) {
 
 extern "C" {
 
+// CTAs that order T * k slots, and the slots of each: a round of slots each if there are few, fewer
+// CTAs when the table of counts, which every CTA reads, would grow past
+// 64 Ki entries.
+static void order_plan(int64_t total, int64_t E, int* ctas, int64_t* per_cta) {
+  if (total <= sgl::kOrderRound) {
+    *ctas = 1;
+    *per_cta = total;
+    return;
+  }
+  int64_t n = (total + sgl::kOrderRound - 1) / sgl::kOrderRound;
+  const int64_t cap = (64 * 1024) / E;
+  if (n > sgl::kOrderMaxCtas) n = sgl::kOrderMaxCtas;
+  if (n > cap) n = cap;
+  *per_cta = (total + n - 1) / n;
+  *ctas = static_cast<int>((total + *per_cta - 1) / *per_cta);
+}
+
+int64_t sgl_expert_order_scratch_bytes(int64_t T, int64_t k, int64_t E) {
+  int rc = validate_routing(T, k, E);
+  if (rc) return rc;
+  int ctas;
+  int64_t per;
+  order_plan(T * k, E, &ctas, &per);
+  return ctas > 1 ? static_cast<int64_t>(ctas) * E * 4 : 0;
+}
+
 int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, int64_t ld_ids,
-                     int64_t E, void* offsets, void* slots, void* rows, void* stream) {
+                     int64_t E, void* offsets, void* slots, void* rows, void* scratch,
+                     int64_t scratch_bytes, void* stream) {
   int rc;
   if ((rc = validate_routing(T, k, E))) return rc;
   if ((rc = validate_words(ids, "ids", ids_are_int64 ? 8 : 4)) ||
@@ -430,24 +456,34 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
   if (ld_ids < k)
     return fail(SGL_ERR_BAD_STRIDE, "ld_ids=%lld is smaller than k=%lld",
                 static_cast<long long>(ld_ids), static_cast<long long>(k));
+  sgl::OrderParams p;
+  int ctas;
+  order_plan(T * k, E, &ctas, &p.per_cta);
+  if (ctas > 1) {
+    if ((rc = validate_words(scratch, "scratch", 4))) return rc;
+    if (scratch_bytes < static_cast<int64_t>(ctas) * E * 4)
+      return fail(SGL_ERR_BAD_ARGUMENT, "scratch holds %lld bytes, %lld needed",
+                  static_cast<long long>(scratch_bytes), static_cast<long long>(ctas) * E * 4);
+  }
   DeviceInfo* info = nullptr;
   if ((rc = check_device(&info))) return rc;
   const int smem = sgl::order_smem_bytes(static_cast<int>(E));
-  {
+  if (smem > 48 * 1024) {
     int dev = 0;
     if ((rc = current_device(&dev))) return rc;
     std::lock_guard<std::mutex> lock(g_dev_mutex);
     ExpertDevice& d = g_expert_devices[dev];
     if (!d.order_ready) {
-      cudaError_t e = cudaFuncSetAttribute(
-          reinterpret_cast<const void*>(sgl::expert_order_kernel),
-          cudaFuncAttributeMaxDynamicSharedMemorySize,
-          sgl::order_smem_bytes(sgl::kOrderMaxExperts));
+      const int most = sgl::order_smem_bytes(sgl::kOrderMaxExperts);
+      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_order_kernel),
+                                           cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+      if (e == cudaSuccess)
+        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_count_kernel),
+                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
       if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(expert_order)");
       d.order_ready = true;
     }
   }
-  sgl::OrderParams p;
   p.ids = ids;
   p.ld_ids = ld_ids;
   p.total = T * k;
@@ -457,9 +493,15 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
   p.offsets = static_cast<int*>(offsets);
   p.slots = static_cast<int*>(slots);
   p.rows = static_cast<int*>(rows);
-  const unsigned ctas = p.total > 4 * sgl::kOrderThreads ? sgl::kOrderCluster : 1;
-  return launch_after("expert_order", sgl::expert_order_kernel, dim3(ctas), dim3(sgl::kOrderThreads),
-                      smem, ctas, stream, p);
+  p.counts = static_cast<int*>(scratch);
+  const dim3 threads(sgl::kOrderThreads);
+  if (ctas == 1)
+    return launch_after("expert_order", sgl::expert_order_kernel, dim3(1), threads, smem, stream, p);
+  if ((rc = launch_after("expert_count", sgl::expert_count_kernel, dim3(ctas), threads, smem, stream,
+                         p)))
+    return rc;
+  return launch_after("expert_place", sgl::expert_place_kernel, dim3(ctas), threads,
+                      (2 * static_cast<int>(E) + 40) * 4, stream, p);
 }
 
 int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
@@ -484,8 +526,8 @@ int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, i
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, info, &grid, &block);
-  return launch_after("expert_dispatch", sgl::expert_dispatch_kernel, grid, block, 0, 1, stream, p);
+  row_geometry(T, p.nvec, 4096, info, &grid, &block);
+  return launch_after("expert_dispatch", sgl::expert_dispatch_kernel, grid, block, 0, stream, p);
 }
 
 int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
@@ -520,10 +562,13 @@ int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const vo
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, info, &grid, &block);
+  row_geometry(T, p.nvec, 8, info, &grid, &block);
   return launch_after("expert_combine",
-                      in_is_f32 ? sgl::expert_combine_kernel<true> : sgl::expert_combine_kernel<false>,
-                      grid, block, 0, 1, stream, p);
+                      k <= 2 ? (in_is_f32 ? sgl::expert_combine_kernel<true, 2, 2>
+                                          : sgl::expert_combine_kernel<false, 2, 2>)
+                             : (in_is_f32 ? sgl::expert_combine_kernel<true, 1, 4>
+                                          : sgl::expert_combine_kernel<false, 1, 4>),
+                      grid, block, 0, stream, p);
 }
 
 int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32, const void* rows,
@@ -567,11 +612,13 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32,
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, info, &grid, &block);
+  row_geometry(T, p.nvec, 8, info, &grid, &block);
   return launch_after("expert_combine_grad",
-                      in_is_f32 ? sgl::expert_combine_grad_kernel<true>
-                                : sgl::expert_combine_grad_kernel<false>,
-                      grid, block, 0, 1, stream, p);
+                      k <= 2 ? (in_is_f32 ? sgl::expert_combine_grad_kernel<true, 2, 2>
+                                          : sgl::expert_combine_grad_kernel<false, 2, 2>)
+                             : (in_is_f32 ? sgl::expert_combine_grad_kernel<true, 1, 4>
+                                          : sgl::expert_combine_grad_kernel<false, 1, 4>),
+                      grid, block, 0, stream, p);
 }
 
 int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int64_t* scale_bytes,
@@ -801,7 +848,7 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
   if (blocks > cap) blocks = cap;
   return launch_after("grad_preact_saved",
                       bits == 8 ? sgl::grad_preact_saved_kernel<8> : sgl::grad_preact_saved_kernel<16>,
-                      dim3(static_cast<unsigned>(blocks)), dim3(256), 0, 1, stream, p);
+                      dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
 }
 
 // ---- the expert layer at inference, one call ----
@@ -809,7 +856,7 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct ExpertsWorkspace {
-  int64_t offsets, slots, rows, xs, h, ys, total;
+  int64_t offsets, slots, rows, scratch, scratch_bytes, xs, h, ys, total;
 };
 
 static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
@@ -826,6 +873,9 @@ static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t
   at += align256(R * 4);
   w->rows = at;
   at += align256(R * 4);
+  w->scratch = at;
+  w->scratch_bytes = sgl_expert_order_scratch_bytes(T, k, E);
+  at += align256(w->scratch_bytes);
   w->xs = at;
   at += align256(R * D * 2);
   w->h = at;
@@ -873,7 +923,7 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t R = T * k;
   if ((rc = sgl_expert_order(ids, ids_are_int64, T, k, ld_ids, E, ws + l.offsets, ws + l.slots,
-                             ws + l.rows, stream)) ||
+                             ws + l.rows, ws + l.scratch, l.scratch_bytes, stream)) ||
       (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream)) ||
       (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
                                      w_stride, N, stream)) ||

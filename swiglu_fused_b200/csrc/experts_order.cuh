@@ -6,7 +6,8 @@
 //   offsets[e]  = number of kept slots with an id below e      (offsets[E] = kept slots)
 //   slots[r]    = slot that row r holds, -1 for rows at and behind offsets[E]
 //   rows[t, j]  = row of slot (t, j), -1 if dropped
-// Nothing here uses atomics: every result is a fixed function of the inputs, bit for bit.
+// Every result is a fixed function of the inputs, bit for bit (the only atomics are integer sums
+// in shared memory).
 #pragma once
 
 #include <cstdint>
@@ -20,26 +21,28 @@ namespace sgl {
 constexpr int kOrderThreads = 1024;
 constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kOrderMaxExperts = 1024;
-constexpr int kOrderCluster = 8;       // CTAs of the long form, one thread-block cluster
-constexpr int kOrderUnroll = 4;
+constexpr int kOrderSteps = 2;                               // slots of a thread in one round
+constexpr int kOrderRound = kOrderThreads * kOrderSteps;     // slots of a CTA in one round
+constexpr int kOrderMaxCtas = 128;
 
-// Shared memory: a count per (warp, expert), and three words per expert.
-constexpr int order_smem_bytes(int E) { return (kOrderWarps + 3) * E * 4 + 64 * 4; }
+// Shared memory: a count per (warp, expert), two words per expert, and the scan's scratch.
+constexpr int order_smem_bytes(int E) { return (kOrderWarps + 2) * E * 4 + 40 * 4; }
 
 struct OrderParams {
   const void* ids;
   int64_t ld_ids;      // row pitch of ids, elements
   int64_t total;       // T * k slots
+  int64_t per_cta;     // slots of a CTA (a contiguous range)
   int k, E;
   int ids64;           // ids are int64 (else int32)
   int* offsets;        // [E + 1]
   int* slots;          // [T * k]
   int* rows;           // [T * k]
+  int* counts;         // several CTAs: [CTAs][E], kept slots of each CTA and expert
 };
 
-// Expert of slot s, or -1 (dropped, or past the last slot).
+// Expert of slot s, or -1 (dropped).
 __device__ __forceinline__ int order_key(const OrderParams& p, int64_t s) {
-  if (s >= p.total) return -1;
   int64_t at = s;
   if (p.ld_ids != p.k) {
     const int64_t t = s / p.k;
@@ -50,143 +53,212 @@ __device__ __forceinline__ int order_key(const OrderParams& p, int64_t s) {
   return (id >= 0 && id < p.E) ? static_cast<int>(id) : -1;
 }
 
-// One launch: the CTAs of one cluster (or a single CTA) each own a contiguous range of slots,
-// and so does each warp inside its CTA.  Warps count their slots per expert (match.any groups
-// the 32 slots of a step, one lane per group adds), the counts are turned into the first row of
-// every (expert, CTA, warp) - CTA totals are exchanged through distributed shared memory - and
-// the warps walk their slots a second time to hand out the rows in slot order.
-//
-// Bound by latency: 2 x (slots / (CTAs * 1024)) steps of a match and a shared-memory update.
-__global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const OrderParams p) {
-  extern __shared__ int order_smem[];
-  const int E = p.E;
-  int* count = order_smem;                         // [kOrderWarps][E]
-  int* cta_total = count + kOrderWarps * E;        // [E], read by the other CTAs
-  int* base = cta_total + E;                       // [E]
-  int* scan = base + E;                            // [E]
-  int* warp_sum = scan + E;                        // [33]
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  uint32_t nctas = gridDim.x, rank = blockIdx.x;   // the grid is one cluster
-
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-
-  for (int i = tid; i < kOrderWarps * E; i += kOrderThreads) count[i] = 0;
-  __syncthreads();
-
-  // slots of this warp: a multiple of 32, contiguous
-  const int64_t per_warp =
-      (p.total + static_cast<int64_t>(nctas) * kOrderThreads - 1) /
-      (static_cast<int64_t>(nctas) * kOrderThreads) * 32;
-  const int64_t first = (static_cast<int64_t>(rank) * kOrderWarps + warp) * per_warp;
-  int64_t last = first + per_warp;
-  if (last > p.total) last = p.total;
-  int* my_count = count + warp * E;
-
-  for (int64_t s0 = first; s0 < last; s0 += 32 * kOrderUnroll) {
-    int key[kOrderUnroll];
-#pragma unroll
-    for (int u = 0; u < kOrderUnroll; ++u) {
-      const int64_t s = s0 + u * 32 + lane;
-      key[u] = s < last ? order_key(p, s) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kOrderUnroll; ++u) {
-      const unsigned same = __match_any_sync(0xffffffffu, key[u]);
-      if (key[u] >= 0 && lane == __ffs(same) - 1) my_count[key[u]] += __popc(same);
-      __syncwarp();
-    }
+// Lanes whose key equals this lane's: a ballot per bit (all lanes of the warp).  768 slots of 128
+// experts: 3.1 us for the whole launch, 3.5 us with one match.any instead.
+__device__ __forceinline__ unsigned same_key(int key, int bits) {
+  unsigned same = 0xffffffffu;
+  for (int b = 0; b < bits; ++b) {
+    const bool one = (key >> b) & 1;
+    const unsigned ones = __ballot_sync(0xffffffffu, one);
+    same &= one ? ones : ~ones;
   }
-  __syncthreads();
+  return same;
+}
 
-  // counts -> exclusive sums over the warps of this CTA; totals for the cluster
-  for (int e = tid; e < E; e += kOrderThreads) {
-    int sum = 0;
-#pragma unroll 8
-    for (int w = 0; w < kOrderWarps; ++w) {
-      const int c = count[w * E + e];
-      count[w * E + e] = sum;
-      sum += c;
-    }
-    cta_total[e] = sum;
+// Ranks the slots [first, last), at most kOrderRound, inside their expert: key[u] / rank[u] are
+// this thread's u-th slot (index slot_of(u)), rank counting the CTA's earlier slots of the same
+// expert, total[e] of earlier rounds included; total[e] is advanced.  A warp owns a contiguous run
+// of slots and takes 32 at a time: lanes with equal experts find each other, one of them adds
+// to the warp's counts; then the counts are summed over the warps.
+struct OrderRound {
+  int key[kOrderSteps], rank[kOrderSteps];
+  int64_t base;        // first slot of this warp
+  int steps;
+  __device__ __forceinline__ int64_t slot_of(int u) const {
+    return base + u * 32 + (threadIdx.x & 31);
   }
-  if (nctas > 1) {
-    ptx::cluster_sync();
-  } else {
+  __device__ __forceinline__ void run(const OrderParams& p, int64_t first, int64_t last, int* count,
+                                      int* total) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, E = p.E;
+    steps = static_cast<int>((last - first + kOrderThreads - 1) / kOrderThreads);
+    base = first + static_cast<int64_t>(warp) * steps * 32;
+    int* mine = count + warp * E;
+    const int bits = 33 - __clz(E);   // of a key in [-1, E)
+#pragma unroll
+    for (int u = 0; u < kOrderSteps; ++u) {
+      const int64_t s = slot_of(u);
+      key[u] = (u < steps && s < last) ? order_key(p, s) : -1;
+    }
+    for (int i = tid; i < kOrderWarps * E; i += kOrderThreads) count[i] = 0;
     __syncthreads();
-  }
-  // (E <= kOrderThreads: one expert per thread from here)
-  int before = 0, total = 0;
-  if (tid < E) {
-    if (nctas > 1) {
-      const uint32_t mine = ptx::smem_u32(cta_total + tid);
-      for (uint32_t c = 0; c < nctas; ++c) {
-        int v;
-        asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(ptx::mapa(mine, c)));
-        if (c < rank) before += v;
-        total += v;
+#pragma unroll
+    for (int u = 0; u < kOrderSteps; ++u) {
+      if (u < steps) {
+        const unsigned same = same_key(key[u], bits);
+        if (key[u] >= 0) rank[u] = mine[key[u]] + __popc(same & ((1u << lane) - 1u));
+        __syncwarp();
+        if (key[u] >= 0 && lane == __ffs(same) - 1) mine[key[u]] += __popc(same);
+        __syncwarp();
       }
-    } else {
-      total = cta_total[tid];
     }
+    __syncthreads();
+    for (int e = tid; e < E; e += kOrderThreads) {
+      int sum = total[e];
+#pragma unroll 8
+      for (int w = 0; w < kOrderWarps; ++w) {
+        const int c = count[w * E + e];
+        count[w * E + e] = sum;
+        sum += c;
+      }
+      total[e] = sum;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int u = 0; u < kOrderSteps; ++u)
+      if (key[u] >= 0) rank[u] += mine[key[u]];
   }
-  // exclusive scan of the totals over the experts
-  int inc = total;
+};
+
+// Exclusive scan over the experts (thread e holds v; E <= kOrderThreads): its result, and the sum
+// of all in *sum.  scratch: 33 words.
+__device__ __forceinline__ int order_scan(int v, int* scratch, int* sum) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int inc = v;
 #pragma unroll
   for (int d = 1; d < 32; d <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, d);
-    if (lane >= d) inc += v;
+    const int n = __shfl_up_sync(0xffffffffu, inc, d);
+    if (lane >= d) inc += n;
   }
-  if (lane == 31) warp_sum[warp] = inc;
+  if (lane == 31) scratch[warp] = inc;
   __syncthreads();
   if (warp == 0) {
-    const int mine = warp_sum[lane];
+    const int mine = scratch[lane];
     int w = mine;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, w, d);
-      if (lane >= d) w += v;
+      const int n = __shfl_up_sync(0xffffffffu, w, d);
+      if (lane >= d) w += n;
     }
-    warp_sum[lane] = w - mine;
-    if (lane == 31) warp_sum[32] = w;
+    scratch[lane] = w - mine;
+    if (lane == 31) scratch[32] = w;
   }
   __syncthreads();
-  const int start = warp_sum[warp] + inc - total;
-  const int kept = warp_sum[32];
-  if (tid < E) {
-    base[tid] = start + before;
-    if (rank == 0) p.offsets[tid] = start;
-  }
-  if (rank == 0 && tid == 0) p.offsets[E] = kept;
-  __syncthreads();
+  *sum = scratch[32];
+  return scratch[warp] + inc - v;
+}
 
-  for (int64_t s0 = first; s0 < last; s0 += 32 * kOrderUnroll) {
-    int key[kOrderUnroll];
+// Up to kOrderRound slots: everything in one CTA.  Bound by latency (a load, the ballots of each 32
+// slots, a few barriers).
+__global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const OrderParams p) {
+  extern __shared__ int order_smem[];
+  const int E = p.E, tid = threadIdx.x;
+  int* count = order_smem;
+  int* total = count + kOrderWarps * E;
+  int* start = total + E;
+  int* scratch = start + E;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int e = tid; e < E; e += kOrderThreads) total[e] = 0;
+  OrderRound r;
+  r.run(p, 0, p.total, count, total);
+  int kept;
+  const int first = order_scan(tid < E ? total[tid] : 0, scratch, &kept);
+  if (tid < E) {
+    start[tid] = first;
+    p.offsets[tid] = first;
+  }
+  if (tid == 0) p.offsets[E] = kept;
+  __syncthreads();
 #pragma unroll
-    for (int u = 0; u < kOrderUnroll; ++u) {
-      const int64_t s = s0 + u * 32 + lane;
-      key[u] = s < last ? order_key(p, s) : -1;
-    }
-#pragma unroll
-    for (int u = 0; u < kOrderUnroll; ++u) {
-      const int64_t s = s0 + u * 32 + lane;
-      const unsigned same = __match_any_sync(0xffffffffu, key[u]);
-      int row = -1;
-      if (key[u] >= 0) {
-        row = base[key[u]] + my_count[key[u]] + __popc(same & ((1u << lane) - 1u));
-        p.slots[row] = static_cast<int>(s);
-      }
-      __syncwarp();
-      if (key[u] >= 0 && lane == __ffs(same) - 1) my_count[key[u]] += __popc(same);
-      if (s < last) p.rows[s] = row;
-      __syncwarp();
+  for (int u = 0; u < kOrderSteps; ++u) {
+    const int64_t s = r.slot_of(u);
+    if (u < r.steps && s < p.total) {
+      const int row = r.key[u] >= 0 ? start[r.key[u]] + r.rank[u] : -1;
+      p.rows[s] = row;
+      if (row >= 0) p.slots[row] = static_cast<int>(s);
     }
   }
-  for (int64_t r = kept + static_cast<int64_t>(rank) * kOrderThreads + tid; r < p.total;
-       r += static_cast<int64_t>(nctas) * kOrderThreads)
-    p.slots[r] = -1;
-  // no CTA leaves while another may still read its totals
-  if (nctas > 1) ptx::cluster_sync();
+  for (int64_t i = kept + tid; i < p.total; i += kOrderThreads) p.slots[i] = -1;
+}
+
+// More slots: one range per CTA.  The first kernel leaves every slot's rank inside its CTA in
+// `rows` and the CTA's counts in `counts`; the second adds up the counts of the CTAs before it
+// (all of them read the whole table, CTAs * E words from L2) and places its slots.  262144 slots
+// of 256 experts: 10.6 us for both, where one cluster of 8 CTAs took 66 us, bound by the
+// scattered stores that 8 SMs can issue.
+__global__ void __launch_bounds__(kOrderThreads, 1) expert_count_kernel(const OrderParams p) {
+  extern __shared__ int order_smem[];
+  const int E = p.E, tid = threadIdx.x;
+  int* count = order_smem;
+  int* total = count + kOrderWarps * E;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int e = tid; e < E; e += kOrderThreads) total[e] = 0;
+  const int64_t lo = blockIdx.x * p.per_cta;
+  const int64_t hi = lo + p.per_cta < p.total ? lo + p.per_cta : p.total;
+  for (int64_t s0 = lo; s0 < hi; s0 += kOrderRound) {
+    OrderRound r;
+    r.run(p, s0, s0 + kOrderRound < hi ? s0 + kOrderRound : hi, count, total);
+#pragma unroll
+    for (int u = 0; u < kOrderSteps; ++u) {
+      const int64_t s = r.slot_of(u);
+      if (u < r.steps && s < hi) p.rows[s] = r.key[u] >= 0 ? r.rank[u] : -1;
+    }
+    __syncthreads();
+  }
+  __syncthreads();
+  for (int e = tid; e < E; e += kOrderThreads)
+    p.counts[static_cast<int64_t>(blockIdx.x) * E + e] = total[e];
+}
+
+__global__ void __launch_bounds__(kOrderThreads, 1) expert_place_kernel(const OrderParams p) {
+  extern __shared__ int order_smem[];
+  const int E = p.E, tid = threadIdx.x;
+  int* start = order_smem;       // [E] kept slots of earlier CTAs, then the first row
+  int* total = start + E;        // [E]
+  int* scratch = total + E;
+  const int ctas = gridDim.x, cta = blockIdx.x;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  for (int e = tid; e < E; e += kOrderThreads) start[e] = total[e] = 0;
+  __syncthreads();
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  {
+    // thread (group, e): every group adds up every n-th CTA's counts of expert e
+    const int groups = kOrderThreads / E, e = tid % E, g = tid / E;
+    if (g < groups) {
+      int before = 0, all = 0;
+#pragma unroll 4
+      for (int c = g; c < ctas; c += groups) {
+        const int n = p.counts[static_cast<int64_t>(c) * E + e];
+        all += n;
+        if (c < cta) before += n;
+      }
+      atomicAdd(&total[e], all);
+      atomicAdd(&start[e], before);
+    }
+  }
+  __syncthreads();
+  int kept;
+  const int first = order_scan(tid < E ? total[tid] : 0, scratch, &kept);
+  if (tid < E) {
+    start[tid] += first;
+    if (cta == 0) p.offsets[tid] = first;
+  }
+  if (cta == 0 && tid == 0) p.offsets[E] = kept;
+  __syncthreads();
+  const int64_t lo = cta * p.per_cta;
+  const int64_t hi = lo + p.per_cta < p.total ? lo + p.per_cta : p.total;
+  for (int64_t s = lo + tid; s < hi; s += kOrderThreads) {
+    const int rank = p.rows[s];
+    if (rank >= 0) {
+      const int row = start[order_key(p, s)] + rank;
+      p.rows[s] = row;
+      p.slots[row] = static_cast<int>(s);
+    }
+  }
+  for (int64_t i = kept + static_cast<int64_t>(cta) * kOrderThreads + tid; i < p.total;
+       i += static_cast<int64_t>(ctas) * kOrderThreads)
+    p.slots[i] = -1;
 }
 
 // ---------------------------------------------------------------- rows out and back
@@ -268,19 +340,32 @@ __device__ __forceinline__ int row_of(const RowParams& p, int64_t t, int j) {
   return (r >= 0 && r < p.R) ? r : -1;
 }
 
+// kVecs vectors of each of kBatch rows are a thread's loads in flight.  Four in all is what 64
+// registers (four CTAs on an SM; three for fp32 rows) carry: 2 x 2 up to two choices a token, 1 x 4
+// beyond.  16384
+// tokens x 2 choices x 4096 columns: combine 64 us (6.3 TB/s) so and 77 us with 1 x 4; 4096 tokens
+// x 6 choices x 2048: 28 us with 2 x 2 and 23 us with 1 x 4.
+
 // out[rows[t, j]] = x[t]: x is read once, each of its rows written once.
 __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p) {
+  constexpr int kVecs = 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tx = blockDim.x;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
        t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    const uint4* src = reinterpret_cast<const uint4*>(
-        static_cast<const __nv_bfloat16*>(p.in) + t * p.ld_in);
-    for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
-      const uint4 val = src[v];
+    for (int v0 = threadIdx.x; v0 < p.nvec; v0 += kVecs * tx) {
+      Vec8<false> val[kVecs];
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (v0 + i * tx < p.nvec) val[i].load(p.in, t, p.ld_in, v0 + i * tx);
       for (int j = 0; j < p.k; ++j) {
         const int r = row_of(p, t, j);
-        if (r >= 0) reinterpret_cast<uint4*>(p.out + r * p.ld_out)[v] = val;
+        if (r < 0) continue;
+        uint4* dst = reinterpret_cast<uint4*>(p.out + r * p.ld_out);
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i)
+          if (v0 + i * tx < p.nvec) dst[v0 + i * tx] = val[i].v[0];
       }
     }
   }
@@ -288,102 +373,138 @@ __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p)
 
 // out[t] = sum_j weights[t, j] * rows[rows[t, j]], fp32 in the order of j, rounded once.  A
 // dropped choice adds nothing (its weight is not read either); a token without any is zero.
-template <bool kF32>
-__global__ void __launch_bounds__(256) expert_combine_kernel(const RowParams p) {
+template <bool kF32, int kVecs, int kBatch>
+__global__ void __launch_bounds__(256, kF32 ? 3 : 4) expert_combine_kernel(const RowParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  constexpr int kBatch = 4;   // rows whose loads are in flight together
+  const int tx = blockDim.x;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
        t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
-      float acc[8] = {};
+    for (int v0 = threadIdx.x; v0 < p.nvec; v0 += kVecs * tx) {
+      float acc[kVecs][8] = {};
       for (int j0 = 0; j0 < p.k; j0 += kBatch) {
-        Vec8<kF32> val[kBatch];
+        Vec8<kF32> val[kBatch][kVecs];
         float w[kBatch];
-        bool on[kBatch];
+        int r[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) r[u] = j0 + u < p.k ? row_of(p, t, j0 + u) : -1;
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          const int j = j0 + u;
-          const int r = j < p.k ? row_of(p, t, j) : -1;
-          on[u] = r >= 0;
-          if (on[u]) {
-            val[u].load(p.in, r, p.ld_in, v);
-            w[u] = load_weight(p, t, j);
-          }
+          if (r[u] < 0) continue;
+          w[u] = load_weight(p, t, j0 + u);
+#pragma unroll
+          for (int i = 0; i < kVecs; ++i)
+            if (v0 + i * tx < p.nvec) val[u][i].load(p.in, r[u], p.ld_in, v0 + i * tx);
         }
 #pragma unroll
         for (int u = 0; u < kBatch; ++u) {
-          if (on[u]) {
-            float f[8];
-            val[u].get(f);
+          if (r[u] < 0) continue;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] = fmaf(w[u], f[i], acc[i]);
+          for (int i = 0; i < kVecs; ++i) {
+            float f[8];
+            val[u][i].get(f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) acc[i][c] = fmaf(w[u], f[c], acc[i][c]);
           }
         }
       }
-      reinterpret_cast<uint4*>(p.out + t * p.ld_out)[v] = f32_to_bf16x8(acc);
+#pragma unroll
+      for (int i = 0; i < kVecs; ++i)
+        if (v0 + i * tx < p.nvec)
+          reinterpret_cast<uint4*>(p.out + t * p.ld_out)[v0 + i * tx] = f32_to_bf16x8(acc[i]);
     }
   }
 }
 
 // Gradients of the weighted sum: grad_rows[r] = w * grad_out[t] (w = 1 without weights),
-// grad_weights[t, j] = <grad_out[t], rows[r]> (0 for a dropped choice), in one pass over the rows.  The dot product is
-// summed in fp32: by thread over its columns, then over the threads in a fixed tree.
-template <bool kF32>
-__global__ void __launch_bounds__(256) expert_combine_grad_kernel(const RowParams p) {
-  __shared__ float part[8];
+// grad_weights[t, j] = <grad_out[t], rows[r]> (0 for a dropped choice), in one pass over the rows.
+// The dot product is summed in fp32: by thread over its columns, then over the threads in a fixed
+// order.
+template <bool kF32, int kVecs, int kBatch>
+__global__ void __launch_bounds__(256, kF32 ? 3 : 4) expert_combine_grad_kernel(const RowParams p) {
+  __shared__ float part[kBatch][8];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int warps = blockDim.x / 32;                       // warps of one token
+  const int tx = blockDim.x, warps = tx / 32;              // threads and warps of one token
   const int warp_in_token = threadIdx.x / 32, lane = threadIdx.x & 31;
   // every thread of the CTA makes the same number of steps (there are barriers inside)
   for (int64_t t0 = static_cast<int64_t>(blockIdx.x) * blockDim.y; t0 < p.T;
        t0 += static_cast<int64_t>(gridDim.x) * blockDim.y) {
     const int64_t t = t0 + threadIdx.y;
     const bool live = t < p.T;
-    const uint4* dy = reinterpret_cast<const uint4*>(
-        static_cast<const __nv_bfloat16*>(p.in) + (live ? t : 0) * p.ld_in);
-    for (int j = 0; j < p.k; ++j) {
-      const int r = live ? row_of(p, t, j) : -1;
-      float dot = 0.f;
-      if (r >= 0) {
-        const float w = load_weight(p, t, j);
-        uint4* dst = reinterpret_cast<uint4*>(p.out + r * p.ld_out);
-        for (int v = threadIdx.x; v < p.nvec; v += blockDim.x) {
-          float g[8];
-          bf16x8_to_f32(dy[v], g);
-          if (p.in2) {
-            Vec8<kF32> val;
-            float y[8];
-            val.load(p.in2, r, p.ld_in2, v);
-            val.get(y);
+    for (int j0 = 0; j0 < p.k; j0 += kBatch) {
+      int r[kBatch];
+      float w[kBatch], dot[kBatch];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) dot = fmaf(g[i], y[i], dot);
+      for (int u = 0; u < kBatch; ++u) {
+        r[u] = live && j0 + u < p.k ? row_of(p, t, j0 + u) : -1;
+        w[u] = r[u] >= 0 ? load_weight(p, t, j0 + u) : 0.f;
+        dot[u] = 0.f;
+      }
+      for (int v0 = threadIdx.x; live && v0 < p.nvec; v0 += kVecs * tx) {
+        Vec8<false> g[kVecs];
+        Vec8<kF32> y[kBatch][kVecs];
+#pragma unroll
+        for (int i = 0; i < kVecs; ++i) {
+          if (v0 + i * tx >= p.nvec) continue;
+          g[i].load(p.in, t, p.ld_in, v0 + i * tx);
+          if (p.in2 != nullptr) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u)
+              if (r[u] >= 0) y[u][i].load(p.in2, r[u], p.ld_in2, v0 + i * tx);
           }
+        }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] *= w;
-          dst[v] = f32_to_bf16x8(g);
+        for (int i = 0; i < kVecs; ++i) {
+          if (v0 + i * tx >= p.nvec) continue;
+          float gf[8];
+          g[i].get(gf);
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) {
+            if (r[u] < 0) continue;
+            if (p.in2 != nullptr) {
+              float yf[8];
+              y[u][i].get(yf);
+#pragma unroll
+              for (int c = 0; c < 8; ++c) dot[u] = fmaf(gf[c], yf[c], dot[u]);
+            }
+            float o[8];
+#pragma unroll
+            for (int c = 0; c < 8; ++c) o[c] = gf[c] * w[u];
+            reinterpret_cast<uint4*>(p.out + r[u] * p.ld_out)[v0 + i * tx] = f32_to_bf16x8(o);
+          }
         }
       }
+      if (p.grad_weights == nullptr) continue;
 #pragma unroll
-      for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
+      for (int u = 0; u < kBatch; ++u) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) dot[u] += __shfl_xor_sync(0xffffffffu, dot[u], d);
+      }
       if (warps > 1) {
-        if (lane == 0) part[threadIdx.y * warps + warp_in_token] = dot;
-        __syncthreads();
-        if (threadIdx.x == 0) {
-          dot = 0.f;
-          for (int w = 0; w < warps; ++w) dot += part[threadIdx.y * warps + w];
+        if (lane == 0) {
+#pragma unroll
+          for (int u = 0; u < kBatch; ++u) part[u][threadIdx.y * warps + warp_in_token] = dot[u];
         }
         __syncthreads();
       }
-      if (live && threadIdx.x == 0 && p.grad_weights) {
-        const int64_t at = t * p.k + j;
-        if (p.w_bf16) {
-          reinterpret_cast<__nv_bfloat16*>(p.grad_weights)[at] = __float2bfloat16_rn(dot);
+      if (live && threadIdx.x < kBatch && j0 + threadIdx.x < p.k) {
+        const int u = threadIdx.x;
+        float sum = 0.f;
+        if (warps > 1) {
+          for (int i = 0; i < warps; ++i) sum += part[u][threadIdx.y * warps + i];
         } else {
-          reinterpret_cast<float*>(p.grad_weights)[at] = dot;
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) sum = u == i ? dot[i] : sum;
+        }
+        const int64_t at = t * p.k + j0 + u;
+        if (p.w_bf16) {
+          reinterpret_cast<__nv_bfloat16*>(p.grad_weights)[at] = __float2bfloat16_rn(sum);
+        } else {
+          reinterpret_cast<float*>(p.grad_weights)[at] = sum;
         }
       }
+      if (warps > 1) __syncthreads();
     }
   }
 }

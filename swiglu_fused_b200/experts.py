@@ -22,17 +22,48 @@ rows, checks before anything is launched, torch's current stream unless ``stream
 """
 from __future__ import annotations
 
-import ctypes as C
 from typing import NamedTuple
 
 import torch
 
 from . import _lib
-from .ops import (DTYPE, _check_matrix, _ld, _on_device, _prep_out, _same_device, _stream_handle,
+from .ops import (DTYPE, _check_matrix, _ld, _prep_out, _same_device, _stream_handle,
                   stream_context)
 
 MAX_EXPERTS = 1024
 MAX_CHOICES = 64
+_ONE_CTA_SLOTS = 2048      # up to here sgl_expert_order needs no scratch
+
+
+class _launch:
+    """``with _launch(stream, dev) as handle:`` makes ``dev`` the current device and ``stream``, if one
+    is given, torch's current stream (so that allocations inside are ordered with the launch),
+    and yields the raw stream handle.  Costs next to nothing where neither has to change."""
+
+    __slots__ = ("stream", "dev", "prev", "ctx")
+
+    def __init__(self, stream, dev: torch.device):
+        self.stream = stream
+        self.dev = dev
+        self.prev = -1
+        self.ctx = None
+
+    def __enter__(self) -> int:
+        cur = torch.cuda.current_device()
+        if cur != self.dev.index:
+            self.prev = cur
+            torch.cuda.set_device(self.dev.index)
+        if self.stream is not None:
+            self.ctx = stream_context(self.stream, self.dev)
+            self.ctx.__enter__()
+        return _stream_handle(self.stream, self.dev)
+
+    def __exit__(self, *exc):
+        if self.ctx is not None:
+            self.ctx.__exit__(*exc)
+        if self.prev >= 0:
+            torch.cuda.set_device(self.prev)
+        return False
 
 
 class ExpertOrder(NamedTuple):
@@ -190,18 +221,24 @@ def expert_order(expert_ids, num_experts: int, *, stream=None) -> ExpertOrder:
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"num_experts={E} outside [1, {MAX_EXPERTS}]")
     dev = expert_ids.device
-    with stream_context(stream, dev):
-        buf = torch.empty(E + 1 + 2 * T * k, dtype=torch.int32, device=dev)
-        offsets, slots, rows = buf.split((E + 1, T * k, T * k))
+    R = T * k
+    with _launch(stream, dev) as handle:
+        offsets = torch.empty(E + 1, dtype=torch.int32, device=dev)
+        slots = torch.empty(R, dtype=torch.int32, device=dev)
+        rows = torch.empty((T, k), dtype=torch.int32, device=dev)
         if T == 0:
             offsets.zero_()
-            return ExpertOrder(offsets, slots, rows.view(0, k))
-    with _on_device(dev):
-        _lib.check(_lib.load().sgl_expert_order(
-            expert_ids.data_ptr(), int(expert_ids.dtype == torch.int64), T, k,
-            _choice_ld(expert_ids), E, offsets.data_ptr(), slots.data_ptr(), rows.data_ptr(),
-            _stream_handle(stream, dev)))
-    return ExpertOrder(offsets, slots, rows.view(T, k))
+            return ExpertOrder(offsets, slots, rows)
+        lib = _lib.load()
+        need, scratch = 0, None
+        if R > _ONE_CTA_SLOTS:
+            need = lib.sgl_expert_order_scratch_bytes(T, k, E)
+            scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        _lib.check(lib.sgl_expert_order(
+            expert_ids.data_ptr(), expert_ids.dtype == torch.int64, T, k, _choice_ld(expert_ids), E,
+            offsets.data_ptr(), slots.data_ptr(), rows.data_ptr(),
+            scratch.data_ptr() if scratch is not None else None, need, handle))
+    return ExpertOrder(offsets, slots, rows)
 
 
 def expert_dispatch(x, order: ExpertOrder, *, out=None, stream=None):
@@ -216,12 +253,11 @@ def expert_dispatch(x, order: ExpertOrder, *, out=None, stream=None):
     dev = _same_device(("x", x), ("order.rows", order.rows))
     if T == 0:
         return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         o = _prep_out(out, T * k, D, dev)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_expert_dispatch(
             x.data_ptr(), order.rows.data_ptr(), o.data_ptr(), T, k, D, T * k, _ld(x), _ld(o),
-            _stream_handle(stream, dev)))
+            handle))
     return o
 
 
@@ -248,15 +284,14 @@ def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=N
     dev = _same_device(*named)
     if T == 0:
         return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         o = _prep_out(out, T, D, dev)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_expert_combine(
             rows.data_ptr(), int(rows.dtype == torch.float32), order.rows.data_ptr(),
             weights.data_ptr() if weights is not None else None,
             int(weights is not None and weights.dtype == DTYPE), o.data_ptr(), T, k, D, T * k,
             _ld(rows), _choice_ld(weights) if weights is not None else 0, _ld(o),
-            _stream_handle(stream, dev)))
+            handle))
     return o
 
 
@@ -283,19 +318,17 @@ def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, weighted
     _multiple_of_8(D=D)
     _check_weights(weights, T, k)
     dev = _same_device(*named)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         gw = torch.empty((T, k), dtype=weights.dtype, device=dev) if rows is not None else None
         if T == 0:
             return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev), gw
         gr = _prep_out(out, T * k, D, dev)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_expert_combine_grad(
             grad_out.data_ptr(), rows.data_ptr() if rows is not None else None,
             int(rows is not None and rows.dtype == torch.float32), order.rows.data_ptr(),
             weights.data_ptr() if weighted else None, int(weights.dtype == DTYPE), gr.data_ptr(),
             gw.data_ptr() if gw is not None else None, T, k, D, T * k, _ld(grad_out),
-            _ld(rows) if rows is not None else D, _choice_ld(weights), _ld(gr),
-            _stream_handle(stream, dev)))
+            _ld(rows) if rows is not None else D, _choice_ld(weights), _ld(gr), handle))
     return gr, gw
 
 
@@ -326,23 +359,18 @@ def grouped_fused_swiglu(x, W, offsets, *, out=None, stream=None):
     R, K, N, E, dev = _swiglu_operands(x, W, offsets)
     if R == 0:
         return out if out is not None else torch.empty((0, N), dtype=DTYPE, device=dev)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         h = _prep_out(out, R, N, dev)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_grouped_fused_swiglu(
             x.data_ptr(), W.data_ptr(), offsets.data_ptr(), h.data_ptr(), R, N, K, E, _ld(x),
-            _expert_ld(W), W.stride(0), _ld(h), _stream_handle(stream, dev)))
+            _expert_ld(W), W.stride(0), _ld(h), handle))
     return h
 
 
 def _preact_shapes(bits: int, rows: int, N: int):
-    """Shapes of ``SavedPreact.data`` and ``.scales`` (None for 16 bits)."""
-    pitch, scale_pitch = C.c_int64(), C.c_int64()
-    n = _lib.load().sgl_preact_bytes(bits, rows, N, C.byref(pitch), None, C.byref(scale_pitch))
-    if n < 0:
-        _lib.check(int(n))
-    return ((rows, 2, pitch.value // (2 * bits // 8)),
-            (rows, 2, scale_pitch.value // 2) if bits == 8 else None)
+    """Shapes of ``SavedPreact.data`` and ``.scales`` (None for 16 bits): halves padded to whole
+    blocks of 32 columns, an even number of scales (``sgl_preact_bytes`` has the same in bytes)."""
+    return (rows, 2, (N + 31) // 32 * 32), (rows, 2, (N + 63) // 64 * 2) if bits == 8 else None
 
 
 def _empty_preact(bits: int, rows: int, N: int, dev) -> SavedPreact:
@@ -366,16 +394,15 @@ def _check_preact(p: SavedPreact) -> None:
 
 
 def _save(x, w_ptr, offsets, E, ldw, w_stride, R, K, N, bits, out, stream, dev):
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         h = _prep_out(out, R, N, dev) if R else torch.empty((0, N), dtype=DTYPE, device=dev)
         pre = _empty_preact(bits, R, N, dev)
-    if R:
-        with _on_device(dev):
+        if R:
             _lib.check(_lib.load().sgl_grouped_fused_swiglu_save(
                 x.data_ptr(), w_ptr, offsets.data_ptr() if offsets is not None else None,
                 h.data_ptr(), pre.data.data_ptr(),
                 pre.scales.data_ptr() if pre.scales is not None else None, bits, R, N, K, E, _ld(x),
-                ldw, w_stride, _ld(h), _stream_handle(stream, dev)))
+                ldw, w_stride, _ld(h), handle))
     return h, pre
 
 
@@ -430,19 +457,18 @@ def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h:
         _check_ints(offsets, "offsets", (offsets.numel(),))
         named.append(("offsets", offsets))
     dev = _same_device(*named)
-    with stream_context(stream, dev):
+    end = offsets.data_ptr() + 4 * (offsets.numel() - 1) if offsets is not None else None
+    with _launch(stream, dev) as handle:
         h = torch.empty((R, N), dtype=DTYPE, device=dev) if return_h else None
         if R == 0:
             g = out if out is not None else torch.empty((0, 2 * N), dtype=DTYPE, device=dev)
             return (g, h) if return_h else g
         g = _prep_out(out, R, 2 * N, dev)
-    end = offsets.data_ptr() + 4 * (offsets.numel() - 1) if offsets is not None else None
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_swiglu_grad_preact_saved(
             dy.data_ptr(), preact.data.data_ptr(),
             preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
             g.data_ptr(), h.data_ptr() if h is not None else None, end, R, N, _ld(dy), _ld(g),
-            _ld(h) if h is not None else 0, _stream_handle(stream, dev)))
+            _ld(h) if h is not None else 0, handle))
     return (g, h) if return_h else g
 
 
@@ -467,13 +493,12 @@ def grouped_matmul(a, B, offsets, *, out=None, stream=None, transpose_b: bool = 
     dev = _same_device(("a", a), ("B", B), ("offsets", offsets))
     if R == 0:
         return out if out is not None else torch.empty((0, N), dtype=out_dtype, device=dev)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         c = _prep_rows(out, R, N, dev, out_dtype)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_grouped_matmul(
             a.data_ptr(), B.data_ptr(), offsets.data_ptr(), c.data_ptr(), R, N, K, E, _ld(a),
             _expert_ld(B), B.stride(0), _ld(c), int(transpose_b), int(out_dtype == torch.float32),
-            _stream_handle(stream, dev)))
+            handle))
     return c
 
 
@@ -515,12 +540,11 @@ def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrd
         _check_weights(weights, T, k)
         named.append(("weights", weights))
     dev = _same_device(*named)
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         h = torch.empty((R, N), dtype=DTYPE, device=dev)
         if R == 0:
             return (out if out is not None else torch.empty((0, 2 * N), dtype=DTYPE, device=dev)), h
         g = _prep_out(out, R, 2 * N, dev)
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_grouped_grad_preact(
             grad_rows.data_ptr(), W_down.data_ptr(), order.offsets.data_ptr(),
             order.slots.data_ptr() if weights is not None else None,
@@ -529,7 +553,7 @@ def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrd
             preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
             g.data_ptr(), h.data_ptr(), R, N, D, E, k, _ld(grad_rows), _expert_ld(W_down),
             W_down.stride(0), _choice_ld(weights) if weights is not None else 0, _ld(g), _ld(h),
-            _stream_handle(stream, dev)))
+            handle))
     return g, h
 
 
@@ -549,7 +573,7 @@ def grouped_weight_grad(a, g, offsets, *, out=None, stream=None):
     E = offsets.numel() - 1
     _check_ints(offsets, "offsets", (E + 1,))
     dev = _same_device(("a", a), ("g", g), ("offsets", offsets))
-    with stream_context(stream, dev):
+    with _launch(stream, dev) as handle:
         if out is None:
             c = torch.empty((E, M, N), dtype=DTYPE, device=dev)
         else:
@@ -561,10 +585,9 @@ def grouped_weight_grad(a, g, offsets, *, out=None, stream=None):
                 raise ValueError(f"out is on {c.device}, expected {dev}")
         if R == 0:
             return c.zero_()
-    with _on_device(dev):
         _lib.check(_lib.load().sgl_grouped_weight_grad(
             a.data_ptr(), g.data_ptr(), offsets.data_ptr(), c.data_ptr(), R, M, N, E, _ld(a), _ld(g),
-            _expert_ld(c), c.stride(0), _stream_handle(stream, dev)))
+            _expert_ld(c), c.stride(0), handle))
     return c
 
 
@@ -617,18 +640,22 @@ def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=Non
     T, k, E, D, N, D_out, dev = _layer_operands(x, expert_ids, weights, W, W_down)
     if T == 0:
         return out if out is not None else torch.empty((0, D_out), dtype=DTYPE, device=dev)
-    need = experts_swiglu_workspace_bytes(T, k, E, D, N, D_out)
-    with stream_context(stream, dev):
+    lib = _lib.load()
+    need = lib.sgl_experts_swiglu_workspace_bytes(T, k, E, D, N, D_out)
+    if need < 0:
+        _lib.check(int(need))
+    with _launch(stream, dev) as handle:
         y = _prep_out(out, T, D_out, dev)
         if workspace is None:
             workspace = torch.empty(need, dtype=torch.uint8, device=dev)
-    if workspace.dtype != torch.uint8 or workspace.device != dev or not workspace.is_contiguous():
-        raise ValueError("workspace must be a contiguous uint8 CUDA tensor on the operands' device")
-    with _on_device(dev):
-        _lib.check(_lib.load().sgl_experts_swiglu(
-            x.data_ptr(), expert_ids.data_ptr(), int(expert_ids.dtype == torch.int64),
-            weights.data_ptr(), int(weights.dtype == DTYPE), W.data_ptr(), W_down.data_ptr(),
+        elif workspace.dtype != torch.uint8 or workspace.device != dev \
+                or not workspace.is_contiguous():
+            raise ValueError(
+                "workspace must be a contiguous uint8 CUDA tensor on the operands' device")
+        _lib.check(lib.sgl_experts_swiglu(
+            x.data_ptr(), expert_ids.data_ptr(), expert_ids.dtype == torch.int64,
+            weights.data_ptr(), weights.dtype == DTYPE, W.data_ptr(), W_down.data_ptr(),
             y.data_ptr(), workspace.data_ptr(), workspace.numel(), T, k, E, D, N, D_out, _ld(x),
             _choice_ld(expert_ids), _choice_ld(weights), _expert_ld(W), W.stride(0),
-            _expert_ld(W_down), W_down.stride(0), _ld(y), _stream_handle(stream, dev)))
+            _expert_ld(W_down), W_down.stride(0), _ld(y), handle))
     return y

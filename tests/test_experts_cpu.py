@@ -23,11 +23,22 @@ def call(fn, code, needle, *args):
     (dict(ids=0), -1, "ids is NULL"), (dict(ids=P + 4), -4, "8-byte"), (dict(T=0), -2, "T=0"),
     (dict(k=0), -2, "k=0"), (dict(k=65, ld=65), -2, "k=65"), (dict(E=0), -2, "E=0"),
     (dict(E=1025), -2, "E=1025"), (dict(T=2 ** 31), -2, "31 bits"), (dict(ld=1), -3, "ld_ids"),
+    (dict(T=1025, bytes=4096), -1, "scratch"),
+    (dict(T=1025, scratch=P, bytes=60), -10, "scratch"),
     (dict(offsets=0), -1, "offsets"), (dict(slots=P + 2), -4, "slots"), (dict(rows=0), -1, "rows")])
 def test_order_refusals(change, code, needle):
-    a = dict(ids=P, T=4, k=2, ld=2, E=8, offsets=P, slots=P, rows=P) | change
+    a = dict(ids=P, T=4, k=2, ld=2, E=8, offsets=P, slots=P, rows=P, scratch=0, bytes=0) | change
     call("sgl_expert_order", code, needle, a["ids"], 1, a["T"], a["k"], a["ld"], a["E"],
-         a["offsets"], a["slots"], a["rows"], None)
+         a["offsets"], a["slots"], a["rows"], a["scratch"], a["bytes"], None)
+
+
+def test_order_scratch():
+    size = _lib.load().sgl_expert_order_scratch_bytes
+    assert size(1024, 2, 1024) == 0 and experts._ONE_CTA_SLOTS == 2048
+    assert size(1025, 2, 8) == 2 * 8 * 4
+    assert size(2 ** 30, 1, 8) == 128 * 8 * 4          # never more than 128 CTAs
+    assert size(2 ** 20, 8, 1024) == 64 * 1024 * 4     # nor a table of more than 64 Ki counts
+    assert size(4, 2, 1025) == -2
 
 
 @pytest.mark.parametrize("change,code,needle", [
@@ -116,6 +127,11 @@ def test_workspace_holds_every_part():
 def test_preact_shapes(N, half, scale):
     assert experts._preact_shapes(8, 5, N) == ((5, 2, half), (5, 2, scale))
     assert experts._preact_shapes(16, 5, N) == ((5, 2, half), None)
+    pitch, scale_bytes, scale_pitch = C.c_int64(), C.c_int64(), C.c_int64()
+    size = _lib.load().sgl_preact_bytes
+    assert size(8, 5, N, C.byref(pitch), C.byref(scale_bytes), C.byref(scale_pitch)) == 10 * half
+    assert (pitch.value, scale_bytes.value, scale_pitch.value) == (2 * half, 10 * scale, 2 * scale)
+    assert size(16, 5, N, None, None, None) == 20 * half
 
 
 def test_python_refusals():

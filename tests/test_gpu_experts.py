@@ -42,7 +42,7 @@ def make_ids(T, k, E, seed, drop=0.1, dtype=torch.int64):
 @pytest.mark.parametrize("T,k,E,drop", [
     (1, 1, 1, 0.0), (1, 2, 8, 0.0), (1, 1, 4, 1.0), (7, 3, 5, 0.3), (33, 1, 1024, 0.0),
     (96, 8, 128, 0.0), (1000, 4, 3, 0.1), (2048, 2, 8, 0.0), (2049, 2, 8, 0.0), (4097, 3, 257, 0.2),
-    (20000, 2, 1000, 0.05), (5000, 64, 64, 0.0)])
+    (20000, 2, 1000, 0.05), (5000, 64, 64, 0.0), (100000, 6, 7, 0.3), (150000, 2, 1024, 0.0)])
 def test_order(T, k, E, drop, dtype):
     ids = make_ids(T, k, E, T + k, drop, dtype)
     got = sg.expert_order(ids, E)
