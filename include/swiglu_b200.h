@@ -606,7 +606,9 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
  *   y[t] = sum_j weights[t, j] * (silu(x[t] @ Wg) * (x[t] @ Wu)) @ Wd,  expert ids[t, j]
  * x[T, D], w[E, D, 2N], w_down[E, N, D_out], y[T, D_out].  `workspace`: caller-owned device memory
  * of sgl_experts_swiglu_workspace_bytes bytes, overwritten; calls that overlap on the GPU must not
- * share it.
+ * share it.  With few rows per expert the down projection's sum is cut into ranges (a function of
+ * the sizes alone) that are added in order: against the separate calls only the order of fp32
+ * additions differs then.
  */
 int64_t sgl_experts_swiglu_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N,
                                            int64_t D_out);

@@ -171,6 +171,8 @@ struct ExpertLaunch {
   const void* weights = nullptr;
   int64_t ld_w = 0, k = 1;
   int w_bf16 = 0;
+  int splits = 1;            // EXP_GEMM32: ranges of K, each with its own slot of the result
+  int64_t k_per_split = 0;
 };
 
 // Byte layout of saved pre-activations: rows of [up | gate], each half padded to whole blocks.
@@ -213,14 +215,14 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   const int64_t groups_used = wgrad ? s.E : (s.E < s.R ? s.E : s.R);
   const int64_t max_tiles_m = wgrad ? (s.M + tile_rows - 1) / tile_rows * s.E
                                     : s.R / tile_rows + groups_used;
+  // Single-CTA tiles: half as wide while there are fewer than two for each SM.  (64 columns are
+  // not worth it: a k-block takes 0.5 us at 64 and at 128 columns.  8 tokens x 2 of 8 experts,
+  // 14336 -> 4096: 255 us at 64 columns, 142 at 128.)
   int acc_cols = sgl::kAccCols;
-  const int min_cols = swiglu ? 128 : 64;
+  const int min_cols = 128;
   if (cta_group == 1 && !wgrad) {
-    while (acc_cols > min_cols) {
-      const int64_t cols = swiglu ? acc_cols / 2 : acc_cols;
-      if (max_tiles_m * ((s.N + cols - 1) / cols) >= 2 * info->sm_count) break;
-      acc_cols /= 2;
-    }
+    const int64_t cols = swiglu ? acc_cols / 2 : acc_cols;
+    if (max_tiles_m * ((s.N + cols - 1) / cols) * s.splits < 2 * info->sm_count) acc_cols = min_cols;
   }
   int a_rows = sgl::kBlockM;
   if (cta_group == 1 && !wgrad && s.R <= 32) a_rows = static_cast<int>((s.R + 15) / 16 * 16);
@@ -231,7 +233,8 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   }
   const int tile_cols = swiglu ? acc_cols / 2 : acc_cols;
   const int64_t tiles_n = (s.N + tile_cols - 1) / tile_cols;
-  if (max_tiles_m * tiles_n > 0x7fffffffll) return fail(SGL_ERR_BAD_SHAPE, "too many tiles");
+  const int64_t units = max_tiles_m * tiles_n * s.splits;
+  if (units > 0x7fffffffll) return fail(SGL_ERR_BAD_SHAPE, "too many tiles");
   const int smem = v.smem_bytes(static_cast<int>(s.E), a_rows, acc_cols, stages);
 
   sgl::ExpertMaps maps;
@@ -262,7 +265,9 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
     // three results (or the 8-bit halves) share the staging
     const bool triple = s.form == sgl::EXP_SAVE16 || grad;
     const bool f32 = s.form == sgl::EXP_GEMM32;
-    rc = make_expert_map(&maps.out, s.out, s.N, s.R, 0, s.ld_out * (f32 ? 4 : 2), 0,
+    const int64_t slot_bytes = f32 ? s.R * s.ld_out * 4 : 0;
+    rc = make_expert_map(&maps.out, s.out, s.N, s.R, f32 ? s.splits : 0, s.ld_out * (f32 ? 4 : 2),
+                         slot_bytes,
                          triple || f32 ? 32 : 64, 32, "out",
                          f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kBf16, triple ? kSw64 : kSw128,
                          kNoPromo);
@@ -291,6 +296,9 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.group_m = 16;
   p.stages = stages;
   p.acc_cols = acc_cols;
+  p.splits = s.splits;
+  p.k_per_split = static_cast<int>(s.k_per_split);
+  p.slot_stride = s.R * s.ld_out;
   p.a_rows = a_rows;
   p.b_kmajor = s.b_transposed;
   p.out = static_cast<__nv_bfloat16*>(s.out);
@@ -314,8 +322,7 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.l2_hints = 2 | (2 << 2) | (1 << 4);
   p.wait_limit_ns = g_wait_limit_ns.load();
 
-  int64_t grid = clusters;
-  if (max_tiles_m * tiles_n < grid) grid = max_tiles_m * tiles_n;
+  const int64_t grid = units < clusters ? units : clusters;
   cudaLaunchConfig_t lc = {};
   lc.gridDim = dim3(static_cast<unsigned>(grid * cta_group), 1, 1);
   lc.blockDim = dim3(sgl::kExpThreads, 1, 1);
@@ -333,10 +340,10 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   if (log_enabled())
     fprintf(stderr,
             "[libswiglu_b200] launch sgl %s R=%lld N=%lld K=%lld M=%lld E=%lld cta_group=%d "
-            "acc_cols=%d a_rows=%d stages=%d grid=%lld smem=%d\n",
+            "acc_cols=%d splits=%d a_rows=%d stages=%d grid=%lld smem=%d\n",
             s.name, static_cast<long long>(s.R), static_cast<long long>(s.N),
             static_cast<long long>(s.K), static_cast<long long>(s.M), static_cast<long long>(s.E),
-            cta_group, acc_cols, a_rows, stages, static_cast<long long>(grid * cta_group), smem);
+            cta_group, acc_cols, s.splits, a_rows, stages, static_cast<long long>(grid * cta_group), smem);
   if (nvtx_enabled()) nvtxRangePushA(s.name);
   cudaError_t e = cudaLaunchKernelEx(&lc, v.fn, maps, p);
   if (nvtx_enabled()) nvtxRangePop();
@@ -398,13 +405,20 @@ int validate_row_call(int64_t T, int64_t k, int64_t D, int64_t R) {
 
 // Threads of a token (a power of two of warps, at most 256) and CTAs for `T` tokens, at most
 // `per_sm` per SM (16384 x 4096: dispatch 61 us without a limit and 68 us with 8; combine 73 and
-// 64 us).
-void row_geometry(int64_t T, int nvec, int64_t per_sm, const DeviceInfo* info, dim3* grid,
-                  dim3* block) {
+// 64 us).  With few tokens, and where the kernel allows it (split), small CTAs share a token.
+void row_geometry(int64_t T, int nvec, int64_t per_sm, bool split, const DeviceInfo* info,
+                  dim3* grid, dim3* block) {
   unsigned tx = 32;
   while (tx < 256 && tx < static_cast<unsigned>(nvec)) tx *= 2;
+  if (split && T * ((nvec + 255) / 256) < info->sm_count) {
+    tx = tx < 64 ? tx : 64;
+    *block = dim3(tx, 1, 1);
+    const unsigned per_token = (static_cast<unsigned>(nvec) + tx - 1) / tx;
+    *grid = dim3(static_cast<unsigned>(T), per_token < 64 ? per_token : 64, 1);
+    return;
+  }
   *block = dim3(tx, 256 / tx, 1);
-  int64_t ctas = (T + block->y - 1) / block->y;
+  const int64_t ctas = (T + block->y - 1) / block->y;
   const int64_t cap = static_cast<int64_t>(info->sm_count) * per_sm;
   *grid = dim3(static_cast<unsigned>(ctas < cap ? ctas : cap), 1, 1);
 }
@@ -526,13 +540,15 @@ int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, i
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, 4096, info, &grid, &block);
+  row_geometry(T, p.nvec, 4096, true, info, &grid, &block);
   return launch_after("expert_dispatch", sgl::expert_dispatch_kernel, grid, block, 0, stream, p);
 }
 
-int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
-                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
-                       int64_t ld_w, int64_t ldo, void* stream) {
+// `splits`: partial sums of every fp32 row, R rows apart (sgl_experts_swiglu).
+static int combine_rows(const void* in, int in_is_f32, int splits, const void* rows,
+                        const void* weights, int weights_bf16, void* out, int64_t T, int64_t k,
+                        int64_t D, int64_t R, int64_t ld_in, int64_t ld_w, int64_t ldo,
+                        void* stream) {
   int rc;
   if ((rc = validate_row_call(T, k, D, R))) return rc;
   if ((rc = validate_ptr(in, "in")) || (rc = validate_words(rows, "rows", 4)) ||
@@ -552,6 +568,8 @@ int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const vo
   p.in = in;
   p.out = static_cast<__nv_bfloat16*>(out);
   p.rows = static_cast<const int*>(rows);
+  p.splits = splits;
+  p.slot_stride = R * ld_in;
   p.weights = weights;
   p.w_bf16 = weights_bf16 != 0;
   p.ld_in = ld_in;
@@ -562,13 +580,22 @@ int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const vo
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, 8, info, &grid, &block);
+  row_geometry(T, p.nvec, 8, true, info, &grid, &block);
+  if (splits > 1)
+    return launch_after("expert_combine", sgl::expert_combine_parts_kernel, grid, block, 0, stream, p);
   return launch_after("expert_combine",
                       k <= 2 ? (in_is_f32 ? sgl::expert_combine_kernel<true, 2, 2>
                                           : sgl::expert_combine_kernel<false, 2, 2>)
                              : (in_is_f32 ? sgl::expert_combine_kernel<true, 1, 4>
                                           : sgl::expert_combine_kernel<false, 1, 4>),
                       grid, block, 0, stream, p);
+}
+
+int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
+                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R,
+                       int64_t ld_in, int64_t ld_w, int64_t ldo, void* stream) {
+  return combine_rows(in, in_is_f32, 1, rows, weights, weights_bf16, out, T, k, D, R, ld_in, ld_w,
+                      ldo, stream);
 }
 
 int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32, const void* rows,
@@ -612,7 +639,7 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32,
   p.nvec = static_cast<int>(D / 8);
   p.R = R;
   dim3 grid, block;
-  row_geometry(T, p.nvec, 8, info, &grid, &block);
+  row_geometry(T, p.nvec, 8, false, info, &grid, &block);
   return launch_after("expert_combine_grad",
                       k <= 2 ? (in_is_f32 ? sgl::expert_combine_grad_kernel<true, 2, 2>
                                           : sgl::expert_combine_grad_kernel<false, 2, 2>)
@@ -689,9 +716,10 @@ int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offs
                         E, ldx, ldw, w_stride, ldh, stream);
 }
 
-int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
-                       int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
-                       int64_t ldc, int b_transposed, int c_is_f32, void* stream) {
+static int grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
+                          int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb,
+                          int64_t b_stride, int64_t ldc, int b_transposed, int c_is_f32, int splits,
+                          int64_t k_per_split, void* stream) {
   int rc;
   if ((rc = validate_groups(R, E, offsets, true))) return rc;
   if ((rc = validate_ptr(a, "a")) || (rc = validate_ptr(b, "b")) || (rc = validate_ptr(c, "c")))
@@ -718,7 +746,16 @@ int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* 
   s.b_stride = E > 1 ? b_stride : b_rows * ldb;
   s.ld_out = ldc;
   s.b_transposed = b_transposed != 0;
+  s.splits = splits;
+  s.k_per_split = k_per_split;
   return launch_experts(s, stream);
+}
+
+int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
+                       int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
+                       int64_t ldc, int b_transposed, int c_is_f32, void* stream) {
+  return grouped_matmul(a, b, offsets, c, R, N, K, E, lda, ldb, b_stride, ldc, b_transposed,
+                        c_is_f32, 1, 0, stream);
 }
 
 int sgl_grouped_grad_preact(const void* dy, const void* w_down, const void* offsets,
@@ -857,7 +894,31 @@ static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }
 
 struct ExpertsWorkspace {
   int64_t offsets, slots, rows, scratch, scratch_bytes, xs, h, ys, total;
+  int splits;              // ranges of the down projection's sum
+  int64_t k_per_split;
 };
+
+// Few rows make few tiles, and the down projection (long sums, narrow results) then leaves SMs
+// idle while others stream long columns of weight.  Its sum is cut into ranges of at least 512
+// whose partial rows the combine step adds up in order: as many as give every SM about four
+// tiles if all groups are used, while the partial rows written and read stay below an eighth of
+// the weight.  A function of the sizes alone.  1 token x 2 of 8 experts, 14336 -> 4096: XXX us
+// in one range, XXX us in XXX.
+static void down_ranges(int64_t R, int64_t E, int64_t N, int64_t D_out, int* splits,
+                        int64_t* per_split) {
+  *splits = 1;
+  *per_split = 0;
+  const int64_t groups = E < R ? E : R;
+  if (R / E >= 64) return;
+  const int64_t tiles = (groups + R / sgl::kBlockM) * ((D_out + 127) / 128);
+  int64_t s = (4 * 148 + tiles - 1) / tiles;
+  if (s > N / 512) s = N / 512;
+  if (s > groups * N / (32 * R)) s = groups * N / (32 * R);
+  if (s > 16) s = 16;
+  if (s < 2) return;
+  *per_split = (((N + s - 1) / s) + 127) / 128 * 128;
+  *splits = static_cast<int>((N + *per_split - 1) / *per_split);
+}
 
 static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
                              ExpertsWorkspace* w) {
@@ -881,7 +942,8 @@ static int experts_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t
   w->h = at;
   at += align256(R * N * 2);
   w->ys = at;
-  at += align256(R * D_out * 4);
+  down_ranges(R, E, N, D_out, &w->splits, &w->k_per_split);
+  at += align256(R * D_out * 4 * w->splits);
   w->total = at;
   return SGL_OK;
 }
@@ -927,10 +989,10 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
       (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream)) ||
       (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
                                      w_stride, N, stream)) ||
-      (rc = sgl_grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
-                               d_stride, D_out, 0, 1, stream)))
+      (rc = grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
+                           d_stride, D_out, 0, 1, l.splits, l.k_per_split, stream)))
     return rc;
-  return sgl_expert_combine(ws + l.ys, 1, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
+  return combine_rows(ws + l.ys, 1, l.splits, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
                             ld_weights, ldy, stream);
 }
 

@@ -263,8 +263,9 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_place_kernel(const Or
 
 // ---------------------------------------------------------------- rows out and back
 //
-// All three kernels give `tx` threads (a multiple of 32) to a token, 256 / tx tokens to a CTA,
-// and let each thread move 16 bytes (8 columns) of the row at a time.  HBM bound.
+// The kernels give a multiple of 32 threads to a token, 256 threads of several tokens to a CTA, and
+// with few tokens several CTAs (gridDim.y) to one; a thread moves 8 columns of a row at a time.
+// HBM bound.
 
 struct RowParams {
   const void* in;              // x [T, D] | rows [R, D] | grad_out [T, D]; bf16, rows also fp32
@@ -277,6 +278,8 @@ struct RowParams {
   int64_t T;
   int k, nvec;                 // nvec = D / 8
   int w_bf16;
+  int splits;                  // combine_parts: a row is the sum of `splits` partial rows,
+  int64_t slot_stride;         // slot_stride elements apart
   int64_t R;                   // rows the row tensors have: an index outside is not followed
 };
 
@@ -351,10 +354,11 @@ __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p)
   constexpr int kVecs = 2;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tx = blockDim.x;
+  const int tx = blockDim.x * gridDim.y;     // threads of a token
+  const int first = blockIdx.y * blockDim.x + threadIdx.x;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
        t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    for (int v0 = threadIdx.x; v0 < p.nvec; v0 += kVecs * tx) {
+    for (int v0 = first; v0 < p.nvec; v0 += kVecs * tx) {
       Vec8<false> val[kVecs];
 #pragma unroll
       for (int i = 0; i < kVecs; ++i)
@@ -377,10 +381,11 @@ template <bool kF32, int kVecs, int kBatch>
 __global__ void __launch_bounds__(256, kF32 ? 3 : 4) expert_combine_kernel(const RowParams p) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int tx = blockDim.x;
+  const int tx = blockDim.x * gridDim.y;     // threads of a token
+  const int first = blockIdx.y * blockDim.x + threadIdx.x;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
        t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
-    for (int v0 = threadIdx.x; v0 < p.nvec; v0 += kVecs * tx) {
+    for (int v0 = first; v0 < p.nvec; v0 += kVecs * tx) {
       float acc[kVecs][8] = {};
       for (int j0 = 0; j0 < p.k; j0 += kBatch) {
         Vec8<kF32> val[kBatch][kVecs];
@@ -412,6 +417,46 @@ __global__ void __launch_bounds__(256, kF32 ? 3 : 4) expert_combine_kernel(const
       for (int i = 0; i < kVecs; ++i)
         if (v0 + i * tx < p.nvec)
           reinterpret_cast<uint4*>(p.out + t * p.ld_out)[v0 + i * tx] = f32_to_bf16x8(acc[i]);
+    }
+  }
+}
+
+// The same for rows that are sums of p.splits fp32 partial rows, added in order.  Few tokens, so
+// latency bound: a thread has up to eight partial rows in flight.
+__global__ void __launch_bounds__(256, 2) expert_combine_parts_kernel(const RowParams p) {
+  constexpr int kParts = 8;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int tx = blockDim.x * gridDim.y;     // threads of a token
+  const int first = blockIdx.y * blockDim.x + threadIdx.x;
+  for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;
+       t += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+    for (int v = first; v < p.nvec; v += tx) {
+      float acc[8] = {};
+      for (int j = 0; j < p.k; ++j) {
+        const int r = row_of(p, t, j);
+        if (r < 0) continue;
+        const float w = load_weight(p, t, j);
+        float sum[8] = {};
+        for (int s0 = 0; s0 < p.splits; s0 += kParts) {
+          Vec8<true> part[kParts];
+#pragma unroll
+          for (int i = 0; i < kParts; ++i)
+            if (s0 + i < p.splits)
+              part[i].load(static_cast<const float*>(p.in) + (s0 + i) * p.slot_stride, r, p.ld_in, v);
+#pragma unroll
+          for (int i = 0; i < kParts; ++i) {
+            if (s0 + i >= p.splits) continue;
+            float f[8];
+            part[i].get(f);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) sum[c] += f[c];
+          }
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) acc[c] = fmaf(w, sum[c], acc[c]);
+      }
+      reinterpret_cast<uint4*>(p.out + t * p.ld_out)[v] = f32_to_bf16x8(acc);
     }
   }
 }

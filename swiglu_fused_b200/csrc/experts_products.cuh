@@ -15,8 +15,8 @@
 // With offsets == NULL there is one group of all rows (the dense stage's 8-bit checkpoints).
 //
 // Structure as the dense kernel's (swiglu_kernel.cuh): persistent CTAs (or CTA pairs on 256-row
-// tiles, tcgen05 cta_group::2), warp 0 = TMA producer, warp 1 = MMA issuer, warps 2-5 = epilogue,
-// a 256-column fp32 accumulator in two TMEM stages.  What the groups change:
+// tiles, tcgen05 cta_group::2), warps 0 and 6 = TMA producers (A, B), warp 1 = MMA issuer, warps
+// 2-5 = epilogue, a 256-column fp32 accumulator in two TMEM stages.  What the groups change:
 //   * every CTA turns the offsets into a table of first tile rows once, and finds the expert
 //     of a tile by bisection in it;
 //   * an A tile whose rows run past its group takes them along in the operand (their
@@ -26,13 +26,15 @@
 //     14336 -> 4096: 1.76 ms with boxes of 16 throughout, 1.38 ms so);
 //   * the epilogue stores 32 whole rows with TMA; a warp whose rows end inside its 32 copies
 //     the rows that exist with plain stores, so that no row of another group is touched;
-//   * EXP_WGRAD sums over rows, so rows past the group must not reach the MMA: warp 6 waits
-//     for such a block of operands to land, overwrites them with zeros (TMA cannot clip at a
-//     border inside the tensor) and only then hands the block to the MMA issuer.
+//   * EXP_WGRAD sums over rows, so rows past the group must not reach the MMA: whole steps of 16
+//     are not issued, and where the group ends inside a step warp 7 waits for the operands to
+//     land, overwrites the rest of the step with zeros (TMA cannot clip at a border inside the
+//     tensor) and only then hands the block to the MMA issuer.
 // Every wait is bounded, as everywhere in this library.
 #pragma once
 
 #include <cstdint>
+#include <type_traits>
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -48,7 +50,7 @@ enum : int {
   EXP_GRAD8 = 6, EXP_WGRAD = 7, EXP_FORMS = 8
 };
 
-constexpr int kExpThreads = 224;       // producer, MMA issuer, 4 epilogue warps, tail warp
+constexpr int kExpThreads = 256;       // two producers, MMA issuer, 4 epilogue warps, tail warp
 constexpr int kExpMaxStages = 16;
 constexpr int kExpBarrierBytes = 8 * (3 * kExpMaxStages + 2 * kAccStages) + 32;
 constexpr int kExpMaxGroups = 1024;
@@ -79,11 +81,13 @@ struct ExpertParams {
   int tiles_n;
   int group_m;          // tile rows walked together inside a group
   int stages;
-  int acc_cols;         // accumulator columns of a tile (256; single-CTA tiles also 128, 64)
+  int acc_cols;         // accumulator columns of a tile (256; single-CTA tiles also 128)
+  int splits;           // EXP_GEMM32: K is cut into ranges of k_per_split (a multiple of BLOCK_K),
+  int k_per_split;      // range s of a row's sum goes to slot s of the result
   int a_rows;           // rows of an A slot: 128, or a multiple of 16 below it when R is small
   int b_kmajor;         // B[e] is stored [n, k] (multiplied transposed)
   __nv_bfloat16* out;   // forward forms: raw pointers for rows that end inside a warp's 32
-  int64_t ld_out;
+  int64_t ld_out, slot_stride;   // elements
   uint8_t* pre;         // pre-activations or their gradients (written), gate half at + gate_off
   int64_t ld_pre;       // row pitch, bytes
   int64_t gate_off;     // bytes from the up half to the gate half of a row
@@ -199,6 +203,37 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const CUtensorMap
         "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes"
         ".L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %6;" ::"r"(smem_dst),
         "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar), "l"(policy)
+        : "memory");
+  }
+}
+
+// ptx::umma_bf16 with the two descriptors as (low word, common high word).
+template <int kCtaGroup>
+__device__ __forceinline__ void umma_bf16_lohi(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo,
+                                               uint32_t hi, uint32_t idesc, uint32_t accumulate) {
+  if constexpr (kCtaGroup == 2) {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], da, db, %4, p;\n\t"
+        "}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
+        : "memory");
+  } else {
+    asm volatile(
+        "{\n\t"
+        ".reg .pred p;\n\t"
+        ".reg .b64 da, db;\n\t"
+        "mov.b64 da, {%1, %3};\n\t"
+        "mov.b64 db, {%2, %3};\n\t"
+        "setp.ne.b32 p, %5, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t"
+        "}" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate)
         : "memory");
   }
 }
@@ -350,9 +385,9 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     abort_flag[0] = 0;
     abort_flag[1] = 0;
     for (int s = 0; s < stages; ++s) {
-      ptx::mbar_init(bar_full + 8 * s, kCtaGroup);
+      ptx::mbar_init(bar_full + 8 * s, 2 * kCtaGroup);   // one arrive.expect_tx per producer
       ptx::mbar_init(bar_empty + 8 * s, 1);
-      ptx::mbar_init(bar_land + 8 * s, 1);
+      ptx::mbar_init(bar_land + 8 * s, 2);
     }
     for (int s = 0; s < kAccStages; ++s) {
       ptx::mbar_init(bar_tfull + 8 * s, 1);
@@ -410,17 +445,20 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   const uint32_t tmem_base = *tmem_slot_ptr;
 
   const int wgrad_tiles_m = kWgrad ? (p.M + kTileRows - 1) / kTileRows : 0;
-  const int total_units = (kWgrad ? wgrad_tiles_m * G : tile_lo[G]) * p.tiles_n;
+  const int splits = kForm == EXP_GEMM32 ? p.splits : 1;
+  const int total_units = (kWgrad ? wgrad_tiles_m * G : tile_lo[G]) * p.tiles_n * splits;
 
   struct Unit {
     int e;          // group
     int row;        // forward: first row of the tile; EXP_WGRAD: first row of the group
     int rows;       // forward: rows from there to the group's end; EXP_WGRAD: rows of the group
     int m, n;       // EXP_WGRAD: first row of C[e]; first column of the result
+    int k0;         // EXP_GEMM32: first of the range of the sum
   };
   auto unit_of = [&](int u) {
     Unit r;
-    const int tm = u / p.tiles_n;
+    const int tm = u / (p.tiles_n * splits);
+    r.k0 = 0;
     if constexpr (kWgrad) {
       r.e = tm / wgrad_tiles_m;
       const TileCoord tc = tile_coord(u - r.e * wgrad_tiles_m * p.tiles_n, wgrad_tiles_m,
@@ -437,8 +475,16 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         if (tile_lo[mid] <= tm) lo = mid; else hi = mid;
       }
       r.e = lo;
-      const TileCoord tc = tile_coord(u - tile_lo[lo] * p.tiles_n, tile_lo[lo + 1] - tile_lo[lo],
-                                      p.tiles_n, p.group_m);
+      const int tiles_m = tile_lo[lo + 1] - tile_lo[lo];
+      int t = u - tile_lo[lo] * p.tiles_n * splits;
+      if (splits > 1) {
+        // all tiles of a group for one range of the sum, then the next range: neighbouring CTAs
+        // read neighbouring columns
+        const int range = t / (tiles_m * p.tiles_n);
+        t -= range * tiles_m * p.tiles_n;
+        r.k0 = range * p.k_per_split;
+      }
+      const TileCoord tc = tile_coord(t, tiles_m, p.tiles_n, p.group_m);
       r.row = row_lo(lo) + tc.m * kTileRows;
       r.rows = row_lo(lo + 1) - r.row;
       r.m = 0;
@@ -446,140 +492,146 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     }
     return r;
   };
-  // k-blocks of a unit
-  auto unit_kb = [&](const Unit& un) {
-    return ((kWgrad ? un.rows : p.K) + kBlockK - 1) / kBlockK;
+  // extent of a unit's sum, and its k-blocks
+  auto unit_len = [&](const Unit& un) {
+    if constexpr (kWgrad) return un.rows;
+    if (splits > 1) return p.K - un.k0 < p.k_per_split ? p.K - un.k0 : p.k_per_split;
+    return p.K;
+  };
+  auto unit_kb = [&](const Unit& un) { return (unit_len(un) + kBlockK - 1) / kBlockK; };
+  // EXP_WGRAD: whether block kb holds rows behind the group inside a step of 16 that is used
+  auto mixed_block = [&](const Unit& un, int kb) {
+    return kWgrad && un.rows - kb * kBlockK < kBlockK && (un.rows & 15) != 0;
   };
 
   const uint64_t limit = p.wait_limit_ns;
 
-  if (warp == 0) {
-    // =========================== TMA producer ===========================
-    if (lane == 0) {
-      const uint64_t pol_a = ptx::make_l2_policy(p.l2_hints & 3);
-      const uint64_t pol_b = ptx::make_l2_policy((p.l2_hints >> 2) & 3);
-      int s = 0;
-      uint32_t ph = 0;
-      bool ok = true;
-      Unit next;
-      if (cluster_id < total_units) next = unit_of(cluster_id);
-      for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
-        const Unit un = next;
-        const int num_kb = unit_kb(un);
-        if (num_kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
-        // forward: rows of this CTA's half of the tile, and the boxes that cover them
-        int left = un.rows - static_cast<int>(rank) * kBlockM;
-        left = left < 0 ? 0 : (left > kBlockM ? kBlockM : left);
-        const int my_row = un.row + static_cast<int>(rank) * kBlockM;
-        const bool whole = left > 32 && p.a_rows == kBlockM;
-        const int boxes16 = (left + 15) / 16;
-        const uint32_t b_bytes = static_cast<uint32_t>(b_slabs * T::kBSlabBytes);
-        const uint32_t stage_tx =
-            b_bytes + static_cast<uint32_t>((kWgrad || whole ? kBlockM : boxes16 * 16) * kBlockK * 2);
-        for (int kb = 0; kb < num_kb; ++kb) {
-          if (!ptx::mbar_wait(bar_empty + 8 * s, ph ^ 1u, limit, abort_flag)) {
-            report_error(kErrExpProducerWait, kb, abort_flag);
-            ok = false;
-            break;
+  // =========================== TMA producers ===========================
+  // One thread each for the A and the B operand: a copy takes its thread about 230 cycles to
+  // issue, and a k-block of 128 has four to six of them, more than the tensor core needs.
+  auto produce = [&](auto operand) {
+    constexpr bool kA = decltype(operand)::value == 0;
+    const uint64_t policy = ptx::make_l2_policy((p.l2_hints >> (kA ? 0 : 2)) & 3);
+    int s = 0;
+    uint32_t ph = 0;
+    bool ok = true;
+    Unit next;
+    if (cluster_id < total_units) next = unit_of(cluster_id);
+    for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
+      const Unit un = next;
+      const int num_kb = unit_kb(un);
+      if (num_kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
+      // forward: rows of this CTA's half of the tile, and the boxes that cover them
+      int left = un.rows - static_cast<int>(rank) * kBlockM;
+      left = left < 0 ? 0 : (left > kBlockM ? kBlockM : left);
+      [[maybe_unused]] const int my_row = un.row + static_cast<int>(rank) * kBlockM;
+      const bool whole = left > 32 && p.a_rows == kBlockM;
+      const int boxes16 = (left + 15) / 16;
+      const uint32_t tx = static_cast<uint32_t>(
+          kA ? (kWgrad || whole ? kBlockM : boxes16 * 16) * kBlockK * 2 : b_slabs * T::kBSlabBytes);
+      for (int kb = 0; kb < num_kb; ++kb) {
+        if (!ptx::mbar_wait(bar_empty + 8 * s, ph ^ 1u, limit, abort_flag)) {
+          report_error(kErrExpProducerWait, kb, abort_flag);
+          ok = false;
+          break;
+        }
+        const int k0 = un.k0 + kb * kBlockK;
+        const uint32_t full_local = bar_full + 8 * s;
+        uint32_t bar = (kCtaGroup == 2) ? ptx::mapa(full_local, 0) : full_local;
+        bool peer = kCtaGroup == 2;
+        if (SGL_DBG_COORD_BAD(un.row >= 0 && un.row < p.R && un.e >= 0 && un.e < G &&
+                                  (un.n & 7) == 0 && un.n < p.N && un.m >= 0,
+                              kb)) {
+          *reinterpret_cast<volatile int*>(abort_flag) = 1;
+          ok = false;
+          break;
+        }
+        if constexpr (kWgrad) {
+          // a block that the group ends in reports to this CTA's own barrier: the tail warp
+          // clears the rows behind the group and passes the block on
+          if (mixed_block(un, kb)) {
+            bar = bar_land + 8 * s;
+            peer = false;
           }
-          const int k0 = kb * kBlockK;
-          const uint32_t full_local = bar_full + 8 * s;
-          uint32_t bar = (kCtaGroup == 2) ? ptx::mapa(full_local, 0) : full_local;
-          bool peer = kCtaGroup == 2;
-          if (SGL_DBG_COORD_BAD(un.row >= 0 && un.row < p.R && un.e >= 0 && un.e < G &&
-                                    (un.n & 7) == 0 && un.n < p.N && un.m >= 0,
-                                kb)) {
-            *reinterpret_cast<volatile int*>(abort_flag) = 1;
-            ok = false;
-            break;
-          }
-          if constexpr (kWgrad) {
-            // a block that the group ends in reports to this CTA's own barrier: the tail warp
-            // clears the rows behind the group and passes the block on
-            if (un.rows - k0 < kBlockK) {
-              bar = bar_land + 8 * s;
-              peer = false;
+        }
+        ptx::mbar_arrive_expect_tx_cluster(bar, tx);
+        if constexpr (kWgrad) {
+          constexpr int kSlabs = kA ? kBlockM / 64 : T::kBSlabsMax;
+          const CUtensorMap* map = kA ? &maps.a : &maps.b;
+          const uint32_t dst = kA ? sA + s * a_stage : sB + s * b_stage;
+          const int x0 = kA ? un.m + static_cast<int>(rank) * kBlockM
+                            : un.n + static_cast<int>(rank) * b_slabs * 64;
+#pragma unroll
+          for (int j = 0; j < kSlabs; ++j) {
+            if (!kA && j >= b_slabs) break;
+            if (peer) {
+              ptx::tma_load_2d<true>(dst + j * (kBlockK * 128), map, x0 + j * 64, un.row + k0, bar,
+                                     policy);
+            } else {
+              ptx::tma_load_2d<false>(dst + j * (kBlockK * 128), map, x0 + j * 64, un.row + k0, bar,
+                                      policy);
             }
           }
-          ptx::mbar_arrive_expect_tx_cluster(bar, stage_tx);
+        } else if constexpr (kA) {
           const uint32_t a_dst = sA + s * a_stage;
-          const uint32_t b_dst = sB + s * b_stage;
-          if constexpr (kWgrad) {
 #pragma unroll
-            for (int j = 0; j < kBlockM / 64; ++j) {
-              const int x = un.m + static_cast<int>(rank) * kBlockM + j * 64;
-              if (peer) {
-                ptx::tma_load_2d<true>(a_dst + j * (kBlockK * 128), &maps.a, x, un.row + k0, bar,
-                                       pol_a);
-              } else {
-                ptx::tma_load_2d<false>(a_dst + j * (kBlockK * 128), &maps.a, x, un.row + k0, bar,
-                                        pol_a);
-              }
+          for (int j = 0; j < kBlockK / 64; ++j) {
+            const uint32_t dst = a_dst + j * (p.a_rows * 128);
+            if (whole) {
+              ptx::tma_load_2d<kCtaGroup == 2>(dst, &maps.a, k0 + j * 64, my_row, bar, policy);
+            } else {
+              for (int i = 0; i < boxes16; ++i)
+                ptx::tma_load_2d<kCtaGroup == 2>(dst + i * (16 * 128), &maps.a16, k0 + j * 64,
+                                                 my_row + i * 16, bar, policy);
             }
+          }
+        } else {
+          const uint32_t b_dst = sB + s * b_stage;
+          if (p.b_kmajor) {
+            // B[e] stored [n, k]: boxes of 64 n-rows x 64 k, one 64-k slice of all this CTA's
+            // rows contiguous
 #pragma unroll
-            for (int j = 0; j < T::kBSlabsMax; ++j) {
-              if (j >= b_slabs) break;
-              const int x = un.n + (static_cast<int>(rank) * b_slabs + j) * 64;
-              if (peer) {
-                ptx::tma_load_2d<true>(b_dst + j * T::kBSlabBytes, &maps.b, x, un.row + k0, bar,
-                                       pol_b);
-              } else {
-                ptx::tma_load_2d<false>(b_dst + j * T::kBSlabBytes, &maps.b, x, un.row + k0, bar,
-                                        pol_b);
+            for (int j = 0; j < kBlockK / 64; ++j) {
+              for (int i = 0; i < b_slabs; ++i) {
+                const int row = un.n + (static_cast<int>(rank) * b_slabs + i) * 64;
+                tma_load_3d(b_dst + j * (b_slabs * 64 * 128) + i * (64 * 128), &maps.b, k0 + j * 64,
+                            row, un.e, bar, policy, peer);
               }
             }
           } else {
 #pragma unroll
-            for (int j = 0; j < kBlockK / 64; ++j) {
-              const uint32_t dst = a_dst + j * (p.a_rows * 128);
-              if (whole) {
-                ptx::tma_load_2d<kCtaGroup == 2>(dst, &maps.a, k0 + j * 64, my_row, bar, pol_a);
-              } else {
-                for (int i = 0; i < boxes16; ++i)
-                  ptx::tma_load_2d<kCtaGroup == 2>(dst + i * (16 * 128), &maps.a16, k0 + j * 64,
-                                                   my_row + i * 16, bar, pol_a);
+            for (int j = 0; j < T::kBSlabsMax; ++j) {
+              if (j >= b_slabs) break;
+              const int g = static_cast<int>(rank) * b_slabs + j;   // slab of the tile
+              int col = un.n + g * 64;
+              if constexpr (kSwiglu) {
+                // the first half of the accumulator is up, the second gate
+                const int half = p.acc_cols / 128;
+                col = g < half ? un.n + g * 64 : p.N + un.n + (g - half) * 64;
               }
-            }
-            if (p.b_kmajor) {
-              // B[e] stored [n, k]: boxes of 64 n-rows x 64 k, one 64-k slice of all this CTA's
-              // rows contiguous
-#pragma unroll
-              for (int j = 0; j < kBlockK / 64; ++j) {
-                for (int i = 0; i < b_slabs; ++i) {
-                  const int row = un.n + (static_cast<int>(rank) * b_slabs + i) * 64;
-                  tma_load_3d(b_dst + j * (b_slabs * 64 * 128) + i * (64 * 128), &maps.b,
-                              k0 + j * 64, row, un.e, bar, pol_b, peer);
-                }
-              }
-            } else {
-#pragma unroll
-              for (int j = 0; j < T::kBSlabsMax; ++j) {
-                if (j >= b_slabs) break;
-                const int g = static_cast<int>(rank) * b_slabs + j;   // slab of the tile
-                int col = un.n + g * 64;
-                if constexpr (kSwiglu) {
-                  // the first half of the accumulator is up, the second gate
-                  const int half = p.acc_cols / 128;
-                  col = g < half ? un.n + g * 64 : p.N + un.n + (g - half) * 64;
-                }
-                tma_load_3d(b_dst + j * T::kBSlabBytes, &maps.b, col, k0, un.e, bar, pol_b, peer);
-              }
+              tma_load_3d(b_dst + j * T::kBSlabBytes, &maps.b, col, k0, un.e, bar, policy, peer);
             }
           }
-          if (++s == stages) {
-            s = 0;
-            ph ^= 1u;
-          }
-          // the next tile is looked up while this one's loads are under way
-          if (kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
         }
-      }
-      if (!ok) {
-        // loads in flight land before the CTA exits
-        const uint64_t t0 = ptx::globaltimer_ns();
-        while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+        if (++s == stages) {
+          s = 0;
+          ph ^= 1u;
+        }
+        // the next tile is looked up while this one's loads are under way
+        if (kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
       }
     }
+    if (!ok) {
+      // loads in flight land before the CTA exits
+      const uint64_t t0 = ptx::globaltimer_ns();
+      while (ptx::globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
+    }
+  };
+
+  if (warp == 0) {
+    if (lane == 0) produce(std::integral_constant<int, 0>{});
+  } else if (warp == 6) {
+    if (lane == 0) produce(std::integral_constant<int, 1>{});
   } else if (warp == 1) {
     // =========================== MMA issuer ===========================
     if (rank == 0 && lane == 0) {
@@ -587,6 +639,19 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
           ptx::make_idesc_bf16(kTileRows, p.acc_cols, /*a_mn_major=*/kWgrad,
                                /*b_mn_major=*/p.b_kmajor == 0);
       const bool b_kmajor = p.b_kmajor != 0;
+      // Shared-memory descriptors by halves, in units of 16 bytes: only the low word (address and
+      // leading-dimension offset) changes from MMA to MMA, by constants; putting the 64-bit
+      // descriptors together for each MMA kept the issuing thread busy for about 100 cycles.
+      const uint64_t desc0 = ptx::smem_desc_sw128(0, 0, 1024);
+      const uint32_t desc_hi = static_cast<uint32_t>(desc0 >> 32);
+      const uint32_t a_lo0 = static_cast<uint32_t>(
+          ptx::smem_desc_sw128(sA, kWgrad ? kBlockK * 128 : 16, 1024));
+      const uint32_t b_lo0 = static_cast<uint32_t>(
+          ptx::smem_desc_sw128(sB, b_kmajor ? 16 : T::kBSlabBytes, 1024));
+      const uint32_t a_step = static_cast<uint32_t>(a_stage) >> 4;
+      const uint32_t b_step = static_cast<uint32_t>(b_stage) >> 4;
+      const uint32_t a_box = static_cast<uint32_t>(p.a_rows) * 8u;      // one 64-deep box of A
+      const uint32_t b_box = static_cast<uint32_t>(b_slabs) * 512u;     // the same of B, K-major
       constexpr uint16_t mask = (kCtaGroup == 2) ? 0x3 : 0x1;
       int s = 0;
       uint32_t ph = 0;
@@ -606,11 +671,11 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         ptx::tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + as * kAccCols;
         const int num_kb = unit_kb(un);
+        const int last_steps = (unit_len(un) - (num_kb - 1) * kBlockK + 15) / 16;
         for (int kb = 0; kb < num_kb; ++kb) {
           // (a block that passed through the peer's tail warp carries its ordinary writes)
-          const bool tail = kWgrad && un.rows - kb * kBlockK < kBlockK;
           const bool landed =
-              (kCtaGroup == 2 && tail)
+              (kCtaGroup == 2 && mixed_block(un, kb))
                   ? ptx::mbar_wait_acquire_cluster(bar_full + 8 * s, ph, limit, abort_flag)
                   : ptx::mbar_wait(bar_full + 8 * s, ph, limit, abort_flag);
           if (!landed) {
@@ -619,19 +684,24 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             break;
           }
           ptx::tc_fence_after_sync();
-          const uint32_t a_base = sA + s * a_stage;
-          const uint32_t b_base = sB + s * b_stage;
+          const uint32_t a_lo = a_lo0 + static_cast<uint32_t>(s) * a_step;
+          const uint32_t b_lo = b_lo0 + static_cast<uint32_t>(s) * b_step;
+          auto step = [&](int kk) {
+            // 16 of the sum further: 32 bytes inside the 128-byte rows of a K-major operand (the
+            // next 64 in the next box), 16 rows of an MN-major one
+            const uint32_t a_off = kWgrad ? kk * 128u : (kk >> 2) * a_box + (kk & 3) * 2u;
+            const uint32_t b_off = b_kmajor ? (kk >> 2) * b_box + (kk & 3) * 2u : kk * 128u;
+            umma_bf16_lohi<kCtaGroup>(d_tmem, a_lo + a_off, b_lo + b_off, desc_hi, idesc,
+                                      (kb > 0 || kk > 0) ? 1u : 0u);
+          };
+          if (kb < num_kb - 1 || last_steps == kBlockK / 16) {
 #pragma unroll
-          for (int kk = 0; kk < kBlockK / 16; ++kk) {
-            const uint64_t a_desc =
-                kWgrad ? ptx::smem_desc_sw128(a_base + kk * 16 * 128, kBlockK * 128, 1024)
-                       : ptx::smem_desc_sw128(
-                             a_base + (kk >> 2) * (p.a_rows * 128) + (kk & 3) * 32, 16, 1024);
-            const uint64_t b_desc =
-                b_kmajor ? ptx::smem_desc_sw128(
-                               b_base + (kk >> 2) * (b_slabs * 64 * 128) + (kk & 3) * 32, 16, 1024)
-                         : ptx::smem_desc_sw128(b_base + kk * 16 * 128, T::kBSlabBytes, 1024);
-            ptx::umma_bf16<kCtaGroup>(d_tmem, a_desc, b_desc, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+            for (int kk = 0; kk < kBlockK / 16; ++kk) step(kk);
+          } else {
+            // the last block is padded (zero fill from TMA, or rows that the tail warp cleared
+            // up to a whole step): only the steps the sum still has
+#pragma unroll 1
+            for (int kk = 0; kk < last_steps; ++kk) step(kk);
           }
           ptx::umma_commit<kCtaGroup>(bar_empty + 8 * s, mask);
           if (++s == stages) {
@@ -643,7 +713,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         if (ok) ptx::umma_commit<kCtaGroup>(bar_tfull + 8 * as, mask);
       }
     }
-  } else if (warp == 6) {
+  } else if (warp == 7) {
     // =========================== tail warp (EXP_WGRAD) ===========================
     if constexpr (kWgrad) {
       // Walks the same sequence of blocks as the producer; acts on the ones a group ends in.
@@ -654,8 +724,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       for (int u = cluster_id; u < total_units; u += num_clusters) {
         const Unit un = unit_of(u);
         const int num_kb = unit_kb(un);
-        const int valid = un.rows - (num_kb - 1) * kBlockK;    // rows of the last block
-        if (num_kb > 0 && valid < kBlockK) {
+        if (num_kb > 0 && mixed_block(un, num_kb - 1)) {
+          const int valid = un.rows - (num_kb - 1) * kBlockK;    // rows of the last block
           const int64_t b = block + num_kb - 1;
           const int s = static_cast<int>(b % stages);
           const bool landed =
@@ -665,10 +735,10 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             break;
           }
           parities ^= 1u << s;
-          // rows [valid, kBlockK) of every 64-column slab, whole 128-byte rows (the swizzle
-          // moves 16-byte pieces only inside a row)
+          // rows from `valid` to the end of their step of 16 in every 64-column slab: whole
+          // 128-byte rows (the swizzle moves 16-byte pieces only inside a row)
           const uint32_t a0 = sA + s * a_stage, b0 = sB + s * b_stage;
-          const int pieces = (kBlockK - valid) * 8;
+          const int pieces = (16 - (valid & 15)) * 8;
           for (int slab = 0; slab < kBlockM / 64 + b_slabs; ++slab) {
             const uint32_t at = (slab < kBlockM / 64 ? a0 + slab * (kBlockK * 128)
                                                      : b0 + (slab - kBlockM / 64) * T::kBSlabBytes) +
@@ -677,7 +747,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
           }
           ptx::fence_proxy_async_smem();
           __syncwarp();
-          if (lane == 0) {
+          if (lane < 2) {   // for both producers
             const uint32_t full_local = bar_full + 8 * s;
             if constexpr (kCtaGroup == 2) {
               ptx::mbar_arrive_release_cluster(ptx::mapa(full_local, 0));
@@ -821,6 +891,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       } else if constexpr (kForm == EXP_GEMM32) {
         // ---- fp32 result, 32 columns at a time, two buffers ----
         const int units = tile_cols / 32;
+        const int slot = splits > 1 ? un.k0 / p.k_per_split : 0;
         for (int c = 0; c < units; ++c) {
           const int x = un.n + c * 32;
           const bool last = c == units - 1;
@@ -841,12 +912,13 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
             if (valid == 32) {
               ptx::fence_proxy_async_smem();
               __syncwarp();
-              if (lane == 0) ptx::tma_store_2d(&maps.out, x, static_cast<int>(grow), buf, pol_out);
+              if (lane == 0)
+                tma_store_3d(&maps.out, x, static_cast<int>(grow), slot, buf, pol_out);
             } else {
               __syncwarp();
               copy_rows<128>(buf,
                              reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) +
-                                                        grow * p.ld_out + x),
+                                                        slot * p.slot_stride + grow * p.ld_out + x),
                              p.ld_out * 4, valid, (p.N - x < 32 ? p.N - x : 32) * 4, lane);
               __syncwarp();
             }

@@ -118,6 +118,9 @@ def test_workspace_holds_every_part():
     n = sg.experts_swiglu_workspace_bytes(T, k, E, D, N, Do)
     assert n >= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + 2 * Do)
     assert n <= 4 * (E + 1) + 8 * T * k + 2 * T * k * (D + N + 2 * Do) + 6 * 256
+    # few rows and a long sum: partial rows of the down projection
+    one = sg.experts_swiglu_workspace_bytes(1, 2, 8, 64, 14336, 4096)
+    assert one >= 2 * 2 * (64 + 14336) + 2 * 4096 * 4 * 8
     with pytest.raises(ValueError):
         sg.experts_swiglu_workspace_bytes(1, 65, E, D, N, Do)
 
