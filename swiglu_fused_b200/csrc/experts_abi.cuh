@@ -23,12 +23,16 @@ ExpertVariant make_expert_variant() {
 }
 
 constexpr int kExpertVariants = sgl::EXP_FORMS * 2;   // form * 2 + (cta_group - 1)
+// Depth of a ring stage.  The weight gradient sums over a group's rows, often a few hundred: its
+// operands come in steps of 64 (126 experts, about 48 rows each: 272 us instead of 280).
 constexpr int kExpertBlockK = 128;
+constexpr int kWgradBlockK = 64;
 
 template <int F>
 void fill_expert_form(ExpertVariant* table) {
-  table[F * 2] = make_expert_variant<F, 1, kExpertBlockK>();
-  table[F * 2 + 1] = make_expert_variant<F, 2, kExpertBlockK>();
+  constexpr int kBlockK = F == sgl::EXP_WGRAD ? kWgradBlockK : kExpertBlockK;
+  table[F * 2] = make_expert_variant<F, 1, kBlockK>();
+  table[F * 2 + 1] = make_expert_variant<F, 2, kBlockK>();
 }
 
 const ExpertVariant& expert_variant(int form, int cta_group) {
@@ -215,14 +219,18 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   const int64_t groups_used = wgrad ? s.E : (s.E < s.R ? s.E : s.R);
   const int64_t max_tiles_m = wgrad ? (s.M + tile_rows - 1) / tile_rows * s.E
                                     : s.R / tile_rows + groups_used;
-  // Single-CTA tiles: half as wide while there are fewer than two for each SM.  (64 columns are
+  // Single-CTA tiles: half as wide while there are fewer than two for each SM, four where the
+  // groups are short and the weight's stream is all there is to balance (64 tokens x 8 of 64
+  // experts, 1024 -> 2048: 50 us at 256 columns, 46 at 128).  (64 columns are
   // not worth it: a k-block takes 0.5 us at 64 and at 128 columns.  8 tokens x 2 of 8 experts,
   // 14336 -> 4096: 255 us at 64 columns, 142 at 128.)
   int acc_cols = sgl::kAccCols;
   const int min_cols = 128;
   if (cta_group == 1 && !wgrad) {
     const int64_t cols = swiglu ? acc_cols / 2 : acc_cols;
-    if (max_tiles_m * ((s.N + cols - 1) / cols) * s.splits < 2 * info->sm_count) acc_cols = min_cols;
+    if (max_tiles_m * ((s.N + cols - 1) / cols) * s.splits <
+        (s.R / s.E < 64 ? 4 : 2) * info->sm_count)
+      acc_cols = min_cols;
   }
   int a_rows = sgl::kBlockM;
   if (cta_group == 1 && !wgrad && s.R <= 32) a_rows = static_cast<int>((s.R + 15) / 16 * 16);
@@ -248,8 +256,8 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   const int64_t pre_pitch = grad ? s.ld_pre * 2 : pl.pitch;
   const int64_t pre_gate = grad ? s.N * 2 : pl.gate_off;
   if (wgrad) {
-    if ((rc = make_expert_map(&maps.a, s.a, s.M, s.R, 0, s.lda * 2, 0, 64, kExpertBlockK, "a")) ||
-        (rc = make_expert_map(&maps.b, s.b, s.N, s.R, 0, s.ldb * 2, 0, 64, kExpertBlockK, "g")) ||
+    if ((rc = make_expert_map(&maps.a, s.a, s.M, s.R, 0, s.lda * 2, 0, 64, kWgradBlockK, "a")) ||
+        (rc = make_expert_map(&maps.b, s.b, s.N, s.R, 0, s.ldb * 2, 0, 64, kWgradBlockK, "g")) ||
         (rc = make_expert_map(&maps.out, s.out, s.N, s.M, s.E, s.ld_out * 2, s.out_stride * 2, 64,
                               32, "out", kBf16, kSw128, kNoPromo)))
       return rc;
@@ -879,13 +887,20 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
   p.ldh = ldh;
   p.rows = rows;
   p.nvec = static_cast<int>(N / 8);
-  const int64_t vecs = rows * p.nvec;
-  int64_t blocks = (vecs + 255) / 256;
-  const int64_t cap = static_cast<int64_t>(info->sm_count) * 8;
-  if (blocks > cap) blocks = cap;
+  // two vectors of 8 columns per thread where a row has more than a CTA's threads
+  const int vecs = p.nvec > sgl::kPreactThreads ? 2 : 1;
+  const int64_t per_cta = static_cast<int64_t>(sgl::kPreactThreads) * vecs;
+  const int64_t chunks = (p.nvec + per_cta - 1) / per_cta;
+  int64_t pairs = (rows + 1) / 2;
+  const int64_t cap = (static_cast<int64_t>(info->sm_count) * 32 + chunks - 1) / chunks;
+  if (pairs > cap) pairs = cap;
   return launch_after("grad_preact_saved",
-                      bits == 8 ? sgl::grad_preact_saved_kernel<8> : sgl::grad_preact_saved_kernel<16>,
-                      dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+                      bits == 8 ? (vecs == 2 ? sgl::grad_preact_saved_kernel<8, 2>
+                                             : sgl::grad_preact_saved_kernel<8, 1>)
+                                : (vecs == 2 ? sgl::grad_preact_saved_kernel<16, 2>
+                                             : sgl::grad_preact_saved_kernel<16, 1>),
+                      dim3(static_cast<unsigned>(chunks), static_cast<unsigned>(pairs)),
+                      dim3(sgl::kPreactThreads), 0, stream, p);
 }
 
 // ---- the expert layer at inference, one call ----

@@ -290,22 +290,18 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
 }
 
 // 32 saved up and gate values of one row, columns x .. x + 31 (a block; the halves are padded to
-// whole blocks, so the last one may be read past N).  Rows that do not exist are not read.
+// whole blocks, so the last one may be read past N), kept as loaded until they are used.
 template <int kBits>
-__device__ __forceinline__ void load_saved(const ExpertParams& p, int64_t row, int x, bool live,
-                                           float (&up)[32], float (&gate)[32]) {
-  const uint8_t* at = p.saved + row * p.ld_saved + x * (kBits / 8);
-  constexpr int kVecs = 32 * kBits / 8 / 16;
-  uint4 u[kVecs], g[kVecs];
-  int su = 0, sg = 0;
+struct SavedBlock {
+  static constexpr int kLoads = 32 * kBits / 8 / 16;
+  uint4 u[kLoads], g[kLoads];
+  int su, sg;
+  // Rows that do not exist are not read.
+  __device__ __forceinline__ void load(const ExpertParams& p, int64_t row, int x, bool live) {
+    if (!live) return;
+    const uint8_t* at = p.saved + row * p.ld_saved + x * (kBits / 8);
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    u[i] = make_uint4(0, 0, 0, 0);
-    g[i] = u[i];
-  }
-  if (live) {
-#pragma unroll
-    for (int i = 0; i < kVecs; ++i) {
+    for (int i = 0; i < kLoads; ++i) {
       u[i] = reinterpret_cast<const uint4*>(at)[i];
       g[i] = reinterpret_cast<const uint4*>(at + p.saved_gate_off)[i];
     }
@@ -315,29 +311,37 @@ __device__ __forceinline__ void load_saved(const ExpertParams& p, int64_t row, i
       sg = sc[p.gate_scale_off];
     }
   }
-  const float fu = kBits == 8 ? block_scale(su) : 1.f, fg = kBits == 8 ? block_scale(sg) : 1.f;
+  __device__ __forceinline__ void get(float (&up)[32], float (&gate)[32]) const {
+    const float fu = kBits == 8 ? block_scale(su) : 1.f, fg = kBits == 8 ? block_scale(sg) : 1.f;
 #pragma unroll
-  for (int i = 0; i < kVecs; ++i) {
-    const uint32_t wu[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-    const uint32_t wg[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
+    for (int i = 0; i < kLoads; ++i) {
+      const uint32_t wu[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+      const uint32_t wg[4] = {g[i].x, g[i].y, g[i].z, g[i].w};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (kBits == 8) {
-        const int o = i * 16 + j * 4;
-        const float2 u0 = e4m3x2_to_f32(wu[j]), u1 = e4m3x2_to_f32(wu[j] >> 16);
-        const float2 g0 = e4m3x2_to_f32(wg[j]), g1 = e4m3x2_to_f32(wg[j] >> 16);
-        up[o] = u0.x * fu; up[o + 1] = u0.y * fu; up[o + 2] = u1.x * fu; up[o + 3] = u1.y * fu;
-        gate[o] = g0.x * fg; gate[o + 1] = g0.y * fg; gate[o + 2] = g1.x * fg; gate[o + 3] = g1.y * fg;
-      } else {
-        const int o = i * 8 + j * 2;
-        up[o] = __uint_as_float(wu[j] << 16);
-        up[o + 1] = __uint_as_float(wu[j] & 0xffff0000u);
-        gate[o] = __uint_as_float(wg[j] << 16);
-        gate[o + 1] = __uint_as_float(wg[j] & 0xffff0000u);
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (kBits == 8) {
+          const int o = i * 16 + j * 4;
+          const float2 u0 = e4m3x2_to_f32(wu[j]), u1 = e4m3x2_to_f32(wu[j] >> 16);
+          const float2 g0 = e4m3x2_to_f32(wg[j]), g1 = e4m3x2_to_f32(wg[j] >> 16);
+          up[o] = u0.x * fu;
+          up[o + 1] = u0.y * fu;
+          up[o + 2] = u1.x * fu;
+          up[o + 3] = u1.y * fu;
+          gate[o] = g0.x * fg;
+          gate[o + 1] = g0.y * fg;
+          gate[o + 2] = g1.x * fg;
+          gate[o + 3] = g1.y * fg;
+        } else {
+          const int o = i * 8 + j * 2;
+          up[o] = __uint_as_float(wu[j] << 16);
+          up[o + 1] = __uint_as_float(wu[j] & 0xffff0000u);
+          gate[o] = __uint_as_float(wg[j] << 16);
+          gate[o + 1] = __uint_as_float(wg[j] & 0xffff0000u);
+        }
       }
     }
   }
-}
+};
 
 // ---------------------------------------------------------------- the kernel
 
@@ -805,7 +809,10 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         const int units = tile_cols / 32;
         const bool live = lane < valid;
         float weight = 1.0f;
+        // the saved values of a unit are fetched while the one before is worked on
+        SavedBlock<kForm == EXP_GRAD8 ? 8 : 16> saved{};
         if constexpr (T::kGrad) {
+          saved.load(p, grow + lane, un.n, live);
           if (p.slots != nullptr && live) {
             const int64_t slot = p.slots[grow + lane];
             weight = 0.f;
@@ -831,7 +838,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
               for (int j = 0; j < 32; ++j) h[j] = silu_mul(b[j], a[j]);
             } else {
               // this row's 32 saved up and gate values, then the gradients in their place
-              load_saved<kForm == EXP_GRAD8 ? 8 : 16>(p, grow + lane, x, live, a, b);
+              saved.get(a, b);
+              if (!last && x + 32 < p.N) saved.load(p, grow + lane, x + 32, live);
               ptx::tmem_ld_32x32b_x32(t_row + c * 32, h);
               ptx::tmem_ld_wait();
               if (last) hand_back();
