@@ -440,6 +440,29 @@ int check_bits(int bits) {
 
 extern "C" {
 
+// First use on a device: the ordering kernels' shared-memory limit (1024 experts need 139 KB).
+static int prepare_order_kernels() {
+  int dev = 0;
+  int rc = current_device(&dev);
+  if (rc) return rc;
+  std::lock_guard<std::mutex> lock(g_dev_mutex);
+  ExpertDevice& d = g_expert_devices[dev];
+  if (d.order_ready) return SGL_OK;
+  const int most = sgl::order_smem_bytes(sgl::kOrderMaxExperts);
+  cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_order_kernel),
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_count_kernel),
+                             cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  if (e == cudaSuccess)
+    e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_order_dispatch_kernel),
+                             cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             most + sgl::kOrderRound * 4);
+  if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(expert_order)");
+  d.order_ready = true;
+  return SGL_OK;
+}
+
 // CTAs that order T * k slots, and the slots of each: a round of slots each if there are few, fewer
 // CTAs when the table of counts, which every CTA reads, would grow past
 // 64 Ki entries.
@@ -490,22 +513,7 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
   DeviceInfo* info = nullptr;
   if ((rc = check_device(&info))) return rc;
   const int smem = sgl::order_smem_bytes(static_cast<int>(E));
-  if (smem > 48 * 1024) {
-    int dev = 0;
-    if ((rc = current_device(&dev))) return rc;
-    std::lock_guard<std::mutex> lock(g_dev_mutex);
-    ExpertDevice& d = g_expert_devices[dev];
-    if (!d.order_ready) {
-      const int most = sgl::order_smem_bytes(sgl::kOrderMaxExperts);
-      cudaError_t e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_order_kernel),
-                                           cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-      if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(reinterpret_cast<const void*>(sgl::expert_count_kernel),
-                                 cudaFuncAttributeMaxDynamicSharedMemorySize, most);
-      if (e != cudaSuccess) return fail_cuda(e, "cudaFuncSetAttribute(expert_order)");
-      d.order_ready = true;
-    }
-  }
+  if ((rc = prepare_order_kernels())) return rc;
   p.ids = ids;
   p.ld_ids = ld_ids;
   p.total = T * k;
@@ -917,8 +925,8 @@ struct ExpertsWorkspace {
 // idle while others stream long columns of weight.  Its sum is cut into ranges of at least 512
 // whose partial rows the combine step adds up in order: as many as give every SM about four
 // tiles if all groups are used, while the partial rows written and read stay below an eighth of
-// the weight.  A function of the sizes alone.  1 token x 2 of 8 experts, 14336 -> 4096: XXX us
-// in one range, XXX us in XXX.
+// the weight.  A function of the sizes alone.  1 token x 2 of 8 experts, 14336 -> 4096: 59 us
+// in one range, 43 us in eight.
 static void down_ranges(int64_t R, int64_t E, int64_t N, int64_t D_out, int* splits,
                         int64_t* per_split) {
   *splits = 1;
@@ -929,7 +937,7 @@ static void down_ranges(int64_t R, int64_t E, int64_t N, int64_t D_out, int* spl
   int64_t s = (4 * 148 + tiles - 1) / tiles;
   if (s > N / 512) s = N / 512;
   if (s > groups * N / (32 * R)) s = groups * N / (32 * R);
-  if (s > 16) s = 16;
+  if (s > 8) s = 8;          // (what the combine step has in flight at once)
   if (s < 2) return;
   *per_split = (((N + s - 1) / s) + 127) / 128 * 128;
   *splits = static_cast<int>((N + *per_split - 1) / *per_split);
@@ -999,10 +1007,36 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
     return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t R = T * k;
-  if ((rc = sgl_expert_order(ids, ids_are_int64, T, k, ld_ids, E, ws + l.offsets, ws + l.slots,
-                             ws + l.rows, ws + l.scratch, l.scratch_bytes, stream)) ||
-      (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream)) ||
-      (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
+  if (R <= sgl::kOrderRound) {
+    DeviceInfo* info = nullptr;
+    if ((rc = check_device(&info)) || (rc = prepare_order_kernels())) return rc;
+    sgl::OrderParams p;
+    std::memset(&p, 0, sizeof(p));
+    p.ids = ids;
+    p.ld_ids = ld_ids;
+    p.total = p.per_cta = R;
+    p.k = static_cast<int>(k);
+    p.E = static_cast<int>(E);
+    p.ids64 = ids_are_int64 != 0;
+    p.offsets = reinterpret_cast<int*>(ws + l.offsets);
+    p.slots = reinterpret_cast<int*>(ws + l.slots);
+    p.rows = reinterpret_cast<int*>(ws + l.rows);
+    int64_t ctas = (T + 3) / 4;
+    if (ctas > info->sm_count) ctas = info->sm_count;
+    rc = launch_after("expert_order_dispatch", sgl::expert_order_dispatch_kernel,
+                      dim3(static_cast<unsigned>(ctas)), dim3(sgl::kOrderThreads),
+                      sgl::order_smem_bytes(static_cast<int>(E)) + sgl::kOrderRound * 4, stream, p,
+                      static_cast<const __nv_bfloat16*>(x),
+                      reinterpret_cast<__nv_bfloat16*>(ws + l.xs), ldx, static_cast<int64_t>(D),
+                      static_cast<int>(D / 8));
+    if (rc) return rc;
+  } else if ((rc = sgl_expert_order(ids, ids_are_int64, T, k, ld_ids, E, ws + l.offsets,
+                                    ws + l.slots, ws + l.rows, ws + l.scratch, l.scratch_bytes,
+                                    stream)) ||
+             (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream))) {
+    return rc;
+  }
+  if ((rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
                                      w_stride, N, stream)) ||
       (rc = grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
                            d_stride, D_out, 0, 1, l.splits, l.k_per_split, stream)))

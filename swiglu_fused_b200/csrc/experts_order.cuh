@@ -181,6 +181,63 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
   for (int64_t i = kept + tid; i < p.total; i += kOrderThreads) p.slots[i] = -1;
 }
 
+// The same, and x's rows sent on in the same launch (sgl_experts_swiglu with few slots): every CTA
+// orders all slots for itself, the first writes the order, and each copies its share of the
+// tokens.  64 tokens x 8 of 64 experts, 2048 x 1024: the layer takes 145 us instead of 151.
+__global__ void __launch_bounds__(kOrderThreads, 1)
+expert_order_dispatch_kernel(const OrderParams p, const __nv_bfloat16* x, __nv_bfloat16* out,
+                             int64_t ldx, int64_t ldo, int nvec) {
+  extern __shared__ int order_smem[];
+  const int E = p.E, tid = threadIdx.x;
+  int* count = order_smem;
+  int* total = count + kOrderWarps * E;
+  int* start = total + E;
+  int* scratch = start + E;
+  int* row_of_slot = scratch + 40;       // [kOrderRound]
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  for (int e = tid; e < E; e += kOrderThreads) total[e] = 0;
+  OrderRound r;
+  r.run(p, 0, p.total, count, total);
+  int kept;
+  const int first = order_scan(tid < E ? total[tid] : 0, scratch, &kept);
+  const bool writer = blockIdx.x == 0;
+  if (tid < E) {
+    start[tid] = first;
+    if (writer) p.offsets[tid] = first;
+  }
+  if (writer && tid == 0) p.offsets[E] = kept;
+  __syncthreads();
+#pragma unroll
+  for (int u = 0; u < kOrderSteps; ++u) {
+    const int64_t s = r.slot_of(u);
+    if (u < r.steps && s < p.total) {
+      const int row = r.key[u] >= 0 ? start[r.key[u]] + r.rank[u] : -1;
+      row_of_slot[s] = row;
+      if (writer) {
+        p.rows[s] = row;
+        if (row >= 0) p.slots[row] = static_cast<int>(s);
+      }
+    }
+  }
+  if (writer)
+    for (int64_t i = kept + tid; i < p.total; i += kOrderThreads) p.slots[i] = -1;
+  __syncthreads();
+  // 256 threads to a token
+  const int tokens = static_cast<int>(p.total) / p.k;
+  for (int t = blockIdx.x * (kOrderThreads / 256) + tid / 256; t < tokens;
+       t += gridDim.x * (kOrderThreads / 256)) {
+    const uint4* src = reinterpret_cast<const uint4*>(x + t * ldx);
+    for (int v = tid % 256; v < nvec; v += 256) {
+      const uint4 val = src[v];
+      for (int j = 0; j < p.k; ++j) {
+        const int row = row_of_slot[t * p.k + j];
+        if (row >= 0) reinterpret_cast<uint4*>(out + row * ldo)[v] = val;
+      }
+    }
+  }
+}
+
 // More slots: one range per CTA.  The first kernel leaves every slot's rank inside its CTA in
 // `rows` and the CTA's counts in `counts`; the second adds up the counts of the CTAs before it
 // (all of them read the whole table, CTAs * E words from L2) and places its slots.  262144 slots
