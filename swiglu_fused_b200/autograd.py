@@ -10,6 +10,7 @@ module (``swiglu/triton/impls.py:2913-3369``) and runs the two GEMMs through cuB
 from __future__ import annotations
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .experts import (ExpertOrder, SavedPreact, _checkpoint_bits, _layer_operands, expert_combine,
                       expert_combine_grad, expert_dispatch, expert_order, grouped_fused_swiglu_save,
@@ -45,6 +46,13 @@ class FusedSwiGLUFunction(torch.autograd.Function):
         return grad_x, grad_w
 
 
+def _rows_of_gradient(g: torch.Tensor) -> torch.Tensor:
+    """An incoming gradient as the kernels take it: dense rows, 16-byte aligned (a gradient may be
+    a broadcast value or a slice that starts anywhere)."""
+    g = g.contiguous()
+    return g if g.data_ptr() % 16 == 0 else g.clone()
+
+
 class FusedSwiGLUPreactFunction(torch.autograd.Function):
     """The same stage over saved pre-activations (8 bits or bf16) instead of the two factors.  The
     backward recomputes what it needs from them and leaves them as they are."""
@@ -57,10 +65,11 @@ class FusedSwiGLUPreactFunction(torch.autograd.Function):
         return h
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_h: torch.Tensor):
         x, w, data, scales = ctx.saved_tensors
         pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
-        grad_preact = swiglu_grad_preact_saved(grad_h.contiguous(), pre)
+        grad_preact = swiglu_grad_preact_saved(_rows_of_gradient(grad_h), pre)
         if x.shape[0] == 0:
             return torch.zeros_like(x), torch.zeros_like(w), None
         grad_x = matmul_bf16(grad_preact, w, transpose_b=True) if ctx.needs_input_grad[0] else None
@@ -105,6 +114,7 @@ class FusedSwiGLUExpertsFunction(torch.autograd.Function):
         return y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, grad_y: torch.Tensor):
         x, weights, w, w_down, offsets, slots, rows, data, scales, ys = ctx.saved_tensors
         need_x, _, need_weights, need_w, need_down, _ = ctx.needs_input_grad
@@ -113,7 +123,7 @@ class FusedSwiGLUExpertsFunction(torch.autograd.Function):
                     torch.zeros_like(w_down), None)
         order = ExpertOrder(offsets, slots, rows)
         # the rows' gradients without the routing weights, and the weights' own
-        grad_rows, grad_weights = expert_combine_grad(grad_y.contiguous(), ys, order, weights,
+        grad_rows, grad_weights = expert_combine_grad(_rows_of_gradient(grad_y), ys, order, weights,
                                                       weighted=False)
         grad_x = grad_w = grad_down = None
         if need_x or need_w or need_down:

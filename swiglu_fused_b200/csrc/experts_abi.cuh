@@ -203,11 +203,14 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   const bool grad = s.form == sgl::EXP_GRAD16 || s.form == sgl::EXP_GRAD8;
   const bool swiglu = s.form == sgl::EXP_SWIGLU || save;
 
-  // CTA pairs (256-row tiles) once the groups fill them on average; single CTAs (128 rows) else.
+  // CTA pairs (256-row tiles) once the groups have that many rows on average, single CTAs (128
+  // rows) below: a pair fetches each weight for twice the rows, but a group's last tile is half
+  // empty on average.  64 experts, 2048 x 1024, gate/up stage: 384 rows each 206 us in pairs and
+  // 225 in single CTAs, 192 rows 147 and 142, 64 rows 110 and 94.
   int cta_group = 1;
   if (wgrad) {
     cta_group = s.M > sgl::kBlockM ? 2 : 1;
-  } else if (s.R / s.E >= 192) {
+  } else if (s.R / s.E >= 256) {
     cta_group = 2;
   }
   int clusters = 0;
@@ -337,14 +340,14 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   lc.dynamicSmemBytes = static_cast<size_t>(smem);
   lc.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attrs[2];
-  attrs[0].id = cudaLaunchAttributeClusterDimension;
-  attrs[0].val.clusterDim.x = static_cast<unsigned>(cta_group);
-  attrs[0].val.clusterDim.y = 1;
-  attrs[0].val.clusterDim.z = 1;
-  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[0].val.programmaticStreamSerializationAllowed = 1;
+  attrs[1].id = cudaLaunchAttributeClusterDimension;
+  attrs[1].val.clusterDim.x = static_cast<unsigned>(cta_group);
+  attrs[1].val.clusterDim.y = 1;
+  attrs[1].val.clusterDim.z = 1;
   lc.attrs = attrs;
-  lc.numAttrs = 2;
+  lc.numAttrs = cta_group == 2 ? 2 : 1;
   if (log_enabled())
     fprintf(stderr,
             "[libswiglu_b200] launch sgl %s R=%lld N=%lld K=%lld M=%lld E=%lld cta_group=%d "

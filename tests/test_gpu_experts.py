@@ -639,6 +639,29 @@ def test_some_leaves_without_gradients():
     assert all(t.grad is not None and torch.isfinite(t.grad).all() for t in every)
 
 
+def test_gradients_that_start_anywhere_and_second_derivatives():
+    x, ids, rw, w, wd = layer_inputs(30, 2, 4, 64, 72, 3)
+    leaves = [t.requires_grad_(True) for t in (x, rw, w, wd)]
+    flat = randn(30 * 64 + 3, seed=2)
+    dy = flat[3:].view(30, 64)                     # contiguous, not 16-byte aligned
+    assert dy.data_ptr() % 16
+    got = torch.autograd.grad(sg.fused_swiglu_experts(x, ids, rw, w, wd), leaves, dy)
+    want = torch.autograd.grad(sg.fused_swiglu_experts(x, ids, rw, w, wd), leaves, dy.clone())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    xs, ws = randn(40, 64).requires_grad_(True), randn(64, 144, std=0.1).requires_grad_(True)
+    flat = randn(40 * 72 + 1, seed=5)
+    h = sg.fused_swiglu(xs, ws, checkpoint="e4m3")
+    a = torch.autograd.grad(h, (xs, ws), flat[1:].view(40, 72), retain_graph=True)
+    b = torch.autograd.grad(h, (xs, ws), flat[1:].view(40, 72).clone())
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    # no second derivatives: an error, not a zero
+    for out, leaf in ((sg.fused_swiglu(xs, ws, checkpoint="bf16"), xs),
+                      (sg.fused_swiglu_experts(x, ids, rw, w, wd), x)):
+        g, = torch.autograd.grad(out.float().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.float().sum().backward()
+
+
 def test_module_runs_and_trains():
     torch.manual_seed(0)
     B, S, D, N, E, k = 3, 17, 64, 72, 4, 2
