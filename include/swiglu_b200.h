@@ -602,6 +602,18 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
                                  int64_t N, int64_t lddy, int64_t ldo, int64_t ldh, void* stream);
 
 /*
+ * The dense stage's backward from saved pre-activations, one call: the step above, then
+ * grad_x[M, K] = grad_preact @ w^T and grad_w[K, 2N] = x^T @ grad_preact (either may be NULL) with
+ * sgl_matmul_bf16_ex.  grad_preact [M, 2N] is the caller's; it and the gradients are dense.
+ * cfg_x and cfg_w as for sgl_matmul_bf16_ex, or NULL.
+ */
+int sgl_fused_swiglu_backward_saved(const void* x, const void* w, const void* dy, const void* pre,
+                                    const void* scales, int bits, void* grad_preact, void* grad_x,
+                                    void* grad_w, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                    int64_t ldw, int64_t lddy, const sgl_config* cfg_x,
+                                    const sgl_config* cfg_w, void* stream);
+
+/*
  * The whole expert layer at inference: order, dispatch, gate/up stage, down projection, combine.
  *   y[t] = sum_j weights[t, j] * (silu(x[t] @ Wg) * (x[t] @ Wu)) @ Wd,  expert ids[t, j]
  * x[T, D], w[E, D, 2N], w_down[E, N, D_out], y[T, D_out].  `workspace`: caller-owned device memory

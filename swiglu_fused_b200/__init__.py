@@ -12,6 +12,7 @@ from ._lib import TileConfig, SglError
 from .autograd import fused_swiglu, fused_swiglu_experts
 from .experts import (ExpertOrder, SavedPreact, expert_combine, expert_combine_grad, expert_dispatch,
                       expert_order, experts_swiglu, experts_swiglu_workspace_bytes,
+                      fused_swiglu_backward_saved,
                       grouped_fused_swiglu, grouped_fused_swiglu_save, grouped_grad_preact,
                       grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
                       swiglu_grad_preact_saved)
@@ -40,6 +41,7 @@ __all__ = [
     "experts_swiglu_workspace_bytes",
     "matmul_fused_swiglu_save_preact",
     "swiglu_grad_preact_saved",
+    "fused_swiglu_backward_saved",
     "ExpertOrder",
     "SavedPreact",
     "PackedSwiGLULinear",

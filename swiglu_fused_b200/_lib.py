@@ -87,6 +87,7 @@ EXPORTED_SYMBOLS = (
     "sgl_grouped_weight_grad",
     "sgl_preact_bytes",
     "sgl_swiglu_grad_preact_saved",
+    "sgl_fused_swiglu_backward_saved",
     "sgl_experts_swiglu_workspace_bytes",
     "sgl_experts_swiglu",
     "sgl_last_error",
@@ -305,6 +306,9 @@ def load() -> C.CDLL:
         lib.sgl_preact_bytes.argtypes = [ip, i64, i64] + [C.POINTER(i64)] * 3
         lib.sgl_swiglu_grad_preact_saved.restype = ip
         lib.sgl_swiglu_grad_preact_saved.argtypes = [vp, vp, vp, ip, vp, vp, vp] + [i64] * 5 + [vp]
+        lib.sgl_fused_swiglu_backward_saved.restype = ip
+        lib.sgl_fused_swiglu_backward_saved.argtypes = [vp] * 5 + [ip, vp, vp, vp] + [i64] * 6 + \
+            [cfgp, cfgp, vp]
         lib.sgl_experts_swiglu_workspace_bytes.restype = i64
         lib.sgl_experts_swiglu_workspace_bytes.argtypes = [i64] * 6
         lib.sgl_experts_swiglu.restype = ip

@@ -13,9 +13,9 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .experts import (ExpertOrder, SavedPreact, _checkpoint_bits, _layer_operands, expert_combine,
-                      expert_combine_grad, expert_dispatch, expert_order, grouped_fused_swiglu_save,
-                      grouped_grad_preact, grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
-                      swiglu_grad_preact_saved)
+                      expert_combine_grad, expert_dispatch, expert_order,
+                      fused_swiglu_backward_saved, grouped_fused_swiglu_save, grouped_grad_preact,
+                      grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact)
 from .ops import matmul_bf16, matmul_fused_swiglu_save_factors, swiglu_grad_preact
 
 
@@ -68,12 +68,9 @@ class FusedSwiGLUPreactFunction(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, grad_h: torch.Tensor):
         x, w, data, scales = ctx.saved_tensors
-        pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
-        grad_preact = swiglu_grad_preact_saved(_rows_of_gradient(grad_h), pre)
-        if x.shape[0] == 0:
-            return torch.zeros_like(x), torch.zeros_like(w), None
-        grad_x = matmul_bf16(grad_preact, w, transpose_b=True) if ctx.needs_input_grad[0] else None
-        grad_w = matmul_bf16(x, grad_preact, transpose_a=True) if ctx.needs_input_grad[1] else None
+        grad_x, grad_w = fused_swiglu_backward_saved(
+            x, w, _rows_of_gradient(grad_h), SavedPreact(data, scales, ctx.bits, ctx.hidden),
+            need_x=ctx.needs_input_grad[0], need_w=ctx.needs_input_grad[1])
         return grad_x, grad_w, None
 
 

@@ -914,6 +914,35 @@ int sgl_swiglu_grad_preact_saved(const void* dy, const void* pre, const void* sc
                       dim3(sgl::kPreactThreads), 0, stream, p);
 }
 
+int sgl_fused_swiglu_backward_saved(const void* x, const void* w, const void* dy, const void* pre,
+                                    const void* scales, int bits, void* grad_preact, void* grad_x,
+                                    void* grad_w, int64_t M, int64_t N, int64_t K, int64_t ldx,
+                                    int64_t ldw, int64_t lddy, const sgl_config* cfg_x,
+                                    const sgl_config* cfg_w, void* stream) {
+  int rc;
+  // everything the launches below would refuse is refused before the first of them
+  if ((rc = validate_ptr(x, "x")) || (rc = validate_ptr(w, "w"))) return rc;
+  if ((grad_x && (rc = validate_ptr(grad_x, "grad_x"))) ||
+      (grad_w && (rc = validate_ptr(grad_w, "grad_w"))))
+    return rc;
+  if ((rc = validate_shape(M, N, K))) return rc;
+  if ((rc = validate_ld(ldx, K, "ldx")) || (rc = validate_ld(ldw, 2 * N, "ldw"))) return rc;
+  sgl_config c;
+  if ((rc = resolve_config(SGL_FORM_MATMUL, cfg_x, M, &c)) ||
+      (rc = resolve_config(SGL_FORM_MATMUL, cfg_w, K, &c)))
+    return rc;
+  if ((rc = sgl_swiglu_grad_preact_saved(dy, pre, scales, bits, grad_preact, nullptr, nullptr, M, N,
+                                         lddy, 2 * N, 0, stream)))
+    return rc;
+  if (grad_x && (rc = sgl_matmul_bf16_ex(grad_preact, w, grad_x, M, K, 2 * N, 2 * N, ldw, K, 0, 1,
+                                         cfg_x, stream)))
+    return rc;
+  if (grad_w)
+    return sgl_matmul_bf16_ex(x, grad_preact, grad_w, K, 2 * N, M, ldx, 2 * N, 2 * N, 1, 0, cfg_w,
+                              stream);
+  return SGL_OK;
+}
+
 // ---- the expert layer at inference, one call ----
 
 static int64_t align256(int64_t n) { return (n + 255) / 256 * 256; }

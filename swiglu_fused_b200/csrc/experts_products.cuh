@@ -412,7 +412,7 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   const int G = p.groups;
   auto row_lo = [&](int e) {
     if (p.offsets == nullptr) return e == 0 ? 0 : p.R;
-    const int lo = __ldg(p.offsets + e);
+    const int lo = p.offsets[e];   // (written by a kernel this one may have started beside: no ld.nc)
     return lo < 0 ? 0 : (lo > p.R ? p.R : lo);
   };
   if constexpr (!kWgrad) {

@@ -14,6 +14,7 @@ expert ``e`` owns ``W[e] = [W_up | W_gate]`` (``[K, 2N]``) and ``W_down[e]`` (``
 ``grouped_weight_grad``   ``a_e^T @ g_e`` for every expert
 ``experts_swiglu``        all of the forward in one call, for inference
 ``swiglu_grad_preact_saved``  the backward's elementwise step from saved pre-activations
+``fused_swiglu_backward_saved``  the dense stage's whole backward from them
 
 The conventions are those of the other operators: bf16 tensors with unit column stride and 16-byte
 rows, checks before anything is launched, torch's current stream unless ``stream=`` is given,
@@ -22,16 +23,19 @@ rows, checks before anything is launched, torch's current stream unless ``stream
 """
 from __future__ import annotations
 
+import ctypes as C
 from typing import NamedTuple
 
 import torch
 
-from . import _lib
+from . import _lib, tile_table
 from .ops import (DTYPE, _check_matrix, _ld, _prep_out, _same_device, _stream_handle,
                   stream_context)
 
 MAX_EXPERTS = 1024
 MAX_CHOICES = 64
+_ID_TYPES = (torch.int64, torch.int32)
+_WEIGHT_TYPES = (torch.float32, torch.bfloat16)
 _ONE_CTA_SLOTS = 2048      # up to here sgl_expert_order needs no scratch
 
 
@@ -211,6 +215,71 @@ def _prep_rows(out, M: int, N: int, device, dtype=DTYPE):
     return out
 
 
+# Plain operands are recognised with a few attribute reads (the calls below cost microseconds, the
+# small problems they are for not many more); anything else goes through the full checks, which say
+# what is wrong or accept it with its strides.
+
+
+def _matrix(t, name: str) -> tuple[int, int, int]:
+    """Checks a bf16 matrix (rows may be none); (rows, columns, row pitch)."""
+    if type(t) is torch.Tensor and t.dtype is DTYPE and t.is_cuda and t.dim() == 2 \
+            and t.is_contiguous():
+        rows, cols = t.shape
+        if cols and cols % 8 == 0 and t.data_ptr() % 16 == 0:
+            return rows, cols, cols
+    _check_matrix(t, name, allow_empty_rows=True)
+    return t.shape[0], t.shape[1], _ld(t)
+
+
+def _rows_matrix(t, name: str) -> tuple[int, int, int]:
+    """The same for rows that may be fp32."""
+    if type(t) is torch.Tensor and t.dtype is torch.float32:
+        _check_rows(t, name)
+        return t.shape[0], t.shape[1], _ld(t)
+    return _matrix(t, name)
+
+
+def _order_rows(order) -> tuple[int, int]:
+    """Checks an order's ``rows``; (tokens, choices)."""
+    if type(order) is ExpertOrder:
+        rows = order.rows
+        if type(rows) is torch.Tensor and rows.dtype is torch.int32 and rows.is_cuda \
+                and rows.dim() == 2 and rows.is_contiguous():
+            T, k = rows.shape
+            if 0 < k <= MAX_CHOICES:
+                return T, k
+    return _check_order_rows(order)
+
+
+def _choices(t, name: str, dtypes) -> tuple[int, int, int]:
+    """Checks a router's [T, k] tensor; (tokens, choices, row pitch)."""
+    if type(t) is torch.Tensor and t.dtype in dtypes and t.is_cuda and t.dim() == 2 \
+            and t.is_contiguous():
+        T, k = t.shape
+        if 0 < k <= MAX_CHOICES:
+            return T, k, k
+    _check_choices(t, name, dtypes)
+    return t.shape[0], t.shape[1], _choice_ld(t)
+
+
+def _weights(weights, T: int, k: int) -> int:
+    """Checks routing weights; their row pitch."""
+    T2, k2, ld = _choices(weights, "weights", _WEIGHT_TYPES)
+    if T2 != T or k2 != k:
+        raise ValueError(f"weights shape {(T2, k2)} != {(T, k)}")
+    return ld
+
+
+def _one_device(*tensors) -> torch.device:
+    """The device of all of them."""
+    first = tensors[0].get_device()
+    for t in tensors:
+        if t.get_device() != first:
+            raise ValueError("operands are on different devices: "
+                             + ", ".join(str(u.device) for u in tensors))
+    return tensors[0].device
+
+
 def _multiple_of_8(**sizes: int) -> None:
     for name, n in sizes.items():
         if n % 8:
@@ -220,8 +289,7 @@ def _multiple_of_8(**sizes: int) -> None:
 def expert_order(expert_ids, num_experts: int, *, stream=None) -> ExpertOrder:
     """Sorts the slots of ``expert_ids[T, k]`` (int32 or int64) by expert, slot order kept inside
     an expert.  Slots with an id outside ``[0, num_experts)`` are dropped."""
-    _check_choices(expert_ids, "expert_ids", (torch.int32, torch.int64))
-    T, k = expert_ids.shape
+    T, k, ld = _choices(expert_ids, "expert_ids", _ID_TYPES)
     E = int(num_experts)
     if not 1 <= E <= MAX_EXPERTS:
         raise ValueError(f"num_experts={E} outside [1, {MAX_EXPERTS}]")
@@ -240,7 +308,7 @@ def expert_order(expert_ids, num_experts: int, *, stream=None) -> ExpertOrder:
             need = lib.sgl_expert_order_scratch_bytes(T, k, E)
             scratch = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
         _lib.check(lib.sgl_expert_order(
-            expert_ids.data_ptr(), expert_ids.dtype == torch.int64, T, k, _choice_ld(expert_ids), E,
+            expert_ids.data_ptr(), expert_ids.dtype is torch.int64, T, k, ld, E,
             offsets.data_ptr(), slots.data_ptr(), rows.data_ptr(),
             scratch.data_ptr() if scratch is not None else None, need, handle))
     return ExpertOrder(offsets, slots, rows)
@@ -249,54 +317,43 @@ def expert_order(expert_ids, num_experts: int, *, stream=None) -> ExpertOrder:
 def expert_dispatch(x, order: ExpertOrder, *, out=None, stream=None):
     """``out[order.rows[t, j]] = x[t]``: ``[T, D]`` -> ``[T * k, D]``, rows grouped by expert.  Rows
     behind the last expert's (there are some if slots were dropped) are left as they were."""
-    T, k = _check_order_rows(order)
-    _check_matrix(x, "x", allow_empty_rows=True)
-    if x.shape[0] != T:
-        raise ValueError(f"x has {x.shape[0]} rows, the order {T} tokens")
-    D = x.shape[1]
+    T, k = _order_rows(order)
+    T2, D, ldx = _matrix(x, "x")
+    if T2 != T:
+        raise ValueError(f"x has {T2} rows, the order {T} tokens")
     _multiple_of_8(D=D)
-    dev = _same_device(("x", x), ("order.rows", order.rows))
+    dev = _one_device(x, order.rows)
     if T == 0:
         return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
     with _launch(stream, dev) as handle:
         o = _prep_rows(out, T * k, D, dev)
         _lib.check(_lib.load().sgl_expert_dispatch(
-            x.data_ptr(), order.rows.data_ptr(), o.data_ptr(), T, k, D, T * k, _ld(x), _ld(o),
-            handle))
+            x.data_ptr(), order.rows.data_ptr(), o.data_ptr(), T, k, D, T * k, ldx, _ld(o), handle))
     return o
-
-
-def _check_weights(weights, T: int, k: int) -> None:
-    _check_choices(weights, "weights", (torch.float32, torch.bfloat16))
-    if tuple(weights.shape) != (T, k):
-        raise ValueError(f"weights shape {tuple(weights.shape)} != {(T, k)}")
 
 
 def expert_combine(rows, order: ExpertOrder, weights=None, *, out=None, stream=None):
     """``out[t] = sum_j weights[t, j] * rows[order.rows[t, j]]``: ``[T * k, D]`` bf16 or fp32 ->
     ``[T, D]`` bf16, fp32 sums in the order of ``j``.  ``weights`` is fp32 or bf16 ``[T, k]``;
     without weights the rows are summed as they are.  Dropped slots add nothing."""
-    T, k = _check_order_rows(order)
-    _check_rows(rows, "rows")
-    if rows.shape[0] != T * k:
-        raise ValueError(f"rows has {rows.shape[0]} rows, the order {T * k} slots")
-    D = rows.shape[1]
+    T, k = _order_rows(order)
+    R, D, ld = _rows_matrix(rows, "rows")
+    if R != T * k:
+        raise ValueError(f"rows has {R} rows, the order {T * k} slots")
     _multiple_of_8(D=D)
-    named = [("rows", rows), ("order.rows", order.rows)]
     if weights is not None:
-        _check_weights(weights, T, k)
-        named.append(("weights", weights))
-    dev = _same_device(*named)
+        ldw, w_ptr, w_bf16 = _weights(weights, T, k), weights.data_ptr(), weights.dtype is DTYPE
+        dev = _one_device(rows, order.rows, weights)
+    else:
+        ldw, w_ptr, w_bf16 = 0, None, False
+        dev = _one_device(rows, order.rows)
     if T == 0:
         return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev)
     with _launch(stream, dev) as handle:
         o = _prep_rows(out, T, D, dev)
         _lib.check(_lib.load().sgl_expert_combine(
-            rows.data_ptr(), int(rows.dtype == torch.float32), order.rows.data_ptr(),
-            weights.data_ptr() if weights is not None else None,
-            int(weights is not None and weights.dtype == DTYPE), o.data_ptr(), T, k, D, T * k,
-            _ld(rows), _choice_ld(weights) if weights is not None else 0, _ld(o),
-            handle))
+            rows.data_ptr(), rows.dtype is torch.float32, order.rows.data_ptr(), w_ptr, w_bf16,
+            o.data_ptr(), T, k, D, R, ld, ldw, _ld(o), handle))
     return o
 
 
@@ -309,31 +366,34 @@ def expert_combine_grad(grad_out, rows, order: ExpertOrder, weights, *, weighted
     With ``rows=None`` only ``grad_rows`` is computed (``grad_weights`` is None).  With
     ``weighted=False`` the rows of ``grad_rows`` are ``grad_out[t]`` as it is, for a caller that
     applies the weight further on (``grouped_grad_preact`` does)."""
-    T, k = _check_order_rows(order)
-    _check_matrix(grad_out, "grad_out", allow_empty_rows=True)
-    D = grad_out.shape[1]
-    named = [("grad_out", grad_out), ("order.rows", order.rows), ("weights", weights)]
+    T, k = _order_rows(order)
+    T2, D, ldg = _matrix(grad_out, "grad_out")
+    R = T * k
+    fits = T2 == T
+    ld = D
     if rows is not None:
-        _check_rows(rows, "rows")
-        named.append(("rows", rows))
-    if grad_out.shape[0] != T or (rows is not None and tuple(rows.shape) != (T * k, D)):
+        R2, D2, ld = _rows_matrix(rows, "rows")
+        fits = fits and R2 == R and D2 == D
+    if not fits:
         raise ValueError(f"grad_out {tuple(grad_out.shape)} and rows "
                          f"{tuple(rows.shape) if rows is not None else None} do not fit {T} tokens "
                          f"of {k} choices")
     _multiple_of_8(D=D)
-    _check_weights(weights, T, k)
-    dev = _same_device(*named)
+    ldw = _weights(weights, T, k)
+    if rows is not None:
+        dev = _one_device(grad_out, order.rows, weights, rows)
+    else:
+        dev = _one_device(grad_out, order.rows, weights)
     with _launch(stream, dev) as handle:
         gw = _empty2(T, k, weights.dtype, dev) if rows is not None else None
         if T == 0:
             return out if out is not None else torch.empty((0, D), dtype=DTYPE, device=dev), gw
-        gr = _prep_rows(out, T * k, D, dev)
+        gr = _prep_rows(out, R, D, dev)
         _lib.check(_lib.load().sgl_expert_combine_grad(
             grad_out.data_ptr(), rows.data_ptr() if rows is not None else None,
-            int(rows is not None and rows.dtype == torch.float32), order.rows.data_ptr(),
-            weights.data_ptr() if weighted else None, int(weights.dtype == DTYPE), gr.data_ptr(),
-            gw.data_ptr() if gw is not None else None, T, k, D, T * k, _ld(grad_out),
-            _ld(rows) if rows is not None else D, _choice_ld(weights), _ld(gr), handle))
+            rows is not None and rows.dtype is torch.float32, order.rows.data_ptr(),
+            weights.data_ptr() if weighted else None, weights.dtype is DTYPE, gr.data_ptr(),
+            gw.data_ptr() if gw is not None else None, T, k, D, R, ldg, ld, ldw, _ld(gr), handle))
     return gr, gw
 
 
@@ -386,6 +446,8 @@ def _empty_preact(bits: int, rows: int, N: int, dev) -> SavedPreact:
 
 
 def _check_preact(p: SavedPreact) -> None:
+    if not isinstance(p, SavedPreact):
+        raise TypeError(f"preact must be a SavedPreact, got {type(p).__name__}")
     if p.bits not in (8, 16):
         raise ValueError(f"preact.bits must be 8 or 16, got {p.bits}")
     shape, scale_shape = _preact_shapes(p.bits, p.data.shape[0], p.hidden)
@@ -398,7 +460,7 @@ def _check_preact(p: SavedPreact) -> None:
             raise ValueError(f"preact.{name} must be a contiguous {dtype} CUDA tensor of shape {want}")
 
 
-def _save(x, w_ptr, offsets, E, ldw, w_stride, R, K, N, bits, out, stream, dev):
+def _save(x, w_ptr, offsets, E, ldx, ldw, w_stride, R, K, N, bits, out, stream, dev):
     with _launch(stream, dev) as handle:
         h = _prep_rows(out, R, N, dev) if R else torch.empty((0, N), dtype=DTYPE, device=dev)
         pre = _empty_preact(bits, R, N, dev)
@@ -406,7 +468,7 @@ def _save(x, w_ptr, offsets, E, ldw, w_stride, R, K, N, bits, out, stream, dev):
             _lib.check(_lib.load().sgl_grouped_fused_swiglu_save(
                 x.data_ptr(), w_ptr, offsets.data_ptr() if offsets is not None else None,
                 h.data_ptr(), pre.data.data_ptr(),
-                pre.scales.data_ptr() if pre.scales is not None else None, bits, R, N, K, E, _ld(x),
+                pre.scales.data_ptr() if pre.scales is not None else None, bits, R, N, K, E, ldx,
                 ldw, w_stride, _ld(h), handle))
     return h, pre
 
@@ -416,8 +478,8 @@ def grouped_fused_swiglu_save(x, W, offsets, *, checkpoint: str = "bf16", out=No
     the pre-activations in 8 bits (a power-of-two scale per row and 32 columns), ``"bf16"`` in 16."""
     bits = _checkpoint_bits(checkpoint)
     R, K, N, E, dev = _swiglu_operands(x, W, offsets)
-    return _save(x, W.data_ptr(), offsets, E, _expert_ld(W), W.stride(0), R, K, N, bits, out, stream,
-                 dev)
+    return _save(x, W.data_ptr(), offsets, E, _ld(x), _expert_ld(W), W.stride(0), R, K, N, bits, out,
+                 stream, dev)
 
 
 def matmul_fused_swiglu_save_preact(A, W, *, checkpoint: str = "e4m3", out=None, stream=None):
@@ -426,17 +488,50 @@ def matmul_fused_swiglu_save_preact(A, W, *, checkpoint: str = "e4m3", out=None,
     A : [M, K] bf16, W : [K, 2N] bf16 = [W_up | W_gate].  The checkpoint takes ``2N + N/16`` bytes
     per row (``"bf16"``: ``4N``); ``matmul_fused_swiglu_save_factors`` keeps two bf16 factors."""
     bits = _checkpoint_bits(checkpoint)
-    _check_matrix(A, "A", allow_empty_rows=True)
-    _check_matrix(W, "W")
-    M, K = A.shape
-    K2, N2 = W.shape
-    if K != K2:
+    M, K, ldx, N, ldw, dev = _stage_operands(A, W)
+    return _save(A, W.data_ptr(), None, 1, ldx, ldw, 0, M, K, N, bits, out, stream, dev)
+
+
+def _stage_operands(A, W):
+    """Checks and sizes of the dense stage: (M, K, pitch of A, N, pitch of W, device)."""
+    M, K, ldx = _matrix(A, "A")
+    K2, N2, ldw = _matrix(W, "W")
+    if K != K2 or K == 0:
         raise ValueError(f"K mismatch: A.K={K} vs W.K={K2}")
     if N2 % 2:
         raise ValueError(f"W's 2nd dim ({N2}) must be even")
     _multiple_of_8(K=K, N=N2 // 2)
-    dev = _same_device(("A", A), ("W", W))
-    return _save(A, W.data_ptr(), None, 1, _ld(W), 0, M, K, N2 // 2, bits, out, stream, dev)
+    return M, K, ldx, N2 // 2, ldw, _one_device(A, W)
+
+
+def fused_swiglu_backward_saved(x, W, dy, preact: SavedPreact, *, need_x: bool = True,
+                                need_w: bool = True, stream=None):
+    """The dense stage's backward from saved pre-activations, one library call: ``(grad_x [M, K],
+    grad_w [K, 2N])`` for ``h = matmul_fused_swiglu(x, W)`` and its gradient ``dy [M, N]``; None for
+    the one that is not needed.  The two products are ``matmul_bf16``'s, tile table included."""
+    M, K, ldx, N, ldw, dev = _stage_operands(x, W)
+    M2, N2, lddy = _matrix(dy, "dy")
+    _check_preact(preact)
+    if M2 != M or N2 != N or preact.hidden != N or preact.data.shape[0] != M:
+        raise ValueError(f"dy shape {tuple(dy.shape)} or the saved pre-activations of "
+                         f"{preact.data.shape[0]} rows and {preact.hidden} columns do not fit x "
+                         f"{tuple(x.shape)} and W {tuple(W.shape)}")
+    _one_device(x, dy, preact.data, *(() if preact.scales is None else (preact.scales,)))
+    with _launch(stream, dev) as handle:
+        gx = _empty2(M, K, DTYPE, dev) if need_x else None
+        gw = _empty2(K, 2 * N, DTYPE, dev) if need_w else None
+        if M == 0:
+            return gx, gw.zero_() if need_w else None
+        gp = _empty2(M, 2 * N, DTYPE, dev)
+        cfg_x = tile_table.lookup(_lib.FORM_MATMUL, M, K, 2 * N)
+        cfg_w = tile_table.lookup(_lib.FORM_MATMUL, K, 2 * N, M)
+        _lib.check(_lib.load().sgl_fused_swiglu_backward_saved(
+            x.data_ptr(), W.data_ptr(), dy.data_ptr(), preact.data.data_ptr(),
+            preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
+            gp.data_ptr(), gx.data_ptr() if need_x else None, gw.data_ptr() if need_w else None,
+            M, N, K, ldx, ldw, lddy, C.byref(cfg_x.to_c()) if cfg_x is not None else None,
+            C.byref(cfg_w.to_c()) if cfg_w is not None else None, handle))
+    return gx, gw
 
 
 def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h: bool = False,
@@ -444,15 +539,12 @@ def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h:
     """Backward elementwise step from saved pre-activations: ``[dy * silu(gate) |
     dy * up * silu'(gate)]``, ``[R, 2N]``; with ``return_h`` also ``h = silu(gate) * up``.  With
     ``offsets`` (of the experts' row groups) rows behind ``offsets[-1]`` are left as they were."""
-    if not isinstance(preact, SavedPreact):
-        raise TypeError(f"preact must be a SavedPreact, got {type(preact).__name__}")
-    _check_matrix(dy, "dy", allow_empty_rows=True)
-    R, N = dy.shape
+    _check_preact(preact)
+    R, N, lddy = _matrix(dy, "dy")
     _multiple_of_8(N=N)
     if preact.hidden != N or preact.data.shape[0] != R:
         raise ValueError(f"dy shape {tuple(dy.shape)} does not fit the saved pre-activations of "
                          f"{preact.data.shape[0]} rows and {preact.hidden} columns")
-    _check_preact(preact)
     named = [("dy", dy), ("preact.data", preact.data)]
     if preact.scales is not None:
         named.append(("preact.scales", preact.scales))
@@ -472,7 +564,7 @@ def swiglu_grad_preact_saved(dy, preact: SavedPreact, *, offsets=None, return_h:
         _lib.check(_lib.load().sgl_swiglu_grad_preact_saved(
             dy.data_ptr(), preact.data.data_ptr(),
             preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
-            g.data_ptr(), h.data_ptr() if h is not None else None, end, R, N, _ld(dy), _ld(g),
+            g.data_ptr(), h.data_ptr() if h is not None else None, end, R, N, lddy, _ld(g),
             _ld(h) if h is not None else 0, handle))
     return (g, h) if return_h else g
 
@@ -519,11 +611,9 @@ def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrd
     W_down    : [E, N, D] bf16
     returns   : ``(grad_preact [R, 2N], h [R, N])``; rows behind the last expert's are left as they were
     """
-    T, k = _check_order_rows(order)
+    T, k = _order_rows(order)
     _check_matrix(grad_rows, "grad_rows", allow_empty_rows=True)
     _check_experts(W_down, "W_down")
-    if not isinstance(preact, SavedPreact):
-        raise TypeError(f"preact must be a SavedPreact, got {type(preact).__name__}")
     R, D = grad_rows.shape
     E, N, D2 = W_down.shape
     if D2 != D or R != T * k:
@@ -541,8 +631,9 @@ def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrd
              ("order.slots", order.slots)]
     if preact.scales is not None:
         named.append(("preact.scales", preact.scales))
+    ldw = 0
     if weights is not None:
-        _check_weights(weights, T, k)
+        ldw = _weights(weights, T, k)
         named.append(("weights", weights))
     dev = _same_device(*named)
     with _launch(stream, dev) as handle:
@@ -557,8 +648,7 @@ def grouped_grad_preact(grad_rows, W_down, preact: SavedPreact, order: ExpertOrd
             int(weights is not None and weights.dtype == DTYPE), preact.data.data_ptr(),
             preact.scales.data_ptr() if preact.scales is not None else None, preact.bits,
             g.data_ptr(), h.data_ptr(), R, N, D, E, k, _ld(grad_rows), _expert_ld(W_down),
-            W_down.stride(0), _choice_ld(weights) if weights is not None else 0, _ld(g), _ld(h),
-            handle))
+            W_down.stride(0), ldw, _ld(g), _ld(h), handle))
     return g, h
 
 
@@ -605,13 +695,13 @@ def experts_swiglu_workspace_bytes(T: int, k: int, E: int, D: int, N: int, D_out
 
 
 def _layer_operands(x, expert_ids, weights, W, W_down):
-    _check_matrix(x, "x", allow_empty_rows=True)
-    _check_choices(expert_ids, "expert_ids", (torch.int32, torch.int64))
-    T, D = x.shape
-    if expert_ids.shape[0] != T:
-        raise ValueError(f"x has {T} rows, expert_ids {expert_ids.shape[0]}")
-    k = expert_ids.shape[1]
-    _check_weights(weights, T, k)
+    """Checks and sizes of the expert layer: (T, k, E, D, N, D_out, pitches of x, ids and weights,
+    device)."""
+    T, D, ldx = _matrix(x, "x")
+    T2, k, ld_ids = _choices(expert_ids, "expert_ids", _ID_TYPES)
+    if T2 != T:
+        raise ValueError(f"x has {T} rows, expert_ids {T2}")
+    ldw = _weights(weights, T, k)
     _check_experts(W, "W")
     _check_experts(W_down, "W_down")
     E, D2, N2 = W.shape
@@ -620,13 +710,12 @@ def _layer_operands(x, expert_ids, weights, W, W_down):
     if N2 % 2:
         raise ValueError(f"W's last dim ({N2}) must be even")
     N = N2 // 2
-    if W_down.shape[0] != E or W_down.shape[1] != N:
+    E2, N3, D_out = W_down.shape
+    if E2 != E or N3 != N:
         raise ValueError(f"W_down shape {tuple(W_down.shape)} does not follow W's {tuple(W.shape)}")
-    D_out = W_down.shape[2]
     _multiple_of_8(K=D, N=N, D=D_out)
-    dev = _same_device(("x", x), ("expert_ids", expert_ids), ("weights", weights), ("W", W),
-                       ("W_down", W_down))
-    return T, k, E, D, N, D_out, dev
+    return (T, k, E, D, N, D_out, ldx, ld_ids, ldw,
+            _one_device(x, expert_ids, weights, W, W_down))
 
 
 def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=None, stream=None):
@@ -642,7 +731,7 @@ def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=Non
                  calls that overlap on the GPU must not share one
     returns    : [T, D_out] bf16
     """
-    T, k, E, D, N, D_out, dev = _layer_operands(x, expert_ids, weights, W, W_down)
+    T, k, E, D, N, D_out, ldx, ld_ids, ldw, dev = _layer_operands(x, expert_ids, weights, W, W_down)
     if T == 0:
         return out if out is not None else torch.empty((0, D_out), dtype=DTYPE, device=dev)
     lib = _lib.load()
@@ -658,9 +747,8 @@ def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=Non
             raise ValueError(
                 "workspace must be a contiguous uint8 CUDA tensor on the operands' device")
         _lib.check(lib.sgl_experts_swiglu(
-            x.data_ptr(), expert_ids.data_ptr(), expert_ids.dtype == torch.int64,
-            weights.data_ptr(), weights.dtype == DTYPE, W.data_ptr(), W_down.data_ptr(),
-            y.data_ptr(), workspace.data_ptr(), workspace.numel(), T, k, E, D, N, D_out, _ld(x),
-            _choice_ld(expert_ids), _choice_ld(weights), _expert_ld(W), W.stride(0),
-            _expert_ld(W_down), W_down.stride(0), _ld(y), handle))
+            x.data_ptr(), expert_ids.data_ptr(), expert_ids.dtype is torch.int64,
+            weights.data_ptr(), weights.dtype is DTYPE, W.data_ptr(), W_down.data_ptr(),
+            y.data_ptr(), workspace.data_ptr(), workspace.numel(), T, k, E, D, N, D_out, ldx, ld_ids,
+            ldw, _expert_ld(W), W.stride(0), _expert_ld(W_down), W_down.stride(0), _ld(y), handle))
     return y

@@ -104,6 +104,19 @@ def test_other_refusals():
     call("sgl_grouped_weight_grad", -3, "c_stride", P, P, P, P, 8, 16, 16, 2, 16, 16, 16, 128, None)
     call("sgl_swiglu_grad_preact_saved", -3, "ldo", P, P, P, 8, P, None, None, 8, 16, 16, 16, 0, None)
     call("sgl_swiglu_grad_preact_saved", -4, "end", P, P, P, 8, P, None, P + 2, 8, 16, 16, 32, 0, None)
+    back = [P, P, P, P, P, 8, P, P, P, 8, 16, 16, 16, 32, 16, None, None, None]
+
+    def backward(code, needle, at, value):
+        call("sgl_fused_swiglu_backward_saved", code, needle, *(back[:at] + [value] + back[at + 1:]))
+
+    backward(-1, "x is NULL", 0, None)
+    backward(-1, "dy is NULL", 2, None)
+    backward(-1, "scales", 4, None)
+    backward(-10, "bits", 5, 7)
+    backward(-4, "grad_w", 8, P + 2)
+    backward(-2, "M=0", 9, 0)
+    backward(-3, "ldw", 13, 16)
+    backward(-3, "lddy", 14, 8)
     call("sgl_experts_swiglu", -10, "workspace", P, P, 1, P, 0, P, P, P, P, 64, 4, 2, 8, 16, 16, 16,
          16, 2, 2, 32, 512, 16, 256, 16, None)
     n = _lib.load().sgl_experts_swiglu_workspace_bytes(4, 2, 8, 16, 16, 16)

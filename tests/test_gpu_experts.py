@@ -616,6 +616,21 @@ def test_dense_stage_over_a_checkpoint(M, K, N, checkpoint):
         for got, want in ((gx, gp @ w.double().t()), (gw, x.double().t() @ gp)):
             # two roundings: grad_preact and the result
             assert (got.double() - want).norm() <= 2 * ref.BF16_HALF * want.norm()
+    # in its separate steps, bit for bit; one gradient alone; strided operands
+    with torch.no_grad():
+        gp16 = sg.swiglu_grad_preact_saved(dy, pre)
+        assert torch.equal(gx, sg.matmul_bf16(gp16, w, transpose_b=True))
+        assert torch.equal(gw, sg.matmul_bf16(x, gp16, transpose_a=True))
+        only, none = sg.fused_swiglu_backward_saved(x, w, dy, pre, need_w=False)
+        assert none is None and torch.equal(only, gx)
+        none, only = sg.fused_swiglu_backward_saved(x, w, dy, pre, need_x=False)
+        assert none is None and torch.equal(only, gw)
+        wide = [torch.zeros(t.shape[0], t.shape[1] + 8, dtype=BF16, device=DEV)[:, :t.shape[1]]
+                for t in (x, w, dy)]
+        for dst, src in zip(wide, (x, w, dy)):
+            dst.copy_(src)
+        again = sg.fused_swiglu_backward_saved(*wide, pre)
+        assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
     # the checkpoint survives its backward: a second one over the same graph is the same
     again = torch.autograd.grad(h, (x, w), dy)
     assert torch.equal(again[0], gx) and torch.equal(again[1], gw)
