@@ -710,6 +710,59 @@ def test_module_runs_and_trains():
     assert torch.isfinite(x.grad).all() and torch.isfinite(lin.weight.grad).all()
 
 
+def test_row_tensors_past_32_bits():
+    """More than 2^31 elements in the row tensors: rows near the end of everything."""
+    T, k, E, D, N = 140000, 2, 3, 8192, 64
+    ids = make_ids(T, k, E, 1, 0.01, torch.int32)
+    order = sg.expert_order(ids, E)
+    R, kept = T * k, int(order.offsets[-1])
+    assert R * D > 2 ** 31
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    x = torch.empty(T, D, dtype=BF16, device=DEV).normal_(generator=gen)
+    xs = sg.expert_dispatch(x, order)
+    w, wd = randn(E, D, 2 * N, seed=3, std=D ** -0.5), randn(E, N, D, seed=4, std=N ** -0.5)
+    h, pre = sg.grouped_fused_swiglu_save(xs, w, order.offsets, checkpoint="e4m3")
+    ys = sg.grouped_matmul(h, wd, order.offsets)
+    off = order.offsets.tolist()
+    for r in (0, off[1] - 1, off[2], kept - 1):
+        e = sum(r >= o for o in off[1:])
+        t = int(order.slots[r]) // k
+        assert torch.equal(xs[r], x[t])
+        want, bound, *_ = ref.swiglu(x[t:t + 1], w[e])
+        ref.assert_within(h[r:r + 1], want, ref.rounded(want, bound), f"h row {r}")
+        want, bound = ref.product(h[r:r + 1], wd[e])
+        ref.assert_within(ys[r:r + 1], want, ref.rounded(want, bound), f"row {r}")
+    rw = torch.rand(T, k, device=DEV)
+    y = sg.expert_combine(ys, order, rw)
+    gys, gw = sg.expert_combine_grad(x, ys, order, rw, out=xs)
+    for t in (0, T // 2, T - 1):
+        rows = order.rows[t].tolist()
+        want = sum((rw[t, j].double() * ys[r].double() for j, r in enumerate(rows) if r >= 0),
+                   torch.zeros(D, dtype=torch.float64, device=DEV))
+        ref.assert_within(y[t], want, ref.rounded(want, 4 * ref.ACC * want.abs().max()), f"y {t}")
+        for j, r in enumerate(rows):
+            if r >= 0:
+                want = rw[t, j].double() * x[t].double()
+                ref.assert_within(gys[r], want, ref.rounded(want, ref.ACC * want.abs()), "grad row")
+    grad = sg.grouped_weight_grad(gys, h, order.offsets)
+    s = slice(off[2], off[3])
+    want = gys[s, :8].double().t() @ h[s].double()
+    mag = gys[s, :8].double().abs().t() @ h[s].double().abs()
+    ref.assert_within(grad[2, :8], want, ref.rounded(want, (s.stop - s.start) * ref.ACC * mag), "C")
+
+
+def test_long_routing_rows_and_wide_tokens():
+    """64 choices for each token, and a layer whose experts outnumber its rows."""
+    x, ids, rw, w, wd = layer_inputs(9, 64, 1024, 72, 40, 5, drop=0.3)
+    want, bound = layer_reference(x, ids, rw, w, wd)
+    ref.assert_within(sg.experts_swiglu(x, ids, rw, w, wd), want, bound, "64 choices")
+    # the same expert several times in one token: separate slots
+    ids = torch.full((7, 3), 2, device=DEV)
+    want, bound = layer_reference(x[:7], ids, rw[:7, :3].contiguous(), w, wd)
+    got = sg.experts_swiglu(x[:7], ids, rw[:7, :3], w, wd)
+    ref.assert_within(got, want, bound, "one expert three times")
+
+
 # ---------------------------------------------------------------- streams and graphs
 
 
@@ -788,3 +841,15 @@ def test_captured_training_step():
     g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_a_device_that_is_not_the_current_one():
+    args = [t.to("cuda:1") for t in layer_inputs(40, 2, 4, 72, 40, 5)]
+    want = sg.experts_swiglu(*(t.to("cuda:0") for t in args))
+    assert torch.cuda.current_device() == 0
+    got = sg.experts_swiglu(*args)
+    assert got.device.index == 1 and torch.equal(got.cpu(), want.cpu())
+    assert torch.cuda.current_device() == 0
+    with pytest.raises(ValueError, match="different devices"):
+        sg.experts_swiglu(args[0].to("cuda:0"), *args[1:])
