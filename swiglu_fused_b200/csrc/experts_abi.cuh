@@ -253,7 +253,7 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   const int bits = s.form == sgl::EXP_SAVE8 || s.form == sgl::EXP_GRAD8 ? 8 : 16;
   const PreactLayout pl = preact_layout(bits, s.N);
   constexpr CUtensorMapDataType kBf16 = CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  constexpr CUtensorMapSwizzle kSw128 = CU_TENSOR_MAP_SWIZZLE_128B, kSw64 = CU_TENSOR_MAP_SWIZZLE_64B;
+  constexpr CUtensorMapSwizzle kSw128 = CU_TENSOR_MAP_SWIZZLE_128B;
   constexpr CUtensorMapL2promotion kNoPromo = CU_TENSOR_MAP_L2_PROMOTION_NONE;
   // pitch of `pre` and distance of its halves, bytes
   const int64_t pre_pitch = grad ? s.ld_pre * 2 : pl.pitch;
@@ -272,25 +272,22 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
         (rc = make_expert_map(&maps.b, s.b, b_cols, b_rows, s.E, s.ldb * 2, s.b_stride * 2, 64,
                               s.b_transposed ? 64 : kExpertBlockK, "b")))
       return rc;
-    // boxes of the results, as the epilogue stages them: 32 rows x 128 bytes, x 64 bytes where
-    // three results (or the 8-bit halves) share the staging
-    const bool triple = s.form == sgl::EXP_SAVE16 || grad;
+    // boxes of the results, as the epilogue stages them: 32 rows x 128 bytes (8-bit codes: x 64);
+    // the forms with three results store without maps
     const bool f32 = s.form == sgl::EXP_GEMM32;
-    const int64_t slot_bytes = f32 ? s.R * s.ld_out * 4 : 0;
-    rc = make_expert_map(&maps.out, s.out, s.N, s.R, f32 ? s.splits : 0, s.ld_out * (f32 ? 4 : 2),
-                         slot_bytes,
-                         triple || f32 ? 32 : 64, 32, "out",
-                         f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kBf16, triple ? kSw64 : kSw128,
-                         kNoPromo);
-    if (rc) return rc;
-    if (triple || s.form == sgl::EXP_SAVE8) {
+    if (!grad && s.form != sgl::EXP_SAVE16) {
+      rc = make_expert_map(&maps.out, s.out, s.N, s.R, f32 ? s.splits : 0, s.ld_out * (f32 ? 4 : 2),
+                           f32 ? s.R * s.ld_out * 4 : 0, f32 ? 32 : 64, 32, "out",
+                           f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : kBf16, kSw128, kNoPromo);
+      if (rc) return rc;
+    }
+    if (s.form == sgl::EXP_SAVE8) {
+      constexpr CUtensorMapDataType kU8 = CU_TENSOR_MAP_DATA_TYPE_UINT8;
       uint8_t* pre = static_cast<uint8_t*>(s.pre);
-      const CUtensorMapDataType type = triple ? kBf16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-      const int cols = triple ? 32 : 64;
-      if ((rc = make_expert_map(&maps.up, pre, s.N, s.R, 0, pre_pitch, 0, cols, 32, "up", type,
-                                kSw64, kNoPromo)) ||
-          (rc = make_expert_map(&maps.gate, pre + pre_gate, s.N, s.R, 0, pre_pitch, 0, cols, 32,
-                                "gate", type, kSw64, kNoPromo)))
+      if ((rc = make_expert_map(&maps.up, pre, s.N, s.R, 0, pre_pitch, 0, 64, 32, "up", kU8,
+                                CU_TENSOR_MAP_SWIZZLE_64B, kNoPromo)) ||
+          (rc = make_expert_map(&maps.gate, pre + pre_gate, s.N, s.R, 0, pre_pitch, 0, 64, 32,
+                                "gate", kU8, CU_TENSOR_MAP_SWIZZLE_64B, kNoPromo)))
         return rc;
     }
   }
@@ -354,7 +351,8 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
             "acc_cols=%d splits=%d a_rows=%d stages=%d grid=%lld smem=%d\n",
             s.name, static_cast<long long>(s.R), static_cast<long long>(s.N),
             static_cast<long long>(s.K), static_cast<long long>(s.M), static_cast<long long>(s.E),
-            cta_group, acc_cols, s.splits, a_rows, stages, static_cast<long long>(grid * cta_group), smem);
+            cta_group, acc_cols, s.splits, a_rows, stages,
+            static_cast<long long>(grid * cta_group), smem);
   if (nvtx_enabled()) nvtxRangePushA(s.name);
   cudaError_t e = cudaLaunchKernelEx(&lc, v.fn, maps, p);
   if (nvtx_enabled()) nvtxRangePop();
@@ -387,7 +385,8 @@ int launch_after(const char* what, void (*fn)(Args...), dim3 grid, dim3 block, i
 
 int validate_routing(int64_t T, int64_t k, int64_t E) {
   if (T < 1 || k < 1 || k > 64 || E < 1 || E > sgl::kOrderMaxExperts)
-    return fail(SGL_ERR_BAD_SHAPE, "T=%lld >= 1 tokens, k=%lld in [1, 64], E=%lld in [1, %d] needed",
+    return fail(SGL_ERR_BAD_SHAPE,
+                "T=%lld >= 1 tokens, k=%lld in [1, 64], E=%lld in [1, %d] needed",
                 static_cast<long long>(T), static_cast<long long>(k), static_cast<long long>(E),
                 sgl::kOrderMaxExperts);
   if (T > 0x7fffff00ll / k)
@@ -529,9 +528,10 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
   p.counts = static_cast<int*>(scratch);
   const dim3 threads(sgl::kOrderThreads);
   if (ctas == 1)
-    return launch_after("expert_order", sgl::expert_order_kernel, dim3(1), threads, smem, stream, p);
-  if ((rc = launch_after("expert_count", sgl::expert_count_kernel, dim3(ctas), threads, smem, stream,
-                         p)))
+    return launch_after("expert_order", sgl::expert_order_kernel, dim3(1), threads, smem, stream,
+                        p);
+  if ((rc = launch_after("expert_count", sgl::expert_count_kernel, dim3(ctas), threads, smem,
+                         stream, p)))
     return rc;
   return launch_after("expert_place", sgl::expert_place_kernel, dim3(ctas), threads,
                       (2 * static_cast<int>(E) + 40) * 4, stream, p);
@@ -601,7 +601,8 @@ static int combine_rows(const void* in, int in_is_f32, int splits, const void* r
   dim3 grid, block;
   row_geometry(T, p.nvec, 8, true, info, &grid, &block);
   if (splits > 1)
-    return launch_after("expert_combine", sgl::expert_combine_parts_kernel, grid, block, 0, stream, p);
+    return launch_after("expert_combine", sgl::expert_combine_parts_kernel, grid, block, 0, stream,
+                        p);
   return launch_after("expert_combine",
                       k <= 2 ? (in_is_f32 ? sgl::expert_combine_kernel<true, 2, 2>
                                           : sgl::expert_combine_kernel<false, 2, 2>)
@@ -1073,8 +1074,8 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
       (rc = grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
                            d_stride, D_out, 0, 1, l.splits, l.k_per_split, stream)))
     return rc;
-  return combine_rows(ws + l.ys, 1, l.splits, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R, D_out,
-                            ld_weights, ldy, stream);
+  return combine_rows(ws + l.ys, 1, l.splits, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R,
+                      D_out, ld_weights, ldy, stream);
 }
 
 }  // extern "C"

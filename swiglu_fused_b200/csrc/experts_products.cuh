@@ -15,8 +15,10 @@
 // With offsets == NULL there is one group of all rows (the dense stage's 8-bit checkpoints).
 //
 // Structure as the dense kernel's (swiglu_kernel.cuh): persistent CTAs (or CTA pairs on 256-row
-// tiles, tcgen05 cta_group::2), warps 0 and 6 = TMA producers (A, B), warp 1 = MMA issuer, warps
-// 2-5 = epilogue, a 256-column fp32 accumulator in two TMEM stages.  What the groups change:
+// tiles, tcgen05 cta_group::2), warps 0 and 6 = TMA producers (A, B), warp 1 = MMA issuer, a 256-column fp32 accumulator in two TMEM stages.  The epilogue has eight warps, two for each 32 rows, which
+// share a staging buffer and split its columns: a sum over a few hundred ends before four warps have
+// worked off a tile (the backward of 8000 rows, 1024 -> 512, in 8 bits: 25.9 us with four warps
+// and TMA stores of its three results, 20.5 us so).  What the groups change:
 //   * every CTA turns the offsets into a table of first tile rows once, and finds the expert
 //     of a tile by bisection in it;
 //   * an A tile whose rows run past its group takes them along in the operand (their
@@ -24,8 +26,9 @@
 //     group of one token does not fetch 128 rows; more come in one box of 128, because many
 //     small boxes hold up the one thread that issues them (16384 rows over 8 uneven experts,
 //     14336 -> 4096: 1.76 ms with boxes of 16 throughout, 1.38 ms so);
-//   * the epilogue stores 32 whole rows with TMA; a warp whose rows end inside its 32 copies
-//     the rows that exist with plain stores, so that no row of another group is touched;
+//   * the epilogue stores 32 whole rows with TMA; where a group ends inside them it copies the
+//     rows that exist with plain stores, so that no row of another group is touched (forms with
+//     three results store every row from the registers);
 //   * EXP_WGRAD sums over rows, so rows past the group must not reach the MMA: whole steps of 16
 //     are not issued, and where the group ends inside a step warp 7 waits for the operands to
 //     land, overwrites the rest of the step with zeros (TMA cannot clip at a border inside the
@@ -50,7 +53,8 @@ enum : int {
   EXP_GRAD8 = 6, EXP_WGRAD = 7, EXP_FORMS = 8
 };
 
-constexpr int kExpThreads = 256;       // two producers, MMA issuer, 4 epilogue warps, tail warp
+constexpr int kExpThreads = 384;       // two producers, MMA issuer, tail warp, 8 epilogue warps
+constexpr int kExpEpiWarps = 2 * kEpiWarps;
 constexpr int kExpMaxStages = 16;
 constexpr int kExpBarrierBytes = 8 * (3 * kExpMaxStages + 2 * kAccStages) + 32;
 constexpr int kExpMaxGroups = 1024;
@@ -67,8 +71,8 @@ struct ExpertMaps {
   CUtensorMap a;        // A operand, whole-tile box
   CUtensorMap a16;      // A operand, boxes of 16 rows (forward forms, few rows)
   CUtensorMap b;        // B operand
-  CUtensorMap out;      // h / c / C / w h
-  CUtensorMap up;       // pre-activations or their gradients: up half
+  CUtensorMap out;      // h / c / C (forms with three results store without maps)
+  CUtensorMap up;       // EXP_SAVE8: codes, up half
   CUtensorMap gate;     // the same, gate half
 };
 
@@ -108,15 +112,12 @@ template <int kForm, int kCtaGroup, int kBlockK>
 struct ExpertTraits {
   static constexpr bool kSwiglu = kForm == EXP_SWIGLU || kForm == EXP_SAVE16 || kForm == EXP_SAVE8;
   static constexpr bool kGrad = kForm == EXP_GRAD16 || kForm == EXP_GRAD8;
-  // Three bf16 results of the same shape: staged 32 columns at a time (64-byte rows), so that a
-  // ring of three 128-deep stages still fits (at 64 columns only two do: save16 took 3.8 ms
-  // instead of 2.8 at 16384 x 4096 x 14336 over 8 experts).
+  // three bf16 results of the same shape, stored without staging (see the epilogue)
   static constexpr bool kTriple = kForm == EXP_SAVE16 || kGrad;
-  // staging of one epilogue warp: two 64-column chunks (of fp32: 32 columns), or one chunk
-  // with its 8-bit pre-activations, or three of 32 columns
-  static constexpr int kStagingPerWarp =
-      kTriple ? 3 * kChunkBytes / 2 : 2 * kChunkBytes;
-  static constexpr int kStagingBytes = kEpiWarps * kStagingPerWarp;
+  // staging of 32 rows: two 64-column chunks (of fp32: 32 columns), or one chunk with its 8-bit
+  // pre-activations
+  static constexpr int kStagingPerRows = kTriple ? 0 : 2 * kChunkBytes;
+  static constexpr int kStagingBytes = kEpiWarps * kStagingPerRows;
   static constexpr int kBSlabsMax = kAccCols / kCtaGroup / 64;
   static constexpr int kBSlabBytes = kBlockK * 128;
 
@@ -247,6 +248,39 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int 
       : "memory");
 }
 
+// 32 lanes x 16 consecutive fp32 columns (see ptx::tmem_ld_32x32b_x32).
+__device__ __forceinline__ void tmem_ld_32x32b_x16(uint32_t taddr, float (&v)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]),
+        "=f"(v[7]), "=f"(v[8]), "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]),
+        "=f"(v[14]), "=f"(v[15])
+      : "r"(taddr)
+      : "memory");
+}
+
+// Barrier of the two warps that share a staging buffer; true if the predicate holds in all their
+// threads.  Both always come here together, whatever their own waits said, so that neither is
+// left behind.
+__device__ __forceinline__ bool pair_barrier_all(int id, bool pred) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t"
+      ".reg .pred p, r;\n\t"
+      "setp.ne.u32 p, %1, 0;\n\t"
+      "barrier.cta.red.and.pred r, %2, 64, p;\n\t"
+      "selp.u32 %0, 1, 0, r;\n\t"
+      "}"
+      : "=r"(all)
+      : "r"(static_cast<uint32_t>(pred)), "r"(id)
+      : "memory");
+  return all != 0;
+}
+__device__ __forceinline__ void pair_barrier(int id) {
+  asm volatile("barrier.cta.sync %0, 64;" ::"r"(id) : "memory");
+}
+
 __device__ __forceinline__ uint4 ld_shared_v4(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];"
@@ -261,14 +295,31 @@ __device__ __forceinline__ void st_shared_v4(uint32_t addr, uint32_t a, uint32_t
                : "memory");
 }
 
+// 16 bf16 to 16 columns of one row: 32 bytes in one store where they are aligned (`wide`), else in
+// two; `cols` (a multiple of 8) of them exist.
+__device__ __forceinline__ void store_row16(__nv_bfloat16* at, const float (&v)[16], int cols,
+                                            bool wide) {
+  uint32_t w[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  if (wide && cols >= 16) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(at), "r"(w[0]), "r"(w[1]),
+                 "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+  } else {
+    if (cols >= 8) ptx::st_global_v4(at, w[0], w[1], w[2], w[3]);
+    if (cols >= 16) ptx::st_global_v4(at + 8, w[4], w[5], w[6], w[7]);
+  }
+}
+
 // Copies the first `rows` of 32 staged rows (row_bytes = 128 or 64 each, in the swizzle of a TMA
-// box of that width) to global memory, `cols16` pieces of 16 bytes per row at most (the last may
-// be cut: `bytes` valid bytes per row, a multiple of 8).  One warp.
+// box of that width) to global memory: `bytes` of each row, a multiple of 8.  The two warps of a
+// pair together (lane 0 .. 63).
 template <int kRowBytes>
 __device__ __forceinline__ void copy_rows(uint32_t buf, uint8_t* dst, int64_t ld, int rows,
                                           int bytes, int lane) {
   constexpr int kPieces = kRowBytes / 16;
-  for (int i = lane; i < rows * kPieces; i += 32) {
+  for (int i = lane; i < rows * kPieces; i += 64) {
     const int r = i / kPieces, piece = i % kPieces;
     if (piece * 16 >= bytes) continue;
     const int sw = kRowBytes == 128 ? (r & 7) : ((r >> 1) & 3);
@@ -289,16 +340,15 @@ __device__ __forceinline__ float2 e4m3x2_to_f32(uint32_t two) {
   return __half22float2(*reinterpret_cast<__half2*>(&h2));
 }
 
-// 32 saved up and gate values of one row, columns x .. x + 31 (a block; the halves are padded to
-// whole blocks, so the last one may be read past N), kept as loaded until they are used.
+// 16 saved up and gate values of one row, columns x .. x + 15 (half a block; the halves of a row are
+// padded to whole blocks, so the last one may be read past N), kept as loaded until they are used.
 template <int kBits>
-struct SavedBlock {
-  static constexpr int kLoads = 32 * kBits / 8 / 16;
-  uint4 u[kLoads], g[kLoads];
-  int su, sg;
-  // Rows that do not exist are not read.
-  __device__ __forceinline__ void load(const ExpertParams& p, int64_t row, int x, bool live) {
-    if (!live) return;
+struct SavedHalfBlock {
+  static constexpr int kLoads = 16 * kBits / 8 / 16;
+  uint4 u[kLoads] = {}, g[kLoads] = {};
+  int su = 0, sg = 0;
+  __device__ __forceinline__ void load(const ExpertParams& p, int64_t row, int x, bool exists) {
+    if (!exists) return;
     const uint8_t* at = p.saved + row * p.ld_saved + x * (kBits / 8);
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -311,7 +361,7 @@ struct SavedBlock {
       sg = sc[p.gate_scale_off];
     }
   }
-  __device__ __forceinline__ void get(float (&up)[32], float (&gate)[32]) const {
+  __device__ __forceinline__ void get(float (&up)[16], float (&gate)[16]) const {
     const float fu = kBits == 8 ? block_scale(su) : 1.f, fg = kBits == 8 ? block_scale(sg) : 1.f;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i) {
@@ -320,7 +370,7 @@ struct SavedBlock {
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if constexpr (kBits == 8) {
-          const int o = i * 16 + j * 4;
+          const int o = j * 4;
           const float2 u0 = e4m3x2_to_f32(wu[j]), u1 = e4m3x2_to_f32(wu[j] >> 16);
           const float2 g0 = e4m3x2_to_f32(wg[j]), g1 = e4m3x2_to_f32(wg[j] >> 16);
           up[o] = u0.x * fu;
@@ -395,12 +445,12 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     }
     for (int s = 0; s < kAccStages; ++s) {
       ptx::mbar_init(bar_tfull + 8 * s, 1);
-      ptx::mbar_init(bar_tempty + 8 * s, kEpiWarps * kCtaGroup);
+      ptx::mbar_init(bar_tempty + 8 * s, kExpEpiWarps * kCtaGroup);
     }
     ptx::fence_mbar_init();
     ptx::prefetch_tensormap(&maps.a);
     ptx::prefetch_tensormap(&maps.b);
-    ptx::prefetch_tensormap(&maps.out);
+    if (!T::kTriple) ptx::prefetch_tensormap(&maps.out);
   }
   if (warp == 1) ptx::tmem_alloc<kCtaGroup>(tmem_slot, kTmemCols);
 
@@ -766,11 +816,17 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     }
   } else {
     // =========================== epilogue ===========================
-    const int q = warp & 3;
-    const uint32_t buf0 = sOut + q * T::kStagingPerWarp;
+    const int q = warp & 3;                 // TMEM lane quarter: 32 rows, shared by two warps ...
+    const int g = warp >= 8 ? 1 : 0;        // ... that own the first and the second half of the
+    const bool issuer = g == 0 && lane == 0;   // columns of every staged chunk
+    const int pair = 1 + q;                 // their named barrier
+    const int pair_lane = g * 32 + lane;
+    const uint32_t buf0 = sOut + q * T::kStagingPerRows;
     const uint32_t tempty = (kCtaGroup == 2) ? ptx::mapa(bar_tempty, 0) : bar_tempty;
     const uint32_t row_sw = static_cast<uint32_t>(lane & 7);
     const uint32_t row_off = static_cast<uint32_t>(lane) * 128u;
+    const uint32_t off64 = static_cast<uint32_t>(lane) * 64u;          // 64-byte rows
+    const uint32_t sw64 = (static_cast<uint32_t>(lane) >> 1) & 3u;
     const uint64_t pol_out = ptx::make_l2_policy((p.l2_hints >> 4) & 3);
     const int gate_col = p.acc_cols / 2;
     int stores = 0;       // staging buffers filled so far
@@ -779,18 +835,43 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
       const Unit un = unit_of(u);
       const int as = i % kAccStages;
       const uint32_t aph = (i / kAccStages) & 1u;
+      // these 32 rows of the tile, and how many of them exist
+      const int in_tile = static_cast<int>(rank) * kBlockM + q * 32;
+      int valid = (kWgrad ? p.M - un.m : un.rows) - in_tile;
+      valid = valid < 0 ? 0 : (valid > 32 ? 32 : valid);
+      const int64_t grow = un.row + in_tile;       // forward forms: first row in the row tensors
+      const bool live = lane < valid;
+      // EXP_GRAD*: the first saved values and the routing weight come in while the product is
+      // still being made, later ones two chunks before they are used (18000 rows of 128 experts,
+      // 768 -> 256: 31.1 us one chunk ahead, 28.8 two, 29.5 three)
+      constexpr int kAhead = T::kGrad ? 2 : 1;
+      SavedHalfBlock<kForm == EXP_GRAD8 ? 8 : 16> saved[kAhead];
+      float weight = 1.0f;
+      if constexpr (T::kGrad) {
+#pragma unroll
+        for (int j = 0; j < kAhead; ++j) {
+          const int x = un.n + j * 32 + g * 16;
+          saved[j].load(p, grow + lane, x, live && j * 32 < tile_cols && un.n + j * 32 < p.N);
+        }
+        if (p.slots != nullptr && live) {
+          const int64_t slot = p.slots[grow + lane];
+          weight = 0.f;
+          if (slot >= 0 && slot < p.num_slots) {
+            const int64_t at = slot / p.k * p.ld_w + slot % p.k;
+            weight = p.w_bf16
+                         ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.weights)[at])
+                         : reinterpret_cast<const float*>(p.weights)[at];
+          }
+        }
+      }
       const bool w = ptx::mbar_wait(bar_tfull + 8 * as, aph, limit, abort_flag);
-      if (!__all_sync(0xffffffffu, w)) {
+      __syncwarp();
+      if (!pair_barrier_all(pair, w)) {
         if (lane == 0) report_error(kErrExpEpilogueWait, i, abort_flag);
         break;
       }
       ptx::tc_fence_after_sync();
       const uint32_t t_row = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + as * kAccCols;
-      // this warp's 32 rows of the tile, and how many of them exist
-      const int in_tile = static_cast<int>(rank) * kBlockM + q * 32;
-      int valid = (kWgrad ? p.M - un.m : un.rows) - in_tile;
-      valid = valid < 0 ? 0 : (valid > 32 ? 32 : valid);
-      const bool empty_sum = kWgrad && un.rows == 0;
       auto hand_back = [&]() {
         ptx::tc_fence_before_sync();
         __syncwarp();
@@ -800,51 +881,62 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         hand_back();
         continue;
       }
-      const int64_t grow = un.row + in_tile;       // forward forms: first row in the row tensors
+      // Before a staging buffer is written the store that used it has to have read it (kPending
+      // younger ones may still be under way), and rows copied out by hand have to be out.
+      auto buffer_free = [&](auto pending) {
+        if (issuer) ptx::bulk_wait_group_read<decltype(pending)::value>();
+        __syncwarp();
+        pair_barrier(pair);
+      };
+      // Both warps' halves are in place (and, for TMA, visible to the asynchronous proxy).
+      auto buffer_full = [&]() {
+        ptx::fence_proxy_async_smem();
+        __syncwarp();
+        pair_barrier(pair);
+      };
       if constexpr (T::kTriple) {
-        // ---- three bf16 results, 32 columns at a time ----
-        constexpr uint32_t kSB = kChunkBytes / 2;
-        const uint32_t off_row = static_cast<uint32_t>(lane) * 64u;
-        const uint32_t sw64 = (static_cast<uint32_t>(lane) >> 1) & 3u;
+        // ---- three bf16 results, 32 columns at a time, 16 for each warp, straight from the
+        // registers: a thread's 32 bytes of a row are a whole sector ----
+        __nv_bfloat16* const row_h = p.out + (grow + lane) * p.ld_out;
+        __nv_bfloat16* const row_up =
+            reinterpret_cast<__nv_bfloat16*>(p.pre + (grow + lane) * p.ld_pre);
+        __nv_bfloat16* const row_gate = reinterpret_cast<__nv_bfloat16*>(
+            reinterpret_cast<uint8_t*>(row_up) + p.gate_off);
+        const bool wide_h = (reinterpret_cast<uintptr_t>(row_h) & 31) == 0;
+        const bool wide_pre = ((reinterpret_cast<uintptr_t>(row_up) |
+                                reinterpret_cast<uintptr_t>(row_gate)) & 31) == 0;
         const int units = tile_cols / 32;
-        const bool live = lane < valid;
-        float weight = 1.0f;
-        // the saved values of a unit are fetched while the one before is worked on
-        SavedBlock<kForm == EXP_GRAD8 ? 8 : 16> saved{};
-        if constexpr (T::kGrad) {
-          saved.load(p, grow + lane, un.n, live);
-          if (p.slots != nullptr && live) {
-            const int64_t slot = p.slots[grow + lane];
-            weight = 0.f;
-            if (slot >= 0 && slot < p.num_slots) {
-              const int64_t at = slot / p.k * p.ld_w + slot % p.k;
-              weight = p.w_bf16
-                           ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p.weights)[at])
-                           : reinterpret_cast<const float*>(p.weights)[at];
+        for (int c0 = 0; c0 < units; c0 += kAhead) {
+#pragma unroll
+          for (int j0 = 0; j0 < kAhead; ++j0) {
+            const int c = c0 + j0;
+            if (c >= units) break;
+            __syncwarp();             // the TMEM reads below are the whole warp's
+            const int x = un.n + c * 32;
+            const bool last = c == units - 1;
+            if (x >= p.N) {
+              if (last) hand_back();
+              continue;
             }
-          }
-        }
-        for (int c = 0; c < units; ++c) {
-          const int x = un.n + c * 32;
-          const bool last = c == units - 1;
-          if (x < p.N) {
-            float a[32], b[32], h[32];
+            const int col = c * 32 + g * 16;
+            float a[16], b[16], h[16];
             if constexpr (kForm == EXP_SAVE16) {
-              ptx::tmem_ld_32x32b_x32(t_row + c * 32, a);
-              ptx::tmem_ld_32x32b_x32(t_row + gate_col + c * 32, b);
+              tmem_ld_32x32b_x16(t_row + col, a);
+              tmem_ld_32x32b_x16(t_row + gate_col + col, b);
               ptx::tmem_ld_wait();
               if (last) hand_back();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) h[j] = silu_mul(b[j], a[j]);
+              for (int j = 0; j < 16; ++j) h[j] = silu_mul(b[j], a[j]);
             } else {
-              // this row's 32 saved up and gate values, then the gradients in their place
-              saved.get(a, b);
-              if (!last && x + 32 < p.N) saved.load(p, grow + lane, x + 32, live);
-              ptx::tmem_ld_32x32b_x32(t_row + c * 32, h);
+              // this row's saved up and gate values, then the gradients in their place
+              saved[j0].get(a, b);
+              saved[j0].load(p, grow + lane, x + kAhead * 32 + g * 16,
+                             live && c + kAhead < units && x + kAhead * 32 < p.N);
+              tmem_ld_32x32b_x16(t_row + col, h);
               ptx::tmem_ld_wait();
               if (last) hand_back();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
+              for (int j = 0; j < 16; ++j) {
                 float hv, sv, dv;
                 silu_factors(b[j], a[j], hv, sv, dv);
                 const float t = weight * h[j];
@@ -853,180 +945,131 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                 h[j] = weight * hv;
               }
             }
-            if (lane == 0) ptx::bulk_wait_group_read<0>();
-            __syncwarp();
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t off = buf0 + off_row + ((static_cast<uint32_t>(j) ^ sw64) << 4);
-              st_shared_v4(off, pack_bf16x2(h[8 * j], h[8 * j + 1]),
-                           pack_bf16x2(h[8 * j + 2], h[8 * j + 3]),
-                           pack_bf16x2(h[8 * j + 4], h[8 * j + 5]),
-                           pack_bf16x2(h[8 * j + 6], h[8 * j + 7]));
-              st_shared_v4(off + kSB, pack_bf16x2(a[8 * j], a[8 * j + 1]),
-                           pack_bf16x2(a[8 * j + 2], a[8 * j + 3]),
-                           pack_bf16x2(a[8 * j + 4], a[8 * j + 5]),
-                           pack_bf16x2(a[8 * j + 6], a[8 * j + 7]));
-              st_shared_v4(off + 2 * kSB, pack_bf16x2(b[8 * j], b[8 * j + 1]),
-                           pack_bf16x2(b[8 * j + 2], b[8 * j + 3]),
-                           pack_bf16x2(b[8 * j + 4], b[8 * j + 5]),
-                           pack_bf16x2(b[8 * j + 6], b[8 * j + 7]));
+            if (live) {
+              const int xc = x + g * 16;
+              store_row16(row_h + xc, h, p.N - xc, wide_h);
+              store_row16(row_up + xc, a, p.N - xc, wide_pre);
+              store_row16(row_gate + xc, b, p.N - xc, wide_pre);
             }
-            if (valid == 32) {
-              ptx::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0) {
-                const int y = static_cast<int>(grow);
-                ptx::tma_store_2d(&maps.out, x, y, buf0, pol_out);
-                ptx::tma_store_2d(&maps.up, x, y, buf0 + kSB, pol_out);
-                ptx::tma_store_2d(&maps.gate, x, y, buf0 + 2 * kSB, pol_out);
-                ptx::bulk_commit_group();
-              }
-            } else {
-              // the group ends inside this warp's rows: store the rows it has, and no other
-              __syncwarp();
-              const int bytes = (p.N - x < 32 ? p.N - x : 32) * 2;
-              copy_rows<64>(buf0, reinterpret_cast<uint8_t*>(p.out + grow * p.ld_out + x),
-                            p.ld_out * 2, valid, bytes, lane);
-              uint8_t* at = p.pre + grow * p.ld_pre + x * 2;
-              copy_rows<64>(buf0 + kSB, at, p.ld_pre, valid, bytes, lane);
-              copy_rows<64>(buf0 + 2 * kSB, at + p.gate_off, p.ld_pre, valid, bytes, lane);
-              __syncwarp();
-            }
-          } else if (last) {
-            hand_back();
           }
         }
       } else if constexpr (kForm == EXP_GEMM32) {
-        // ---- fp32 result, 32 columns at a time, two buffers ----
+        // ---- fp32 result, 32 columns at a time (16 for each warp), two buffers ----
         const int units = tile_cols / 32;
         const int slot = splits > 1 ? un.k0 / p.k_per_split : 0;
         for (int c = 0; c < units; ++c) {
           const int x = un.n + c * 32;
           const bool last = c == units - 1;
-          if (x < p.N) {
-            const uint32_t buf = buf0 + (stores & 1) * kChunkBytes;
-            ++stores;
-            if (lane == 0) ptx::bulk_wait_group_read<1>();
-            __syncwarp();
-            float v[32];
-            ptx::tmem_ld_32x32b_x32(t_row + c * 32, v);
-            ptx::tmem_ld_wait();
+          if (x >= p.N) {
             if (last) hand_back();
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              st_shared_v4(buf + row_off + ((static_cast<uint32_t>(j) ^ row_sw) << 4),
-                           __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
-                           __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
-            if (valid == 32) {
-              ptx::fence_proxy_async_smem();
-              __syncwarp();
-              if (lane == 0)
-                tma_store_3d(&maps.out, x, static_cast<int>(grow), slot, buf, pol_out);
-            } else {
-              __syncwarp();
-              copy_rows<128>(buf,
-                             reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) +
-                                                        slot * p.slot_stride + grow * p.ld_out + x),
-                             p.ld_out * 4, valid, (p.N - x < 32 ? p.N - x : 32) * 4, lane);
-              __syncwarp();
-            }
-            if (lane == 0) ptx::bulk_commit_group();   // keeps the buffers' turn-taking in step
-          } else if (last) {
-            hand_back();
+            continue;
           }
+          const uint32_t buf = buf0 + (stores & 1) * kChunkBytes;
+          ++stores;
+          float v[16];
+          tmem_ld_32x32b_x16(t_row + c * 32 + g * 16, v);
+          ptx::tmem_ld_wait();
+          if (last) hand_back();
+          buffer_free(std::integral_constant<int, 1>{});
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            st_shared_v4(buf + row_off + ((static_cast<uint32_t>(g * 4 + j) ^ row_sw) << 4),
+                         __float_as_uint(v[4 * j]), __float_as_uint(v[4 * j + 1]),
+                         __float_as_uint(v[4 * j + 2]), __float_as_uint(v[4 * j + 3]));
+          buffer_full();
+          if (valid == 32) {
+            if (issuer) tma_store_3d(&maps.out, x, static_cast<int>(grow), slot, buf, pol_out);
+          } else {
+            copy_rows<128>(buf,
+                           reinterpret_cast<uint8_t*>(reinterpret_cast<float*>(p.out) +
+                                                      slot * p.slot_stride + grow * p.ld_out + x),
+                           p.ld_out * 4, valid, (p.N - x < 32 ? p.N - x : 32) * 4, pair_lane);
+          }
+          if (issuer) ptx::bulk_commit_group();   // keeps the buffers' turn-taking in step
         }
       } else {
-      // ---- one bf16 result, 64 columns at a time (EXP_SAVE8: with its 8-bit pre-activations) ----
-      const int chunks = tile_cols / 64;
+        // ---- one bf16 result, 64 columns at a time, 32 for each warp (EXP_SAVE8: with its 8-bit
+        // pre-activations, of which a warp's 32 columns are one block) ----
+        const int chunks = tile_cols / 64;
 #pragma unroll 1
-      for (int c = 0; c < chunks; ++c) {
-        const int x = un.n + c * 64;
-        const bool last = c == chunks - 1;
-        // the staging buffer(s) of this chunk
-        uint32_t buf = buf0;
-        if constexpr (kForm == EXP_SAVE8) {
-          if (lane == 0) ptx::bulk_wait_group_read<0>();
-        } else {
-          if (lane == 0) ptx::bulk_wait_group_read<1>();
-          buf = buf0 + (stores & 1) * kChunkBytes;
-        }
-        ++stores;
-        __syncwarp();
-        uint32_t up_scales = 0, gate_scales = 0;
-        if (x < p.N) {
+        for (int c = 0; c < chunks; ++c) {
+          const int x = un.n + c * 64;
+          const bool last = c == chunks - 1;
+          if (x >= p.N) {
+            if (last) hand_back();
+            continue;
+          }
+          uint32_t buf = buf0;
+          if constexpr (kForm != EXP_SAVE8) buf = buf0 + (stores & 1) * kChunkBytes;
+          ++stores;
+          const int col = c * 64 + g * 32;
+          float v0[32];
+          ptx::tmem_ld_32x32b_x32(t_row + col, v0);
+          uint32_t up_codes[8], gate_codes[8];
+          int up_scale = 0, gate_scale = 0;
+          if constexpr (kSwiglu) {
+            float gate[32];
+            ptx::tmem_ld_32x32b_x32(t_row + gate_col + col, gate);
+            ptx::tmem_ld_wait();
+            if (last) hand_back();
+            if constexpr (kForm == EXP_SAVE8) {
+              // columns at and past N hold sums over nothing (the operand reads as zero there,
+              // or as the gate half's weights): they do not belong to the block
+              const int n_left = p.N - (x + g * 32);
+              if (n_left < 32) {
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const int col = c * 64 + half * 32;
-            float v0[32];
-            ptx::tmem_ld_32x32b_x32(t_row + col, v0);
-            if constexpr (kSwiglu) {
-              float gate[32];
-              ptx::tmem_ld_32x32b_x32(t_row + gate_col + col, gate);
-              ptx::tmem_ld_wait();
-              if constexpr (kForm == EXP_SAVE8) {
-                // columns at and past N hold sums over nothing (the operand reads as zero
-                // there, or as the gate half's weights): they do not belong to a block
-                const int n_left = p.N - (x + half * 32);
-                if (n_left < 32) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) {
-                    v0[j] = j < n_left ? v0[j] : 0.f;
-                    gate[j] = j < n_left ? gate[j] : 0.f;
-                  }
-                }
-                const uint32_t off64 = static_cast<uint32_t>(lane) * 64u;
-                const uint32_t sw64 = (static_cast<uint32_t>(lane) >> 1) & 3u;
-                uint32_t codes[8];
-                up_scales |= static_cast<uint32_t>(round_block_e4m3(v0, codes)) << (8 * half);
-                st_shared_v4(buf + kChunkBytes + off64 + (((half * 2) ^ sw64) << 4), codes[0],
-                             codes[1], codes[2], codes[3]);
-                st_shared_v4(buf + kChunkBytes + off64 + (((half * 2 + 1) ^ sw64) << 4), codes[4],
-                             codes[5], codes[6], codes[7]);
-                gate_scales |= static_cast<uint32_t>(round_block_e4m3(gate, codes)) << (8 * half);
-                const uint32_t gbuf = buf + kChunkBytes + kChunkBytes / 2;
-                st_shared_v4(gbuf + off64 + (((half * 2) ^ sw64) << 4), codes[0], codes[1],
-                             codes[2], codes[3]);
-                st_shared_v4(gbuf + off64 + (((half * 2 + 1) ^ sw64) << 4), codes[4], codes[5],
-                             codes[6], codes[7]);
-              }
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v0[j] = silu_mul(gate[j], v0[j]);
-            } else {
-              ptx::tmem_ld_wait();
-              if constexpr (kWgrad) {
-                if (empty_sum) {
-#pragma unroll
-                  for (int j = 0; j < 32; ++j) v0[j] = 0.f;
+                for (int j = 0; j < 32; ++j) {
+                  v0[j] = j < n_left ? v0[j] : 0.f;
+                  gate[j] = j < n_left ? gate[j] : 0.f;
                 }
               }
+              up_scale = round_block_e4m3(v0, up_codes);
+              gate_scale = round_block_e4m3(gate, gate_codes);
             }
-            if (last && half == 1) hand_back();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              st_shared_v4(buf + row_off + ((static_cast<uint32_t>(half * 4 + j) ^ row_sw) << 4),
-                           pack_bf16x2(v0[8 * j], v0[8 * j + 1]),
-                           pack_bf16x2(v0[8 * j + 2], v0[8 * j + 3]),
-                           pack_bf16x2(v0[8 * j + 4], v0[8 * j + 5]),
-                           pack_bf16x2(v0[8 * j + 6], v0[8 * j + 7]));
+            for (int j = 0; j < 32; ++j) v0[j] = silu_mul(gate[j], v0[j]);
+          } else {
+            ptx::tmem_ld_wait();
+            if (last) hand_back();
+            if constexpr (kWgrad) {
+              if (un.rows == 0) {       // a sum over nothing: the accumulator was not written
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v0[j] = 0.f;
+              }
             }
           }
-        } else if (last) {
-          hand_back();
-        }
-        if constexpr (kForm == EXP_SAVE8) {
-          if (x < p.N && lane < valid) {
-            // two scale bytes of this row for each half (the pitch has room for a whole chunk)
-            uint8_t* at = p.scales + (grow + lane) * p.ld_scales + (x >> 5);
-            *reinterpret_cast<uint16_t*>(at) = static_cast<uint16_t>(up_scales);
-            *reinterpret_cast<uint16_t*>(at + p.gate_scale_off) =
-                static_cast<uint16_t>(gate_scales);
+          if constexpr (kForm == EXP_SAVE8) {
+            buffer_free(std::integral_constant<int, 0>{});
+          } else {
+            buffer_free(std::integral_constant<int, 1>{});
           }
-        }
-        if (kWgrad || valid == 32) {
-          ptx::fence_proxy_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            if (x < p.N) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            st_shared_v4(buf + row_off + ((static_cast<uint32_t>(g * 4 + j) ^ row_sw) << 4),
+                         pack_bf16x2(v0[8 * j], v0[8 * j + 1]),
+                         pack_bf16x2(v0[8 * j + 2], v0[8 * j + 3]),
+                         pack_bf16x2(v0[8 * j + 4], v0[8 * j + 5]),
+                         pack_bf16x2(v0[8 * j + 6], v0[8 * j + 7]));
+          if constexpr (kForm == EXP_SAVE8) {
+            const uint32_t ubuf = buf + kChunkBytes, gbuf = ubuf + kChunkBytes / 2;
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const uint32_t off = off64 + ((static_cast<uint32_t>(g * 2 + j) ^ sw64) << 4);
+              st_shared_v4(ubuf + off, up_codes[4 * j], up_codes[4 * j + 1], up_codes[4 * j + 2],
+                           up_codes[4 * j + 3]);
+              st_shared_v4(gbuf + off, gate_codes[4 * j], gate_codes[4 * j + 1],
+                           gate_codes[4 * j + 2], gate_codes[4 * j + 3]);
+            }
+            if (lane < valid) {
+              // this row's scale of the block (the pitch has room for a whole chunk)
+              uint8_t* at = p.scales + (grow + lane) * p.ld_scales + (x >> 5) + g;
+              at[0] = static_cast<uint8_t>(up_scale);
+              at[p.gate_scale_off] = static_cast<uint8_t>(gate_scale);
+            }
+          }
+          buffer_full();
+          if (kWgrad || valid == 32) {
+            if (issuer) {
               if constexpr (kWgrad) {
                 tma_store_3d(&maps.out, x, un.m + in_tile, un.e, buf, pol_out);
               } else {
@@ -1038,28 +1081,22 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
                 }
               }
             }
-            ptx::bulk_commit_group();
-          }
-        } else {
-          __syncwarp();
-          if (x < p.N) {
+          } else {
             const int cols = p.N - x < 64 ? p.N - x : 64;
             copy_rows<128>(buf, reinterpret_cast<uint8_t*>(p.out + grow * p.ld_out + x),
-                           p.ld_out * 2, valid, cols * 2, lane);
+                           p.ld_out * 2, valid, cols * 2, pair_lane);
             if constexpr (kForm == EXP_SAVE8) {
               uint8_t* at = p.pre + grow * p.ld_pre + x;
-              copy_rows<64>(buf + kChunkBytes, at, p.ld_pre, valid, cols, lane);
+              copy_rows<64>(buf + kChunkBytes, at, p.ld_pre, valid, cols, pair_lane);
               copy_rows<64>(buf + kChunkBytes + kChunkBytes / 2, at + p.gate_off, p.ld_pre, valid,
-                            cols, lane);
+                            cols, pair_lane);
             }
           }
-          __syncwarp();
-          if (lane == 0) ptx::bulk_commit_group();    // keeps the buffers' turn-taking in step
+          if (issuer) ptx::bulk_commit_group();    // keeps the buffers' turn-taking in step
         }
       }
-      }
     }
-    if (lane == 0) ptx::bulk_wait_group_read<0>();
+    if (issuer) ptx::bulk_wait_group_read<0>();
   }
 
   // ---- teardown ----
