@@ -631,6 +631,34 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
                        int64_t ld_weights, int64_t ldw, int64_t w_stride, int64_t ldd,
                        int64_t d_stride, int64_t ldy, void* stream);
 
+/*
+ * The layer in training, one call each way.  sgl_experts_swiglu_save: y[T, D_out] (dense) as above
+ * (the down projection's sum in one range), and what the backward needs: order, an int32 buffer of
+ * E + 1 + 2 * T * k words (offsets, slots, rows as by sgl_expert_order), pre and scales as by
+ * sgl_grouped_fused_swiglu_save for T * k rows, and ys [T * k, D_out] fp32, the experts' outputs, which
+ * only grad_weights needs.
+ * sgl_experts_swiglu_backward: from grad_y[T, D_out] (dense) any of grad_x[T, D], grad_weights[T, k] (in
+ * the weights' type), grad_w[E, D, 2N], grad_down[E, N, D_out], all dense; NULL for what is not needed.
+ * `workspace`: caller-owned, of sgl_experts_swiglu_train_workspace_bytes bytes, overwritten.
+ */
+int64_t sgl_experts_swiglu_train_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D,
+                                                 int64_t N, int64_t D_out, int backward);
+int sgl_experts_swiglu_save(const void* x, const void* ids, int ids_are_int64, const void* weights,
+                            int weights_bf16, const void* w, const void* w_down, void* y,
+                            void* order, void* pre, void* scales, int bits, void* ys,
+                            void* workspace, int64_t workspace_bytes, int64_t T, int64_t k,
+                            int64_t E, int64_t D, int64_t N, int64_t D_out, int64_t ldx,
+                            int64_t ld_ids, int64_t ld_weights, int64_t ldw, int64_t w_stride,
+                            int64_t ldd, int64_t d_stride, void* stream);
+int sgl_experts_swiglu_backward(const void* grad_y, const void* x, const void* weights,
+                                int weights_bf16, const void* w, const void* w_down,
+                                const void* order, const void* pre, const void* scales, int bits,
+                                const void* ys, void* grad_x, void* grad_weights, void* grad_w,
+                                void* grad_down, void* workspace, int64_t workspace_bytes, int64_t T,
+                                int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
+                                int64_t ldx, int64_t ld_weights, int64_t ldw, int64_t w_stride,
+                                int64_t ldd, int64_t d_stride, void* stream);
+
 /* Message for the last non-zero return on the calling thread ("" if none). */
 const char* sgl_last_error(void);
 

@@ -10,8 +10,9 @@ mixture of SwiGLU experts (``experts``) and the differentiable forms (``autograd
 """
 from ._lib import TileConfig, SglError
 from .autograd import fused_swiglu, fused_swiglu_experts
-from .experts import (ExpertOrder, SavedPreact, expert_combine, expert_combine_grad, expert_dispatch,
-                      expert_order, experts_swiglu, experts_swiglu_workspace_bytes,
+from .experts import (ExpertOrder, SavedExperts, SavedPreact, expert_combine, expert_combine_grad,
+                      expert_dispatch, expert_order, experts_swiglu, experts_swiglu_backward,
+                      experts_swiglu_save, experts_swiglu_workspace_bytes,
                       fused_swiglu_backward_saved,
                       grouped_fused_swiglu, grouped_fused_swiglu_save, grouped_grad_preact,
                       grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact,
@@ -39,11 +40,14 @@ __all__ = [
     "grouped_weight_grad",
     "experts_swiglu",
     "experts_swiglu_workspace_bytes",
+    "experts_swiglu_save",
+    "experts_swiglu_backward",
     "matmul_fused_swiglu_save_preact",
     "swiglu_grad_preact_saved",
     "fused_swiglu_backward_saved",
     "ExpertOrder",
     "SavedPreact",
+    "SavedExperts",
     "PackedSwiGLULinear",
     "PackedSwiGLUExperts",
     "TileConfig",

@@ -90,6 +90,9 @@ EXPORTED_SYMBOLS = (
     "sgl_fused_swiglu_backward_saved",
     "sgl_experts_swiglu_workspace_bytes",
     "sgl_experts_swiglu",
+    "sgl_experts_swiglu_train_workspace_bytes",
+    "sgl_experts_swiglu_save",
+    "sgl_experts_swiglu_backward",
     "sgl_last_error",
     "sgl_version",
 )
@@ -313,6 +316,14 @@ def load() -> C.CDLL:
         lib.sgl_experts_swiglu_workspace_bytes.argtypes = [i64] * 6
         lib.sgl_experts_swiglu.restype = ip
         lib.sgl_experts_swiglu.argtypes = [vp, vp, ip, vp, ip, vp, vp, vp, vp, i64] + [i64] * 14 + [vp]
+        lib.sgl_experts_swiglu_train_workspace_bytes.restype = i64
+        lib.sgl_experts_swiglu_train_workspace_bytes.argtypes = [i64] * 6 + [ip]
+        lib.sgl_experts_swiglu_save.restype = ip
+        lib.sgl_experts_swiglu_save.argtypes = [vp, vp, ip, vp, ip, vp, vp, vp, vp, vp, vp, ip, vp,
+                                                vp, i64] + [i64] * 13 + [vp]
+        lib.sgl_experts_swiglu_backward.restype = ip
+        lib.sgl_experts_swiglu_backward.argtypes = [vp, vp, vp, ip, vp, vp, vp, vp, vp, ip] + \
+            [vp] * 6 + [i64] * 13 + [vp]
         lib.sgl_last_error.restype = C.c_char_p
         lib.sgl_last_error.argtypes = []
         lib.sgl_version.restype = ip

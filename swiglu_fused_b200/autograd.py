@@ -12,10 +12,9 @@ from __future__ import annotations
 import torch
 from torch.autograd.function import once_differentiable
 
-from .experts import (ExpertOrder, SavedPreact, _checkpoint_bits, _layer_operands, expert_combine,
-                      expert_combine_grad, expert_dispatch, expert_order,
-                      fused_swiglu_backward_saved, grouped_fused_swiglu_save, grouped_grad_preact,
-                      grouped_matmul, grouped_weight_grad, matmul_fused_swiglu_save_preact)
+from .experts import (SavedExperts, SavedPreact, _checkpoint_bits, experts_swiglu_backward,
+                      experts_swiglu_save, fused_swiglu_backward_saved,
+                      matmul_fused_swiglu_save_preact)
 from .ops import matmul_bf16, matmul_fused_swiglu_save_factors, swiglu_grad_preact
 
 
@@ -98,49 +97,26 @@ class FusedSwiGLUExpertsFunction(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, expert_ids, weights, w, w_down, checkpoint):
-        order = expert_order(expert_ids, w.shape[0])
-        xs = expert_dispatch(x, order)
-        h, pre = grouped_fused_swiglu_save(xs, w, order.offsets, checkpoint=checkpoint)
-        del xs
-        ys = grouped_matmul(h, w_down, order.offsets, out_dtype=torch.float32)
-        del h
-        y = expert_combine(ys, order, weights)
-        ctx.save_for_backward(x, weights, w, w_down, *order, pre.data, pre.scales,
-                              ys if ctx.needs_input_grad[2] else None)
+        y, saved = experts_swiglu_save(x, expert_ids, weights, w, w_down, checkpoint=checkpoint)
+        pre = saved.preact
+        ctx.save_for_backward(x, weights, w, w_down, saved.order, pre.data, pre.scales,
+                              saved.outputs if ctx.needs_input_grad[2] else None)
         ctx.bits, ctx.hidden = pre.bits, pre.hidden
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_y: torch.Tensor):
-        x, weights, w, w_down, offsets, slots, rows, data, scales, ys = ctx.saved_tensors
+        x, weights, w, w_down, order, data, scales, outputs = ctx.saved_tensors
         need_x, _, need_weights, need_w, need_down, _ = ctx.needs_input_grad
-        if x.shape[0] == 0:
-            return (torch.zeros_like(x), None, torch.zeros_like(weights), torch.zeros_like(w),
-                    torch.zeros_like(w_down), None)
-        order = ExpertOrder(offsets, slots, rows)
-        # the rows' gradients without the routing weights, and the weights' own
-        grad_rows, grad_weights = expert_combine_grad(_rows_of_gradient(grad_y), ys, order, weights,
-                                                      weighted=False)
-        grad_x = grad_w = grad_down = None
-        if need_x or need_w or need_down:
-            pre = SavedPreact(data, scales, ctx.bits, ctx.hidden)
-            grad_preact, h = grouped_grad_preact(grad_rows, w_down, pre, order, weights)
-            if need_down:
-                grad_down = grouped_weight_grad(h, grad_rows, offsets)
-            del h, grad_rows
-            if need_w:
-                grad_w = grouped_weight_grad(expert_dispatch(x, order), grad_preact, offsets)
-            if need_x:
-                grad_x = expert_combine(
-                    grouped_matmul(grad_preact, w, offsets, transpose_b=True,
-                                   out_dtype=torch.float32), order)
-        return grad_x, None, grad_weights if need_weights else None, grad_w, grad_down, None
+        saved = SavedExperts(order, SavedPreact(data, scales, ctx.bits, ctx.hidden), outputs)
+        grad_x, grad_weights, grad_w, grad_down = experts_swiglu_backward(
+            _rows_of_gradient(grad_y), x, weights, w, w_down, saved,
+            need=(need_x, need_weights, need_w, need_down))
+        return grad_x, None, grad_weights, grad_w, grad_down, None
 
 
 def fused_swiglu_experts(x, expert_ids, weights, w, w_down, *, checkpoint: str = "bf16"):
     """Differentiable expert layer: ``experts_swiglu`` with gradients for ``x``, ``weights``, ``w``
     and ``w_down``.  ``checkpoint`` is how the pre-activations are kept: ``"bf16"`` or ``"e4m3"``."""
-    _checkpoint_bits(checkpoint)
-    _layer_operands(x, expert_ids, weights, w, w_down)
     return FusedSwiGLUExpertsFunction.apply(x, expert_ids, weights, w, w_down, checkpoint)

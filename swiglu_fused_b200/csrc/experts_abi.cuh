@@ -1011,71 +1011,228 @@ int64_t sgl_experts_swiglu_workspace_bytes(int64_t T, int64_t k, int64_t E, int6
   return rc ? rc : w.total;
 }
 
+// What all three forms of the layer refuse, before the first launch.
+struct LayerCall {
+  const void *x, *ids, *weights, *w, *w_down;
+  int ids_are_int64, weights_bf16;
+  int64_t T, k, E, D, N, D_out;
+  int64_t ldx, ld_ids, ld_weights, ldw, w_stride, ldd, d_stride;
+};
+static int validate_layer(const LayerCall& c, bool with_ids) {
+  int rc;
+  if ((rc = validate_ptr(c.x, "x")) ||
+      (with_ids && (rc = validate_words(c.ids, "ids", c.ids_are_int64 ? 8 : 4))) ||
+      (rc = validate_words(c.weights, "weights", c.weights_bf16 ? 2 : 4)) ||
+      (rc = validate_ptr(c.w, "w")) || (rc = validate_ptr(c.w_down, "w_down")))
+    return rc;
+  if ((with_ids && c.ld_ids < c.k) || c.ld_weights < c.k)
+    return fail(SGL_ERR_BAD_STRIDE, "ld_ids=%lld and ld_weights=%lld must be at least k=%lld",
+                static_cast<long long>(c.ld_ids), static_cast<long long>(c.ld_weights),
+                static_cast<long long>(c.k));
+  if ((rc = validate_ld(c.ldx, c.D, "ldx")) || (rc = validate_ld(c.ldw, 2 * c.N, "ldw")) ||
+      (rc = validate_ld(c.ldd, c.D_out, "ldd")) ||
+      (rc = validate_expert_stride(c.w_stride, c.D, c.ldw, c.E, "w_stride")) ||
+      (rc = validate_expert_stride(c.d_stride, c.N, c.ldd, c.E, "d_stride")))
+    return rc;
+  return SGL_OK;
+}
+static int validate_workspace(const void* workspace, int64_t have, int64_t need) {
+  int rc = validate_ptr(workspace, "workspace");
+  if (rc) return rc;
+  if (have < need)
+    return fail(SGL_ERR_BAD_ARGUMENT, "workspace holds %lld bytes, %lld needed",
+                static_cast<long long>(have), static_cast<long long>(need));
+  return SGL_OK;
+}
+
+// The slots in order and x's rows with their experts: one launch for few slots, three for more.
+static int order_and_dispatch(const LayerCall& c, void* offsets, void* slots, void* rows,
+                              void* scratch, int64_t scratch_bytes, void* xs, void* stream) {
+  const int64_t R = c.T * c.k;
+  int rc;
+  if (R > sgl::kOrderRound) {
+    if ((rc = sgl_expert_order(c.ids, c.ids_are_int64, c.T, c.k, c.ld_ids, c.E, offsets, slots, rows,
+                               scratch, scratch_bytes, stream)))
+      return rc;
+    return sgl_expert_dispatch(c.x, rows, xs, c.T, c.k, c.D, R, c.ldx, c.D, stream);
+  }
+  DeviceInfo* info = nullptr;
+  if ((rc = check_device(&info)) || (rc = prepare_order_kernels())) return rc;
+  sgl::OrderParams p;
+  std::memset(&p, 0, sizeof(p));
+  p.ids = c.ids;
+  p.ld_ids = c.ld_ids;
+  p.total = p.per_cta = R;
+  p.k = static_cast<int>(c.k);
+  p.E = static_cast<int>(c.E);
+  p.ids64 = c.ids_are_int64 != 0;
+  p.offsets = static_cast<int*>(offsets);
+  p.slots = static_cast<int*>(slots);
+  p.rows = static_cast<int*>(rows);
+  int64_t ctas = (c.T + 3) / 4;
+  if (ctas > info->sm_count) ctas = info->sm_count;
+  return launch_after("expert_order_dispatch", sgl::expert_order_dispatch_kernel,
+                      dim3(static_cast<unsigned>(ctas)), dim3(sgl::kOrderThreads),
+                      sgl::order_smem_bytes(static_cast<int>(c.E)) + sgl::kOrderRound * 4, stream, p,
+                      static_cast<const __nv_bfloat16*>(c.x), static_cast<__nv_bfloat16*>(xs), c.ldx,
+                      static_cast<int64_t>(c.D), static_cast<int>(c.D / 8));
+}
+
 int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const void* weights,
                        int weights_bf16, const void* w, const void* w_down, void* y,
                        void* workspace, int64_t workspace_bytes, int64_t T, int64_t k, int64_t E,
                        int64_t D, int64_t N, int64_t D_out, int64_t ldx, int64_t ld_ids,
                        int64_t ld_weights, int64_t ldw, int64_t w_stride, int64_t ldd,
                        int64_t d_stride, int64_t ldy, void* stream) {
+  const LayerCall c{x, ids, weights, w,   w_down, ids_are_int64, weights_bf16, T,        k,  E,
+                    D, N,   D_out,   ldx, ld_ids, ld_weights,    ldw,          w_stride, ldd, d_stride};
   ExpertsWorkspace l;
   int rc;
-  if ((rc = experts_workspace(T, k, E, D, N, D_out, &l))) return rc;
-  if ((rc = validate_ptr(x, "x")) || (rc = validate_words(ids, "ids", ids_are_int64 ? 8 : 4)) ||
-      (rc = validate_words(weights, "weights", weights_bf16 ? 2 : 4)) ||
-      (rc = validate_ptr(w, "w")) || (rc = validate_ptr(w_down, "w_down")) ||
-      (rc = validate_ptr(y, "y")) || (rc = validate_ptr(workspace, "workspace")))
-    return rc;
-  if (workspace_bytes < l.total)
-    return fail(SGL_ERR_BAD_ARGUMENT, "workspace holds %lld bytes, %lld needed",
-                static_cast<long long>(workspace_bytes), static_cast<long long>(l.total));
-  // everything the launches below would refuse is refused before the first of them
-  if (ld_ids < k || ld_weights < k)
-    return fail(SGL_ERR_BAD_STRIDE, "ld_ids=%lld and ld_weights=%lld must be at least k=%lld",
-                static_cast<long long>(ld_ids), static_cast<long long>(ld_weights),
-                static_cast<long long>(k));
-  if ((rc = validate_ld(ldx, D, "ldx")) || (rc = validate_ld(ldw, 2 * N, "ldw")) ||
-      (rc = validate_ld(ldd, D_out, "ldd")) || (rc = validate_ld(ldy, D_out, "ldy")) ||
-      (rc = validate_expert_stride(w_stride, D, ldw, E, "w_stride")) ||
-      (rc = validate_expert_stride(d_stride, N, ldd, E, "d_stride")))
+  if ((rc = experts_workspace(T, k, E, D, N, D_out, &l)) || (rc = validate_layer(c, true)) ||
+      (rc = validate_ptr(y, "y")) || (rc = validate_ld(ldy, D_out, "ldy")) ||
+      (rc = validate_workspace(workspace, workspace_bytes, l.total)))
     return rc;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   const int64_t R = T * k;
-  if (R <= sgl::kOrderRound) {
-    DeviceInfo* info = nullptr;
-    if ((rc = check_device(&info)) || (rc = prepare_order_kernels())) return rc;
-    sgl::OrderParams p;
-    std::memset(&p, 0, sizeof(p));
-    p.ids = ids;
-    p.ld_ids = ld_ids;
-    p.total = p.per_cta = R;
-    p.k = static_cast<int>(k);
-    p.E = static_cast<int>(E);
-    p.ids64 = ids_are_int64 != 0;
-    p.offsets = reinterpret_cast<int*>(ws + l.offsets);
-    p.slots = reinterpret_cast<int*>(ws + l.slots);
-    p.rows = reinterpret_cast<int*>(ws + l.rows);
-    int64_t ctas = (T + 3) / 4;
-    if (ctas > info->sm_count) ctas = info->sm_count;
-    rc = launch_after("expert_order_dispatch", sgl::expert_order_dispatch_kernel,
-                      dim3(static_cast<unsigned>(ctas)), dim3(sgl::kOrderThreads),
-                      sgl::order_smem_bytes(static_cast<int>(E)) + sgl::kOrderRound * 4, stream, p,
-                      static_cast<const __nv_bfloat16*>(x),
-                      reinterpret_cast<__nv_bfloat16*>(ws + l.xs), ldx, static_cast<int64_t>(D),
-                      static_cast<int>(D / 8));
-    if (rc) return rc;
-  } else if ((rc = sgl_expert_order(ids, ids_are_int64, T, k, ld_ids, E, ws + l.offsets,
-                                    ws + l.slots, ws + l.rows, ws + l.scratch, l.scratch_bytes,
-                                    stream)) ||
-             (rc = sgl_expert_dispatch(x, ws + l.rows, ws + l.xs, T, k, D, R, ldx, D, stream))) {
-    return rc;
-  }
-  if ((rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
+  if ((rc = order_and_dispatch(c, ws + l.offsets, ws + l.slots, ws + l.rows, ws + l.scratch,
+                               l.scratch_bytes, ws + l.xs, stream)) ||
+      (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
                                      w_stride, N, stream)) ||
       (rc = grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
                            d_stride, D_out, 0, 1, l.splits, l.k_per_split, stream)))
     return rc;
   return combine_rows(ws + l.ys, 1, l.splits, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R,
                       D_out, ld_weights, ldy, stream);
+}
+
+// ---- the expert layer in training: forward and backward, one call each ----
+
+// An order as one int32 buffer: offsets[E + 1], slots[T * k], rows[T * k].
+struct OrderBuffer {
+  int *offsets, *slots, *rows;
+};
+static OrderBuffer split_order(const void* order, int64_t R, int64_t E) {
+  int* p = static_cast<int*>(const_cast<void*>(order));
+  return OrderBuffer{p, p + E + 1, p + E + 1 + R};
+}
+
+// Forward: the grouped x, h and the order's scratch.  Backward: the pre-activations' gradients, and
+// one region that holds the rows' gradients and the weighted h, then the grouped x, then the rows
+// of x's gradient (each is dead when the next is written).
+struct TrainWorkspace {
+  int64_t xs, h, scratch, scratch_bytes, forward;
+  int64_t grad_pre, region, weighted_h, backward;
+};
+static int train_workspace(int64_t T, int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
+                           TrainWorkspace* w) {
+  int rc;
+  if ((rc = validate_routing(T, k, E)) || (rc = validate_shape(T * k, N, D)) ||
+      (rc = validate_shape(T * k, D_out, 8)))
+    return rc;
+  const int64_t R = T * k;
+  w->xs = 0;
+  w->h = align256(R * D * 2);
+  w->scratch = w->h + align256(R * N * 2);
+  w->scratch_bytes = sgl_expert_order_scratch_bytes(T, k, E);
+  w->forward = w->scratch + align256(w->scratch_bytes);
+  w->grad_pre = 0;
+  w->region = align256(R * 2 * N * 2);
+  w->weighted_h = w->region + align256(R * D_out * 2);
+  const int64_t first = align256(R * D_out * 2) + align256(R * N * 2), rows = align256(R * D * 4);
+  w->backward = w->region + (first > rows ? first : rows);
+  return SGL_OK;
+}
+
+int64_t sgl_experts_swiglu_train_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D,
+                                                 int64_t N, int64_t D_out, int backward) {
+  TrainWorkspace w;
+  int rc = train_workspace(T, k, E, D, N, D_out, &w);
+  return rc ? rc : (backward ? w.backward : w.forward);
+}
+
+int sgl_experts_swiglu_save(const void* x, const void* ids, int ids_are_int64, const void* weights,
+                            int weights_bf16, const void* w, const void* w_down, void* y,
+                            void* order, void* pre, void* scales, int bits, void* ys,
+                            void* workspace, int64_t workspace_bytes, int64_t T, int64_t k,
+                            int64_t E, int64_t D, int64_t N, int64_t D_out, int64_t ldx,
+                            int64_t ld_ids, int64_t ld_weights, int64_t ldw, int64_t w_stride,
+                            int64_t ldd, int64_t d_stride, void* stream) {
+  const LayerCall c{x, ids, weights, w,   w_down, ids_are_int64, weights_bf16, T,        k,  E,
+                    D, N,   D_out,   ldx, ld_ids, ld_weights,    ldw,          w_stride, ldd, d_stride};
+  TrainWorkspace l;
+  int rc;
+  if ((rc = check_bits(bits)) || (rc = train_workspace(T, k, E, D, N, D_out, &l)) ||
+      (rc = validate_layer(c, true)) || (rc = validate_ptr(y, "y")) ||
+      (rc = validate_words(order, "order", 4)) || (rc = validate_ptr(pre, "pre")) ||
+      (bits == 8 && (rc = validate_words(scales, "scales", 2))) || (rc = validate_ptr(ys, "ys")) ||
+      (rc = validate_workspace(workspace, workspace_bytes, l.forward)))
+    return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t R = T * k;
+  const OrderBuffer o = split_order(order, R, E);
+  if ((rc = order_and_dispatch(c, o.offsets, o.slots, o.rows, ws + l.scratch, l.scratch_bytes,
+                               ws + l.xs, stream)) ||
+      (rc = sgl_grouped_fused_swiglu_save(ws + l.xs, w, o.offsets, ws + l.h, pre, scales, bits, R, N,
+                                          D, E, D, ldw, w_stride, N, stream)) ||
+      (rc = grouped_matmul(ws + l.h, w_down, o.offsets, ys, R, D_out, N, E, N, ldd, d_stride, D_out,
+                           0, 1, 1, 0, stream)))
+    return rc;
+  return combine_rows(ys, 1, 1, o.rows, weights, weights_bf16, y, T, k, D_out, R, D_out, ld_weights,
+                      D_out, stream);
+}
+
+int sgl_experts_swiglu_backward(const void* grad_y, const void* x, const void* weights,
+                                int weights_bf16, const void* w, const void* w_down,
+                                const void* order, const void* pre, const void* scales, int bits,
+                                const void* ys, void* grad_x, void* grad_weights, void* grad_w,
+                                void* grad_down, void* workspace, int64_t workspace_bytes, int64_t T,
+                                int64_t k, int64_t E, int64_t D, int64_t N, int64_t D_out,
+                                int64_t ldx, int64_t ld_weights, int64_t ldw, int64_t w_stride,
+                                int64_t ldd, int64_t d_stride, void* stream) {
+  const LayerCall c{x, nullptr, weights, w,   w_down, 0,          weights_bf16, T,        k,  E,
+                    D, N,       D_out,   ldx, 0,      ld_weights, ldw,          w_stride, ldd, d_stride};
+  TrainWorkspace l;
+  int rc;
+  if ((rc = check_bits(bits)) || (rc = train_workspace(T, k, E, D, N, D_out, &l)) ||
+      (rc = validate_layer(c, false)) || (rc = validate_ptr(grad_y, "grad_y")) ||
+      (rc = validate_words(order, "order", 4)) || (rc = validate_ptr(pre, "pre")) ||
+      (bits == 8 && (rc = validate_words(scales, "scales", 2))) ||
+      (grad_weights && ((rc = validate_ptr(ys, "ys")) ||
+                        (rc = validate_words(grad_weights, "grad_weights", weights_bf16 ? 2 : 4)))) ||
+      (grad_x && (rc = validate_ptr(grad_x, "grad_x"))) ||
+      (grad_w && (rc = validate_ptr(grad_w, "grad_w"))) ||
+      (grad_down && (rc = validate_ptr(grad_down, "grad_down"))) ||
+      (rc = validate_workspace(workspace, workspace_bytes, l.backward)))
+    return rc;
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  const int64_t R = T * k;
+  const OrderBuffer o = split_order(order, R, E);
+  void *grad_pre = ws + l.grad_pre, *region = ws + l.region, *weighted_h = ws + l.weighted_h;
+  // the rows' gradients without the routing weights, and the weights' own
+  if ((rc = sgl_expert_combine_grad(grad_y, grad_weights ? ys : nullptr, 1, o.rows, nullptr,
+                                    weights_bf16, region, grad_weights, T, k, D_out, R, D_out, D_out,
+                                    0, D_out, stream)))
+    return rc;
+  if (!grad_x && !grad_w && !grad_down) return SGL_OK;
+  if ((rc = sgl_grouped_grad_preact(region, w_down, o.offsets, o.slots, weights, weights_bf16, pre,
+                                    scales, bits, grad_pre, weighted_h, R, N, D_out, E, k, D_out,
+                                    ldd, d_stride, ld_weights, 2 * N, N, stream)))
+    return rc;
+  if (grad_down && (rc = sgl_grouped_weight_grad(weighted_h, region, o.offsets, grad_down, R, N,
+                                                 D_out, E, N, D_out, D_out, N * D_out, stream)))
+    return rc;
+  if (grad_w &&
+      ((rc = sgl_expert_dispatch(x, o.rows, region, T, k, D, R, ldx, D, stream)) ||
+       (rc = sgl_grouped_weight_grad(region, grad_pre, o.offsets, grad_w, R, D, 2 * N, E, D, 2 * N,
+                                     2 * N, D * 2 * N, stream))))
+    return rc;
+  if (grad_x) {
+    if ((rc = grouped_matmul(grad_pre, w, o.offsets, region, R, D, 2 * N, E, 2 * N, ldw, w_stride, D,
+                             1, 1, 1, 0, stream)))
+      return rc;
+    return combine_rows(region, 1, 1, o.rows, nullptr, 0, grad_x, T, k, D, R, D, 0, D, stream);
+  }
+  return SGL_OK;
 }
 
 }  // extern "C"

@@ -13,6 +13,7 @@ expert ``e`` owns ``W[e] = [W_up | W_gate]`` (``[K, 2N]``) and ``W_down[e]`` (``
 ``grouped_grad_preact``   the gate/up stage's backward behind the down projection, one launch
 ``grouped_weight_grad``   ``a_e^T @ g_e`` for every expert
 ``experts_swiglu``        all of the forward in one call, for inference
+``experts_swiglu_save``   the same for training, and ``experts_swiglu_backward``, its backward
 ``swiglu_grad_preact_saved``  the backward's elementwise step from saved pre-activations
 ``fused_swiglu_backward_saved``  the dense stage's whole backward from them
 
@@ -752,3 +753,102 @@ def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=Non
             y.data_ptr(), workspace.data_ptr(), workspace.numel(), T, k, E, D, N, D_out, ldx, ld_ids,
             ldw, _expert_ld(W), W.stride(0), _expert_ld(W_down), W_down.stride(0), _ld(y), handle))
     return y
+
+
+class SavedExperts(NamedTuple):
+    """What ``experts_swiglu_save`` keeps for the backward: the order as one int32 tensor (offsets,
+    slots, rows), the pre-activations, the experts' outputs ``[T * k, D_out]`` in fp32."""
+
+    order: torch.Tensor
+    preact: SavedPreact
+    outputs: torch.Tensor
+
+
+def experts_swiglu_save(x, expert_ids, weights, W, W_down, *, checkpoint: str = "bf16", stream=None):
+    """The expert layer for training, one library call: ``(y [T, D_out], SavedExperts)``.  Operands as
+    for ``experts_swiglu``; ``checkpoint`` as for ``grouped_fused_swiglu_save``."""
+    bits = _checkpoint_bits(checkpoint)
+    T, k, E, D, N, D_out, ldx, ld_ids, ldw, dev = _layer_operands(x, expert_ids, weights, W, W_down)
+    R = T * k
+    lib = _lib.load()
+    with _launch(stream, dev) as handle:
+        y = _empty2(T, D_out, DTYPE, dev)
+        order = torch.empty(E + 1 + 2 * R, dtype=torch.int32, device=dev)
+        pre = _empty_preact(bits, R, N, dev)
+        ys = _empty2(R, D_out, torch.float32, dev)
+        if T == 0:
+            order.zero_()
+            return y, SavedExperts(order, pre, ys)
+        need = lib.sgl_experts_swiglu_train_workspace_bytes(T, k, E, D, N, D_out, 0)
+        if need < 0:
+            _lib.check(int(need))
+        ws = torch.empty(need, dtype=torch.uint8, device=dev)
+        _lib.check(lib.sgl_experts_swiglu_save(
+            x.data_ptr(), expert_ids.data_ptr(), expert_ids.dtype is torch.int64,
+            weights.data_ptr(), weights.dtype is DTYPE, W.data_ptr(), W_down.data_ptr(),
+            y.data_ptr(), order.data_ptr(), pre.data.data_ptr(),
+            pre.scales.data_ptr() if pre.scales is not None else None, bits, ys.data_ptr(),
+            ws.data_ptr(), need, T, k, E, D, N, D_out, ldx, ld_ids, ldw, _expert_ld(W), W.stride(0),
+            _expert_ld(W_down), W_down.stride(0), handle))
+    return y, SavedExperts(order, pre, ys)
+
+
+def experts_swiglu_backward(grad_y, x, weights, W, W_down, saved: SavedExperts, *,
+                            need=(True, True, True, True), stream=None):
+    """Backward of ``experts_swiglu_save``, one library call: gradients of ``x``, ``weights``, ``W`` and
+    ``W_down``, None where ``need`` says so.  ``saved.outputs`` may be None if the weights need none."""
+    T, D, ldx = _matrix(x, "x")
+    T2, D_out, ldg = _matrix(grad_y, "grad_y")
+    if not isinstance(saved, SavedExperts):
+        raise TypeError(f"saved must be a SavedExperts, got {type(saved).__name__}")
+    k = weights.shape[1] if isinstance(weights, torch.Tensor) and weights.dim() == 2 else 0
+    ldw = _weights(weights, T, k)
+    _check_experts(W, "W")
+    _check_experts(W_down, "W_down")
+    E, D2, N2 = W.shape
+    N, R = N2 // 2, T * k
+    if T2 != T or D2 != D or N2 % 2 or tuple(W_down.shape) != (E, N, D_out):
+        raise ValueError(f"grad_y {tuple(grad_y.shape)}, x {tuple(x.shape)}, W {tuple(W.shape)} and "
+                         f"W_down {tuple(W_down.shape)} do not belong together")
+    _multiple_of_8(K=D, N=N, D=D_out)
+    if ldg != D_out:
+        raise ValueError(f"grad_y must be dense, got strides {grad_y.stride()}")
+    order, pre, ys = saved
+    _check_ints(order, "saved.order", (E + 1 + 2 * R,))
+    _check_preact(pre)
+    if pre.hidden != N or pre.data.shape[0] != R:
+        raise ValueError(f"the saved pre-activations are of {pre.data.shape[0]} rows and {pre.hidden} "
+                         f"columns, expected {R} and {N}")
+    need_x, need_weights, need_w, need_down = need
+    tensors = [x, grad_y, weights, W, W_down, order, pre.data]
+    if pre.scales is not None:
+        tensors.append(pre.scales)
+    if need_weights:
+        if ys is None:
+            raise ValueError("saved.outputs is needed for the weights' gradient")
+        R2, D3, ld_ys = _rows_matrix(ys, "saved.outputs")
+        if ys.dtype is not torch.float32 or (R2, D3, ld_ys) != (R, D_out, D_out):
+            raise ValueError(f"saved.outputs must be dense fp32 of shape {(R, D_out)}")
+        tensors.append(ys)
+    dev = _one_device(*tensors)
+    lib = _lib.load()
+    with _launch(stream, dev) as handle:
+        gx = _empty2(T, D, DTYPE, dev) if need_x else None
+        gr = _empty2(T, k, weights.dtype, dev) if need_weights else None
+        gw = torch.empty((E, D, N2), dtype=DTYPE, device=dev) if need_w else None
+        gd = torch.empty((E, N, D_out), dtype=DTYPE, device=dev) if need_down else None
+        if T == 0:
+            return gx, gr, gw.zero_() if need_w else None, gd.zero_() if need_down else None
+        size = lib.sgl_experts_swiglu_train_workspace_bytes(T, k, E, D, N, D_out, 1)
+        if size < 0:
+            _lib.check(int(size))
+        ws = torch.empty(size, dtype=torch.uint8, device=dev)
+        _lib.check(lib.sgl_experts_swiglu_backward(
+            grad_y.data_ptr(), x.data_ptr(), weights.data_ptr(), weights.dtype is DTYPE,
+            W.data_ptr(), W_down.data_ptr(), order.data_ptr(), pre.data.data_ptr(),
+            pre.scales.data_ptr() if pre.scales is not None else None, pre.bits,
+            ys.data_ptr() if need_weights else None, gx.data_ptr() if need_x else None,
+            gr.data_ptr() if need_weights else None, gw.data_ptr() if need_w else None,
+            gd.data_ptr() if need_down else None, ws.data_ptr(), size, T, k, E, D, N, D_out, ldx,
+            ldw, _expert_ld(W), W.stride(0), _expert_ld(W_down), W_down.stride(0), handle))
+    return gx, gr, gw, gd

@@ -122,6 +122,39 @@ def test_other_refusals():
     n = _lib.load().sgl_experts_swiglu_workspace_bytes(4, 2, 8, 16, 16, 16)
     call("sgl_experts_swiglu", -3, "ldd", P, P, 1, P, 0, P, P, P, P, n, 4, 2, 8, 16, 16, 16,
          16, 2, 2, 32, 512, 8, 256, 16, None)
+    size = _lib.load().sgl_experts_swiglu_train_workspace_bytes
+    fwd, bwd = size(4, 2, 8, 16, 16, 16, 0), size(4, 2, 8, 16, 16, 16, 1)
+    assert fwd >= 8 * (16 + 16) * 2 and bwd >= 8 * 32 * 2 + 8 * 16 * 4
+    assert size(4, 2, 1025, 16, 16, 16, 1) == -2
+
+    def save(code, needle, **change):
+        a = dict(ids=P, order=P, scales=P, ys=P, bits=8, bytes=fwd, ldd=16, ld_ids=2) | change
+        call("sgl_experts_swiglu_save", code, needle, P, a["ids"], 1, P, 0, P, P, P, a["order"], P,
+             a["scales"], a["bits"], a["ys"], P, a["bytes"], 4, 2, 8, 16, 16, 16, 16, a["ld_ids"], 2,
+             32, 512, a["ldd"], 256, None)
+
+    def grads(code, needle, **change):
+        a = dict(gy=P, order=P, scales=P, ys=P, gr=P, gw=P, bits=8, bytes=bwd, ldw=32) | change
+        call("sgl_experts_swiglu_backward", code, needle, a["gy"], P, P, 0, P, P, a["order"], P,
+             a["scales"], a["bits"], a["ys"], P, a["gr"], a["gw"], P, P, a["bytes"], 4, 2, 8, 16, 16,
+             16, 16, 2, a["ldw"], 512, 16, 256, None)
+
+    save(-1, "ids", ids=0)
+    save(-1, "order", order=0)
+    save(-1, "scales", scales=0)
+    save(-1, "ys", ys=0)
+    save(-10, "bits", bits=32)
+    save(-10, "workspace", bytes=fwd - 1)
+    save(-3, "ldd", ldd=8)
+    save(-3, "ld_ids", ld_ids=1)
+    grads(-1, "grad_y", gy=0)
+    grads(-4, "order", order=P + 2)
+    grads(-1, "ys", ys=0)
+    grads(-4, "grad_weights", gr=P + 2)
+    grads(-4, "grad_w", gw=P + 8)
+    grads(-10, "bits", bits=0)
+    grads(-10, "workspace", bytes=bwd - 1)
+    grads(-3, "ldw", ldw=16)
     assert _lib.load().sgl_experts_swiglu_workspace_bytes(0, 2, 8, 16, 16, 16) == -2
     assert _lib.load().sgl_preact_bytes(8, 4, 12, None, None, None) == -2
 
@@ -178,6 +211,20 @@ def test_python_refusals():
         sg.PackedSwiGLUExperts(16, 12, 4)
     with pytest.raises(TypeError, match="SavedPreact"):
         sg.swiglu_grad_preact_saved(x, x)
+
+
+def test_training_call_refusals():
+    """The layer's one-call forward and backward have no CPU path."""
+    x, ids, rw = torch.zeros((4, 16), dtype=BF16), torch.zeros((4, 2), dtype=torch.int32), torch.zeros(4, 2)
+    w, wd = torch.zeros((3, 16, 48), dtype=BF16), torch.zeros((3, 24, 8), dtype=BF16)
+    with pytest.raises(ValueError, match="checkpoint"):
+        sg.experts_swiglu_save(x, ids, rw, w, wd, checkpoint="int8")
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.experts_swiglu_save(x, ids, rw, w, wd)
+    pre = sg.SavedPreact(torch.zeros((8, 48), dtype=BF16), None, 16, 24)
+    saved = sg.SavedExperts(torch.zeros(3 + 1 + 16, dtype=torch.int32), pre, torch.zeros(8, 8))
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.experts_swiglu_backward(torch.zeros((4, 8), dtype=BF16), x, rw, w, wd, saved)
 
 
 def test_module_parameters_and_expert_loading():

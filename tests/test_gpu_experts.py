@@ -525,6 +525,68 @@ def test_layer_forward(T, k, E, D, N, D_out, wdtype):
 
 @pytest.mark.parametrize("T,k,E,D,N,D_out", LAYERS)
 @pytest.mark.parametrize("checkpoint", ["bf16", "e4m3"])
+@pytest.mark.parametrize("wdtype", [torch.float32, BF16])
+def test_layer_in_training_is_its_separate_steps(T, k, E, D, N, D_out, checkpoint, wdtype):
+    """The one-call forward and backward against the operators called one by one, bit for bit."""
+    x, ids, rw, w, wd = layer_inputs(T, k, E, D, N, T + 3, drop=0.2, wdtype=wdtype, D_out=D_out)
+    dy = randn(T, wd.shape[2], seed=4)
+    y, saved = sg.experts_swiglu_save(x, ids, rw, w, wd, checkpoint=checkpoint)
+    order = sg.expert_order(ids, E)
+    assert torch.equal(saved.order, torch.cat([t.reshape(-1) for t in order]))
+    kept = int(order.offsets[-1])
+    xs = sg.expert_dispatch(x, order)
+    h, pre = sg.grouped_fused_swiglu_save(xs, w, order.offsets, checkpoint=checkpoint)
+    ys = sg.grouped_matmul(h, wd, order.offsets, out_dtype=torch.float32)
+    assert torch.equal(saved.outputs[:kept], ys[:kept])
+    for a, b in zip(ref.saved_values(saved.preact), ref.saved_values(pre)):
+        assert torch.equal(a[:kept], b[:kept])
+    assert torch.equal(y, sg.expert_combine(ys, order, rw))
+    rows, grw = sg.expert_combine_grad(dy, ys, order, rw, weighted=False)
+    gp, hw = sg.grouped_grad_preact(rows, wd, pre, order, rw)
+    want = (sg.expert_combine(sg.grouped_matmul(gp, w, order.offsets, transpose_b=True,
+                                                out_dtype=torch.float32), order),
+            grw, sg.grouped_weight_grad(xs, gp, order.offsets),
+            sg.grouped_weight_grad(hw, rows, order.offsets))
+    got = sg.experts_swiglu_backward(dy, x, rw, w, wd, saved)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for i in range(4):
+        need = [j == i for j in range(4)]
+        one = sg.experts_swiglu_backward(dy, x, rw, w, wd, saved, need=need)
+        assert all((a is not None) == n for a, n in zip(one, need)) and torch.equal(one[i], want[i])
+    none = sg.experts_swiglu_backward(dy, x, rw, w, wd, saved._replace(outputs=None),
+                                      need=(True, False, True, True))
+    assert none[1] is None and torch.equal(none[0], want[0])
+    with pytest.raises(ValueError, match="outputs"):
+        sg.experts_swiglu_backward(dy, x, rw, w, wd, saved._replace(outputs=None))
+
+
+def test_training_call_refusals():
+    """What does not belong together is refused before any launch."""
+    x, ids, rw, w, wd = layer_inputs(4, 2, 3, 16, 24, 1, D_out=8)
+    dy = randn(4, 8, seed=2)
+    with pytest.raises(ValueError, match="W_down"):
+        sg.experts_swiglu_save(x, ids, rw, w, wd[:2])
+    saved = sg.experts_swiglu_save(x, ids, rw, w, wd)[1]
+    pre = saved.preact
+
+    def refuses(needle, kind=ValueError, g=dy, s=saved, at=x):
+        with pytest.raises(kind, match=needle):
+            sg.experts_swiglu_backward(g, at, rw, w, wd, s)
+
+    refuses("SavedExperts", TypeError, s=tuple(saved))
+    refuses("belong together", g=dy[:3])
+    refuses("belong together", at=randn(4, 24, seed=3))
+    refuses("dense", g=randn(4, 16, seed=3)[:, :8])
+    refuses("saved.order", s=saved._replace(order=saved.order[:-1]))
+    refuses("pre-activations", s=saved._replace(preact=pre._replace(data=pre.data[:7])))
+    refuses("needed for the weights", s=saved._replace(outputs=None))
+    refuses("dense fp32", s=saved._replace(outputs=saved.outputs[:7]))
+    refuses("dense fp32", s=saved._replace(outputs=saved.outputs.to(BF16)))
+    refuses("CUDA", at=x.cpu())
+
+
+@pytest.mark.parametrize("T,k,E,D,N,D_out", LAYERS)
+@pytest.mark.parametrize("checkpoint", ["bf16", "e4m3"])
 def test_layer_gradients(T, k, E, D, N, D_out, checkpoint):
     """Against the formulas in 64 bits, over the pre-activations as they were kept; relative to
     the size of each gradient: two roundings to bf16 lie on the way to each result (h or the
