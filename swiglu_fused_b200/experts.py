@@ -19,7 +19,8 @@ expert ``e`` owns ``W[e] = [W_up | W_gate]`` (``[K, 2N]``) and ``W_down[e]`` (``
 
 The conventions are those of the other operators: bf16 tensors with unit column stride and 16-byte
 rows, checks before anything is launched, torch's current stream unless ``stream=`` is given,
-``out=`` for caller-owned results, no CPU path.  The row counts of the groups live on the device
+``out=`` for caller-owned results (which overlap no operand unless an operator allows it), no CPU
+path.  The row counts of the groups live on the device
 (``offsets``): no call here waits for the GPU.
 """
 from __future__ import annotations
@@ -59,8 +60,13 @@ class _launch:
             self.prev = cur
             torch.cuda.set_device(self.dev.index)
         if self.stream is not None:
-            self.ctx = stream_context(self.stream, self.dev)
-            self.ctx.__enter__()
+            try:
+                ctx = stream_context(self.stream, self.dev)
+                ctx.__enter__()
+            except BaseException:
+                self.__exit__()
+                raise
+            self.ctx = ctx
         return _stream_handle(self.stream, self.dev)
 
     def __exit__(self, *exc):
@@ -449,6 +455,8 @@ def _empty_preact(bits: int, rows: int, N: int, dev) -> SavedPreact:
 def _check_preact(p: SavedPreact) -> None:
     if not isinstance(p, SavedPreact):
         raise TypeError(f"preact must be a SavedPreact, got {type(p).__name__}")
+    if not isinstance(p.data, torch.Tensor) or p.data.dim() != 3:
+        raise ValueError("preact.data must be a [rows, 2, columns] tensor")
     if p.bits not in (8, 16):
         raise ValueError(f"preact.bits must be 8 or 16, got {p.bits}")
     shape, scale_shape = _preact_shapes(p.bits, p.data.shape[0], p.hidden)

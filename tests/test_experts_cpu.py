@@ -227,6 +227,18 @@ def test_training_call_refusals():
         sg.experts_swiglu_backward(torch.zeros((4, 8), dtype=BF16), x, rw, w, wd, saved)
 
 
+def test_a_bad_stream_leaves_the_current_device(monkeypatch):
+    """A call whose stream is not one leaves the device current that was."""
+    from swiglu_fused_b200 import experts
+    at = [1]
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: at[-1])
+    monkeypatch.setattr(torch.cuda, "set_device", at.append)
+    with pytest.raises(ValueError):
+        with experts._launch("no stream", torch.device("cuda", 0)):
+            pass
+    assert at == [1, 0, 1]
+
+
 def test_module_parameters_and_expert_loading():
     mod = sg.PackedSwiGLUExperts(16, 24, 3, out_features=8)
     assert mod.weight.shape == (3, 16, 48) and mod.weight_down.shape == (3, 24, 8)

@@ -661,7 +661,8 @@ def test_layer_gradients_against_differences():
         assert abs(got - slope) <= 8 * ref.BF16_HALF * grad.double().norm().item(), i
 
 
-@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (200, 136, 264), (300, 512, 384), (1024, 256, 72)])
+@pytest.mark.parametrize("M,K,N", [(1, 8, 8), (7, 72, 136), (200, 136, 264), (333, 264, 72), (300, 512, 384),
+                                   (1024, 256, 72)])
 @pytest.mark.parametrize("checkpoint", ["bf16", "e4m3"])
 def test_dense_stage_over_a_checkpoint(M, K, N, checkpoint):
     x = randn(M, K, seed=M).requires_grad_(True)
