@@ -302,6 +302,8 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.K = static_cast<int>(s.K);
   p.M = static_cast<int>(s.M);
   p.tiles_n = static_cast<int>(tiles_n);
+  // (8192 tokens x 2 of 8 experts, 4096 x 14336: 4.73 ms, with 8 tile rows together 4.80, with 32
+  // 4.82, with 4 5.20; no difference with small groups)
   p.group_m = 16;
   p.stages = stages;
   p.acc_cols = acc_cols;
