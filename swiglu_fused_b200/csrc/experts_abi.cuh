@@ -177,7 +177,6 @@ struct ExpertLaunch {
   int w_bf16 = 0;
   int splits = 1;            // EXP_GEMM32: ranges of K, each with its own slot of the result
   int64_t k_per_split = 0;
-  bool early_b = false;      // the launch before this one wrote neither the offsets nor B
 };
 
 // Byte layout of saved pre-activations: rows of [up | gate], each half padded to whole blocks.
@@ -331,7 +330,6 @@ int launch_experts(const ExpertLaunch& s, void* stream) {
   p.w_bf16 = s.w_bf16;
   // operands evict-last, results evict-first, as for the dense stage
   p.l2_hints = 2 | (2 << 2) | (1 << 4);
-  p.early_b = s.early_b;
   p.wait_limit_ns = g_wait_limit_ns.load();
 
   const int64_t grid = units < clusters ? units : clusters;
@@ -687,7 +685,7 @@ int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int6
 static int grouped_swiglu(const char* name, const void* x, const void* w, const void* offsets,
                           void* h, void* pre, void* scales, int bits, int64_t R, int64_t N,
                           int64_t K, int64_t E, int64_t ldx, int64_t ldw, int64_t w_stride,
-                          int64_t ldh, bool early_b, void* stream) {
+                          int64_t ldh, void* stream) {
   int rc;
   if ((rc = validate_groups(R, E, offsets, E > 1))) return rc;
   if ((rc = validate_ptr(x, "x")) || (rc = validate_ptr(w, "w")) || (rc = validate_ptr(h, "h")))
@@ -718,7 +716,6 @@ static int grouped_swiglu(const char* name, const void* x, const void* w, const 
   s.ld_out = ldh;
   s.pre = pre;
   s.scales = scales;
-  s.early_b = early_b;
   return launch_experts(s, stream);
 }
 
@@ -728,7 +725,7 @@ int sgl_grouped_fused_swiglu(const void* x, const void* w, const void* offsets, 
   int rc = validate_groups(R, E, offsets, true);
   if (rc) return rc;
   return grouped_swiglu("grouped_fused_swiglu", x, w, offsets, h, nullptr, nullptr, 0, R, N, K, E,
-                        ldx, ldw, w_stride, ldh, false, stream);
+                        ldx, ldw, w_stride, ldh, stream);
 }
 
 int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offsets, void* h,
@@ -738,13 +735,13 @@ int sgl_grouped_fused_swiglu_save(const void* x, const void* w, const void* offs
   int rc = check_bits(bits);
   if (rc) return rc;
   return grouped_swiglu("grouped_fused_swiglu_save", x, w, offsets, h, pre, scales, bits, R, N, K,
-                        E, ldx, ldw, w_stride, ldh, false, stream);
+                        E, ldx, ldw, w_stride, ldh, stream);
 }
 
 static int grouped_matmul(const void* a, const void* b, const void* offsets, void* c, int64_t R,
                           int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb,
                           int64_t b_stride, int64_t ldc, int b_transposed, int c_is_f32, int splits,
-                          int64_t k_per_split, bool early_b, void* stream) {
+                          int64_t k_per_split, void* stream) {
   int rc;
   if ((rc = validate_groups(R, E, offsets, true))) return rc;
   if ((rc = validate_ptr(a, "a")) || (rc = validate_ptr(b, "b")) || (rc = validate_ptr(c, "c")))
@@ -773,7 +770,6 @@ static int grouped_matmul(const void* a, const void* b, const void* offsets, voi
   s.b_transposed = b_transposed != 0;
   s.splits = splits;
   s.k_per_split = k_per_split;
-  s.early_b = early_b;
   return launch_experts(s, stream);
 }
 
@@ -781,7 +777,7 @@ int sgl_grouped_matmul(const void* a, const void* b, const void* offsets, void* 
                        int64_t N, int64_t K, int64_t E, int64_t lda, int64_t ldb, int64_t b_stride,
                        int64_t ldc, int b_transposed, int c_is_f32, void* stream) {
   return grouped_matmul(a, b, offsets, c, R, N, K, E, lda, ldb, b_stride, ldc, b_transposed,
-                        c_is_f32, 1, 0, false, stream);
+                        c_is_f32, 1, 0, stream);
 }
 
 int sgl_grouped_grad_preact(const void* dy, const void* w_down, const void* offsets,
@@ -1051,14 +1047,12 @@ static int validate_workspace(const void* workspace, int64_t have, int64_t need)
   return SGL_OK;
 }
 
-// The slots in order and x's rows with their experts: one launch for few slots, three for more (of
-// which the last does not write the offsets: the product behind them starts with its weights).
-static bool offsets_come_early(const LayerCall& c) { return c.T * c.k > sgl::kOrderRound; }
+// The slots in order and x's rows with their experts: one launch for few slots, three for more.
 static int order_and_dispatch(const LayerCall& c, void* offsets, void* slots, void* rows,
                               void* scratch, int64_t scratch_bytes, void* xs, void* stream) {
   const int64_t R = c.T * c.k;
   int rc;
-  if (offsets_come_early(c)) {
+  if (R > sgl::kOrderRound) {
     if ((rc = sgl_expert_order(c.ids, c.ids_are_int64, c.T, c.k, c.ld_ids, c.E, offsets, slots, rows,
                                scratch, scratch_bytes, stream)))
       return rc;
@@ -1104,11 +1098,10 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
   const int64_t R = T * k;
   if ((rc = order_and_dispatch(c, ws + l.offsets, ws + l.slots, ws + l.rows, ws + l.scratch,
                                l.scratch_bytes, ws + l.xs, stream)) ||
-      (rc = grouped_swiglu("grouped_fused_swiglu", ws + l.xs, w, ws + l.offsets, ws + l.h, nullptr,
-                           nullptr, 0, R, N, D, E, D, ldw, w_stride, N, offsets_come_early(c),
-                           stream)) ||
+      (rc = sgl_grouped_fused_swiglu(ws + l.xs, w, ws + l.offsets, ws + l.h, R, N, D, E, D, ldw,
+                                     w_stride, N, stream)) ||
       (rc = grouped_matmul(ws + l.h, w_down, ws + l.offsets, ws + l.ys, R, D_out, N, E, N, ldd,
-                           d_stride, D_out, 0, 1, l.splits, l.k_per_split, true, stream)))
+                           d_stride, D_out, 0, 1, l.splits, l.k_per_split, stream)))
     return rc;
   return combine_rows(ws + l.ys, 1, l.splits, ws + l.rows, weights, weights_bf16, y, T, k, D_out, R,
                       D_out, ld_weights, ldy, stream);
@@ -1181,11 +1174,10 @@ int sgl_experts_swiglu_save(const void* x, const void* ids, int ids_are_int64, c
   const OrderBuffer o = split_order(order, R, E);
   if ((rc = order_and_dispatch(c, o.offsets, o.slots, o.rows, ws + l.scratch, l.scratch_bytes,
                                ws + l.xs, stream)) ||
-      (rc = grouped_swiglu("grouped_fused_swiglu_save", ws + l.xs, w, o.offsets, ws + l.h, pre,
-                           scales, bits, R, N, D, E, D, ldw, w_stride, N, offsets_come_early(c),
-                           stream)) ||
+      (rc = sgl_grouped_fused_swiglu_save(ws + l.xs, w, o.offsets, ws + l.h, pre, scales, bits, R, N,
+                                          D, E, D, ldw, w_stride, N, stream)) ||
       (rc = grouped_matmul(ws + l.h, w_down, o.offsets, ys, R, D_out, N, E, N, ldd, d_stride, D_out,
-                           0, 1, 1, 0, true, stream)))
+                           0, 1, 1, 0, stream)))
     return rc;
   return combine_rows(ys, 1, 1, o.rows, weights, weights_bf16, y, T, k, D_out, R, D_out, ld_weights,
                       D_out, stream);
@@ -1237,9 +1229,8 @@ int sgl_experts_swiglu_backward(const void* grad_y, const void* x, const void* w
                                      2 * N, D * 2 * N, stream))))
     return rc;
   if (grad_x) {
-    // (the launch before it is a product of this call)
     if ((rc = grouped_matmul(grad_pre, w, o.offsets, region, R, D, 2 * N, E, 2 * N, ldw, w_stride, D,
-                             1, 1, 1, 0, true, stream)))
+                             1, 1, 1, 0, stream)))
       return rc;
     return combine_rows(region, 1, 1, o.rows, nullptr, 0, grad_x, T, k, D, R, D, 0, D, stream);
   }

@@ -409,9 +409,8 @@ __device__ __forceinline__ int row_of(const RowParams& p, int64_t t, int j) {
 // out[rows[t, j]] = x[t]: x is read once, each of its rows written once.
 __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p) {
   constexpr int kVecs = 2;
-  // (in this order: a product behind it may count on the launch before this one, see early_b)
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int tx = blockDim.x * gridDim.y;     // threads of a token
   const int first = blockIdx.y * blockDim.x + threadIdx.x;
   for (int64_t t = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; t < p.T;

@@ -105,7 +105,6 @@ struct ExpertParams {
   int64_t ld_w, num_slots;
   int k, w_bf16;
   int l2_hints;
-  int early_b;          // offsets and B are not of the launch before this one: see the kernel
   unsigned long long wait_limit_ns;
 };
 
@@ -455,19 +454,8 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   }
   if (warp == 1) ptx::tmem_alloc<kCtaGroup>(tmem_slot, kTmemCols);
 
-  // The next launch may start once this one has seen the end of the launch before it: so all that a
-  // launch with early_b can meet still running is its direct predecessor, which has written
-  // neither its offsets nor its B.  It looks up its tiles and fills its ring with B on SMs that
-  // the predecessor has left, and waits before anything else.  The layer with both its products
-  // so (the gate/up stage only behind a dispatch launch of its own): one token of 2 experts,
-  // 4096 x 14336, 146.1 -> 141.3 us; 1531 tokens x 4 of 40, 1416 x 712, 111.1 -> 107.3.  (Fetching the
-  // blocks beyond the ring into L2 as well gives half of that back: the predecessor's last tiles
-  // slow down.)
-  const bool early = p.early_b != 0;
-  if (!early) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  }
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
 
   // ---- the groups: first row (clamped: rows that do not exist in the row tensors are never
   // addressed, whatever the offsets say), and a table of first tile rows ----
@@ -571,10 +559,6 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
   };
 
   const uint64_t limit = p.wait_limit_ns;
-  if (early && warp != 6) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  }
 
   // =========================== TMA producers ===========================
   // One thread each for the A and the B operand: a copy takes its thread about 230 cycles to
@@ -585,7 +569,6 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
     int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    [[maybe_unused]] bool waits = !kA && early;    // for the launch before, once the ring is full
     Unit next;
     if (cluster_id < total_units) next = unit_of(cluster_id);
     for (int u = cluster_id; u < total_units && ok; u += num_clusters) {
@@ -687,17 +670,11 @@ experts_kernel(const __grid_constant__ ExpertMaps maps, const ExpertParams p) {
         if (++s == stages) {
           s = 0;
           ph ^= 1u;
-          if (!kA && waits) {
-            asm volatile("griddepcontrol.wait;" ::: "memory");
-            asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            waits = false;
-          }
         }
         // the next tile is looked up while this one's loads are under way
         if (kb == 0 && u + num_clusters < total_units) next = unit_of(u + num_clusters);
       }
     }
-    if (!kA && waits) asm volatile("griddepcontrol.wait;" ::: "memory");
     if (!ok) {
       // loads in flight land before the CTA exits
       const uint64_t t0 = ptx::globaltimer_ns();

@@ -1,12 +1,14 @@
 """Refusals and host arithmetic of the mixture-of-experts operators, without a GPU."""
 import ctypes as C
+import os
+import re
 
 import pytest
 import torch
 
 import experts_reference as ref
 import swiglu_fused_b200 as sg
-from swiglu_fused_b200 import _lib, experts
+from swiglu_fused_b200 import _lib, build, experts
 
 BUF = (C.c_uint8 * 4096)()
 P = (C.addressof(BUF) + 15) // 16 * 16
@@ -258,3 +260,34 @@ def test_reference_block_codes():
     assert scales.view(-1).tolist() == [127, 128, 0]
     assert codes[0, 0].item() == 0x7e and codes[0, 1].item() == 0x38
     assert codes[1, 0].item() == 0x76              # 224.5 -> 224
+
+
+def _kernels(source):
+    """(name, body) of every kernel of a source file, comments taken out."""
+    text = re.sub(r"//[^\n]*", "", source)
+    for m in re.finditer(r"__global__ void(?:\s+__launch_bounds__\(.*?\))?\s+(\w+)\(", text):
+        start = text.index("{", m.end())
+        depth, end = 1, start + 1
+        while depth:
+            depth += {"{": 1, "}": -1}.get(text[end], 0)
+            end += 1
+        yield m.group(1), text[start + 1:end - 1]
+
+
+@pytest.mark.parametrize("name", ["experts_order.cuh", "experts_products.cuh", "swiglu_preact.cuh"])
+def test_kernels_wait_before_they_touch_memory(name):
+    """These kernels are launched beside the end of the launch before them.  What that launch, or an
+    earlier one, has written is visible to a kernel only behind its own griddepcontrol.wait: the wait
+    is unconditional, and no global memory is read or written before it."""
+    with open(os.path.join(build.CSRC_DIR, name)) as f:
+        kernels = list(_kernels(f.read()))
+    assert kernels
+    for kernel, body in kernels:
+        at = body.find("griddepcontrol.wait")
+        assert at >= 0, f"{kernel} does not wait"
+        before = body[:at]
+        assert before.count("{") == before.count("}"), f"{kernel} waits under a condition"
+        # (kernel parameters used as addresses, TMA copies, and the helpers that read global memory)
+        touches = re.search(r"p\.\w+\s*\[|\*\s*p\.|tma_|\.load\(|row_lo\(|order_key\(|row_of\(|"
+                            r"load_weight\(|\.run\(", before)
+        assert touches is None, f"{kernel}: {touches and touches.group()!r} before the wait"

@@ -916,3 +916,112 @@ def test_on_a_device_that_is_not_the_current_one():
     assert torch.cuda.current_device() == 0
     with pytest.raises(ValueError, match="different devices"):
         sg.experts_swiglu(args[0].to("cuda:0"), *args[1:])
+
+
+# ---------------------------------------------------------------- calls close behind one another
+
+
+def routings(T, k, E):
+    """Routing that differs from call to call as far as it can: all to the first expert, all to the
+    last, spread evenly, drawn with drops, none kept."""
+    first = torch.zeros((T, k), dtype=torch.int64, device=DEV)
+    even = (torch.arange(T * k, device=DEV) % E).view(T, k)
+    return [first, first + E - 1, even, make_ids(T, k, E, 11, 0.2), first - 1]
+
+
+@pytest.mark.parametrize("T,k,E", [(64, 2, 12), (1100, 2, 12), (700, 4, 40)])
+def test_queued_calls_see_their_own_routing_and_weights(T, k, E):
+    """Layer calls queued without a pause on one workspace and one set of buffers, with the routing
+    and the weights rewritten in the stream between them: each result is that of the call alone."""
+    D, N = 264, 328
+    x, _, rw, w0, wd0 = layer_inputs(T, k, E, D, N, T)
+    weights = [(w0, wd0), (randn(E, D, 2 * N, seed=91, std=D ** -0.5),
+                           randn(E, N, D, seed=92, std=N ** -0.5))]
+    ids_all = routings(T, k, E)
+    alone = {}
+    for i, ids in enumerate(ids_all):
+        for j, (w, wd) in enumerate(weights):
+            alone[i, j] = sg.experts_swiglu(x, ids, rw, w, wd)
+            torch.cuda.synchronize()
+    ws = torch.full((sg.experts_swiglu_workspace_bytes(T, k, E, D, N, D),), 255, dtype=torch.uint8,
+                    device=DEV)
+    ids, w, wd = ids_all[0].clone(), w0.clone(), wd0.clone()
+    order = [(n * 3 % len(ids_all), n // 2 % 2) for n in range(40)]
+    got = [torch.empty_like(x) for _ in order]
+    torch.cuda.synchronize()
+    for (i, j), y in zip(order, got):
+        ids.copy_(ids_all[i])
+        w.copy_(weights[j][0])
+        wd.copy_(weights[j][1])
+        sg.experts_swiglu(x, ids, rw, w, wd, out=y, workspace=ws)
+    torch.cuda.synchronize()
+    for n, ((i, j), y) in enumerate(zip(order, got)):
+        assert torch.equal(y, alone[i, j]), (n, i, j)
+
+
+@pytest.mark.parametrize("checkpoint", ["bf16", "e4m3"])
+def test_queued_training_steps_see_their_own_routing_and_weights(checkpoint):
+    T, k, E, D, N = 1100, 2, 12, 264, 328
+    x, _, rw, w0, wd0 = layer_inputs(T, k, E, D, N, 5)
+    dy = randn(T, D, seed=6)
+    ids_all = routings(T, k, E)
+
+    def step(ids, w, wd):
+        y, saved = sg.experts_swiglu_save(x, ids, rw, w, wd, checkpoint=checkpoint)
+        return (y, *sg.experts_swiglu_backward(dy, x, rw, w, wd, saved))
+
+    scaled = [(w0, wd0), (w0 * 0.5, wd0 * 2)]
+    alone = {}
+    for i, ids in enumerate(ids_all):
+        for j, (w, wd) in enumerate(scaled):
+            alone[i, j] = step(ids, w, wd)
+            torch.cuda.synchronize()
+    ids, w, wd = ids_all[0].clone(), w0.clone(), wd0.clone()
+    got = []
+    for n in range(20):
+        i, j = n * 3 % len(ids_all), n // 2 % 2
+        ids.copy_(ids_all[i])
+        w.copy_(scaled[j][0])
+        wd.copy_(scaled[j][1])
+        got.append((i, j, step(ids, w, wd)))
+    torch.cuda.synchronize()
+    for n, (i, j, result) in enumerate(got):
+        for name, a, b in zip(("y", "x", "weights", "w", "w_down"), result, alone[i, j]):
+            assert torch.equal(a, b), (n, i, j, name)
+
+
+@pytest.mark.parametrize("T,k,E", [(64, 2, 12), (1100, 2, 12)])
+def test_captured_calls_see_rewritten_routing_and_weights(T, k, E):
+    """Two layers in one graph, one behind the other, replayed over rewritten routing and weights
+    without a pause."""
+    D, N = 264, 328
+    x, _, rw, w0, wd0 = layer_inputs(T, k, E, D, N, T + 1)
+    ids_all = routings(T, k, E)
+    other = (randn(E, D, 2 * N, seed=91, std=D ** -0.5), randn(E, N, D, seed=92, std=N ** -0.5))
+    ids, w, wd = ids_all[3].clone(), w0.clone(), wd0.clone()
+
+    def two_layers():
+        return sg.experts_swiglu(sg.experts_swiglu(x, ids, rw, w, wd), ids, rw, w, wd)
+
+    want = {}
+    for i in range(len(ids_all)):
+        for j, (a, b) in enumerate([(w0, wd0), other]):
+            ids.copy_(ids_all[i])
+            w.copy_(a)
+            wd.copy_(b)
+            want[i, j] = two_layers()
+            torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = two_layers()
+    got = []
+    for n in range(20):
+        i, j = n * 3 % len(ids_all), n // 2 % 2
+        ids.copy_(ids_all[i])
+        w.copy_((w0, other[0])[j])
+        wd.copy_((wd0, other[1])[j])
+        g.replay()
+        got.append((i, j, y.clone()))
+    torch.cuda.synchronize()
+    for n, (i, j, v) in enumerate(got):
+        assert torch.equal(v, want[i, j]), (n, i, j)
