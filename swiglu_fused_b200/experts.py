@@ -240,7 +240,7 @@ def _matrix(t, name: str) -> tuple[int, int, int]:
 
 def _rows_matrix(t, name: str) -> tuple[int, int, int]:
     """The same for rows that may be fp32."""
-    if type(t) is torch.Tensor and t.dtype is torch.float32:
+    if isinstance(t, torch.Tensor) and t.dtype is torch.float32:
         _check_rows(t, name)
         return t.shape[0], t.shape[1], _ld(t)
     return _matrix(t, name)

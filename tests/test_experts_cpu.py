@@ -291,3 +291,19 @@ def test_kernels_wait_before_they_touch_memory(name):
         touches = re.search(r"p\.\w+\s*\[|\*\s*p\.|tma_|\.load\(|row_lo\(|order_key\(|row_of\(|"
                             r"load_weight\(|\.run\(", before)
         assert touches is None, f"{kernel}: {touches and touches.group()!r} before the wait"
+
+
+def test_rows_of_any_tensor_class():
+    """fp32 rows are recognised in a tensor subclass too: what is refused here is the device alone."""
+    order = sg.ExpertOrder(torch.zeros(5, dtype=torch.int32), torch.zeros(8, dtype=torch.int32),
+                           torch.zeros((4, 2), dtype=torch.int32))
+    for dtype in (torch.float32, BF16):
+        rows = torch.nn.Parameter(torch.zeros((8, 16), dtype=dtype))
+        with pytest.raises(ValueError, match="rows must be a CUDA tensor"):
+            experts._rows_matrix(rows, "rows")
+    with pytest.raises(TypeError, match="float64"):
+        experts._rows_matrix(torch.nn.Parameter(torch.zeros((8, 16), dtype=torch.float64)), "rows")
+    with pytest.raises(TypeError, match="list"):
+        experts._rows_matrix([1.0], "rows")
+    with pytest.raises(ValueError, match="CUDA"):
+        sg.expert_combine(torch.nn.Parameter(torch.zeros((8, 16))), order)

@@ -1025,3 +1025,26 @@ def test_captured_calls_see_rewritten_routing_and_weights(T, k, E):
     torch.cuda.synchronize()
     for n, (i, j, v) in enumerate(got):
         assert torch.equal(v, want[i, j]), (n, i, j)
+
+
+# ---------------------------------------------------------------- operands of other classes
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16])
+def test_rows_that_are_parameters(dtype):
+    """Rows held in a tensor subclass give what the plain tensor gives."""
+    T, k, E, D, N = 60, 2, 4, 72, 40
+    x, ids, rw, w, wd = layer_inputs(T, k, E, D, N, 3)
+    order, dy = sg.expert_order(ids, E), randn(T, D, seed=4)
+    rows = randn(T * k, D, seed=5).to(dtype)
+    param = torch.nn.Parameter(rows.clone())
+    assert torch.equal(sg.expert_combine(param, order, rw), sg.expert_combine(rows, order, rw))
+    kept = int(order.offsets[-1])
+    for a, b, n in zip(sg.expert_combine_grad(dy, param, order, rw),
+                       sg.expert_combine_grad(dy, rows, order, rw), (kept, T)):
+        assert torch.equal(a[:n], b[:n])
+    _, saved = sg.experts_swiglu_save(x, ids, rw, w, wd)
+    held = saved._replace(outputs=torch.nn.Parameter(saved.outputs.clone()))
+    for a, b in zip(sg.experts_swiglu_backward(dy, x, rw, w, wd, held),
+                    sg.experts_swiglu_backward(dy, x, rw, w, wd, saved)):
+        assert torch.equal(a, b)
