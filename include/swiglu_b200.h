@@ -562,7 +562,8 @@ int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32,
  *   R = T * k; slots and weights NULL: w = 1.  t stays in fp32; with the weight on this side
  *   w_down's gradient is h_e^T @ dy_e.
  * sgl_grouped_weight_grad: c[e] = a_e^T @ g_e, a[R, M], g[R, N], c[E, M, N]; an empty group's
- *   matrix is zero.  M and N are multiples of 8, the groups' row counts are arbitrary.
+ *   matrix is zero.  M and N are multiples of 8, the groups' row counts are arbitrary.  The
+ *   matrices of c must not overlap: c_stride is at least (M - 1) * ldc + N.
  */
 int sgl_grouped_fused_swiglu(const void* x, const void* w, const void* offsets, void* h, int64_t R,
                              int64_t N, int64_t K, int64_t E, int64_t ldx, int64_t ldw,

@@ -145,9 +145,12 @@ int validate_groups(int64_t R, int64_t E, const void* offsets, bool need_offsets
   return SGL_OK;
 }
 
-int validate_expert_stride(int64_t stride, int64_t rows, int64_t ld, int64_t E, const char* name) {
+// Distance of two experts' matrices of `rows` rows.  Operands may share what lies behind the last row's
+// start; a result's matrices (`cols` columns) may not share an element.
+int validate_expert_stride(int64_t stride, int64_t rows, int64_t ld, int64_t E, const char* name,
+                           int64_t cols = 0) {
   if (E == 1) return SGL_OK;
-  if (stride % 8 != 0 || stride < (rows - 1) * ld)
+  if (stride % 8 != 0 || stride < (rows - 1) * ld + cols)
     return fail(SGL_ERR_BAD_STRIDE,
                 "%s=%lld: an expert's matrix must be a multiple of 8 elements and at least its "
                 "rows apart from the next one's",
@@ -847,7 +850,7 @@ int sgl_grouped_weight_grad(const void* a, const void* g, const void* offsets, v
   if ((rc = validate_shape(R, N, M))) return rc;
   if ((rc = validate_ld(lda, M, "lda")) || (rc = validate_ld(ldg, N, "ldg")) ||
       (rc = validate_ld(ldc, N, "ldc")) ||
-      (rc = validate_expert_stride(c_stride, M, ldc, E, "c_stride")))
+      (rc = validate_expert_stride(c_stride, M, ldc, E, "c_stride", N)))
     return rc;
   ExpertLaunch s;
   s.form = sgl::EXP_WGRAD;

@@ -307,3 +307,11 @@ def test_rows_of_any_tensor_class():
         experts._rows_matrix([1.0], "rows")
     with pytest.raises(ValueError, match="CUDA"):
         sg.expert_combine(torch.nn.Parameter(torch.zeros((8, 16))), order)
+
+
+@pytest.mark.parametrize("M,N,ldc,stride", [(16, 16, 16, 240), (16, 16, 24, 360), (16, 16, 24, 368),
+                                            (8, 64, 72, 504)])
+def test_weight_gradients_that_overlap_are_refused(M, N, ldc, stride):
+    """The last row of one expert's result would be the first of the next one's."""
+    assert stride < (M - 1) * ldc + N
+    call("sgl_grouped_weight_grad", -3, "c_stride", P, P, P, P, 8, M, N, 2, M, N, ldc, stride, None)

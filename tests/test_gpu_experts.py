@@ -1048,3 +1048,19 @@ def test_rows_that_are_parameters(dtype):
     for a, b in zip(sg.experts_swiglu_backward(dy, x, rw, w, wd, held),
                     sg.experts_swiglu_backward(dy, x, rw, w, wd, saved)):
         assert torch.equal(a, b)
+
+
+def test_weight_gradients_close_behind_one_another():
+    """Results whose rows lie between the next expert's: as near as they may come, nothing shared."""
+    counts, M, N, ldc = [40, 0, 21, 130], 16, 72, 160
+    R, E, stride = sum(counts), len(counts), 15 * 160 + 72
+    a, g = randn(R, M, seed=1), randn(R, N, seed=2)
+    want = sg.grouped_weight_grad(a, g, offsets_of(counts))
+    buf = torch.full((E * stride + 64,), 7.0, dtype=BF16, device=DEV)
+    out = buf.as_strided((E, M, N), (stride, ldc, 1))
+    assert torch.equal(sg.grouped_weight_grad(a, g, offsets_of(counts), out=out), want)
+    out.fill_(7.0)
+    assert (buf == 7.0).all()
+    with pytest.raises(ValueError, match="overlap"):
+        sg.grouped_weight_grad(a, g, offsets_of(counts),
+                               out=buf.as_strided((E, M, N), (stride - 8, ldc, 1)))
