@@ -589,7 +589,8 @@ int sgl_grouped_weight_grad(const void* a, const void* g, const void* offsets, v
  * Saved pre-activations of `rows` rows: bytes of the code (or bf16) buffer, its row pitch, and for
  * bits = 8 bytes and pitch of the scale buffer.  A row holds the up half, padded to whole blocks of
  * 32 columns, then the gate half; a scale row the exponents + 127 of the up blocks (an even
- * number of bytes), then of the gate blocks.  Negative sgl_status on bad sizes.
+ * number of bytes), then of the gate blocks.  No rows take no bytes.  Negative sgl_status on bad
+ * sizes.
  */
 int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int64_t* scale_bytes,
                          int64_t* scale_pitch);

@@ -677,6 +677,8 @@ int64_t sgl_preact_bytes(int bits, int64_t rows, int64_t N, int64_t* pitch, int6
                          int64_t* scale_pitch) {
   int rc;
   if ((rc = check_bits(bits))) return rc;
+  if (rows < 0)
+    return fail(SGL_ERR_BAD_SHAPE, "rows=%lld must not be negative", static_cast<long long>(rows));
   if ((rc = validate_shape(rows < 1 ? 1 : rows, N, 8))) return rc;
   const PreactLayout l = preact_layout(bits, N);
   if (pitch) *pitch = l.pitch;

@@ -315,3 +315,16 @@ def test_weight_gradients_that_overlap_are_refused(M, N, ldc, stride):
     """The last row of one expert's result would be the first of the next one's."""
     assert stride < (M - 1) * ldc + N
     call("sgl_grouped_weight_grad", -3, "c_stride", P, P, P, P, 8, M, N, 2, M, N, ldc, stride, None)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_preact_bytes_of_no_rows_and_of_fewer(bits):
+    size = _lib.load().sgl_preact_bytes
+    pitch, scale_bytes, scale_pitch = C.c_int64(-7), C.c_int64(-7), C.c_int64(-7)
+    sizes = [C.byref(v) for v in (pitch, scale_bytes, scale_pitch)]
+    for rows in (-1, -(2 ** 40)):
+        call("sgl_preact_bytes", -2, f"rows={rows}", bits, rows, 40, *sizes)
+    assert (pitch.value, scale_bytes.value, scale_pitch.value) == (-7, -7, -7)
+    assert size(bits, 0, 40, *sizes) == 0
+    assert (pitch.value, scale_bytes.value) == (2 * 64 * bits // 8, 0)
+    assert scale_pitch.value == (4 if bits == 8 else 0)
