@@ -144,11 +144,13 @@ struct ExpertTraits {
 // ---------------------------------------------------------------- 8-bit blocks
 //
 // 32 values v share the scale 2^e, e the smallest integer (>= -127) with max|v| <= 448 * 2^e,
-// 448 being the largest e4m3 value: nothing saturates, and a value keeps a relative error of at
-// most 2^-4 down to 2^-15 of the block's largest.  From the bits of the maximum m * 2^x
-// (1 <= m < 2): e = x - 8, or x - 7 when m > 1.75; adding 0x1fffff to the bits carries into the
-// exponent field exactly then.  The stored byte is e + 127; 255 stands for a block that holds an
-// infinity or a NaN, and every value of it reads as NaN.
+// 448 being the largest e4m3 value: nothing saturates.  A value is off by at most 2^-4 of itself or
+// 2^-10 * 2^e (half a step below e4m3's smallest normal value, 2^-6), whichever is more.  The
+// block's largest lies above 224 * 2^e unless e is held at -127, so the relative bound holds down
+// to 2^-13 of it.  From the bits of the maximum m * 2^x (1 <= m < 2): e = x - 8, or x - 7 when
+// m > 1.75; adding 0x1fffff to the bits carries into the exponent field exactly then.  The stored
+// byte is e + 127; 255 stands for a block that holds an infinity or a NaN, and every value of it
+// reads as NaN.
 __device__ __forceinline__ int block_exponent_code(float amax) {
   const uint32_t bits = __float_as_uint(amax);
   if (bits >= 0x7f800000u) return 255;

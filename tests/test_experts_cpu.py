@@ -328,3 +328,28 @@ def test_preact_bytes_of_no_rows_and_of_fewer(bits):
     assert size(bits, 0, 40, *sizes) == 0
     assert (pitch.value, scale_bytes.value) == (2 * 64 * bits // 8, 0)
     assert scale_pitch.value == (4 if bits == 8 else 0)
+
+
+def test_bounds_of_an_8bit_block():
+    """The plain form keeps 2^-4 of a value down to 2^-13 of its block's largest, 2^-10 of the scale
+    below; 2^-15 of the largest is too far down for the relative bound."""
+    largest = torch.linspace(225, 448, 300)
+    for shift, within in ((0, True), (7, True), (13, True), (15, False)):
+        worst = 0.0
+        for part in torch.linspace(1, 1.99, 31):
+            v = torch.zeros(300, 32)
+            v[:, 0], v[:, 1] = largest, largest * 2.0 ** -shift * part
+            if shift == 0:
+                v[:, 1] = largest / part
+            codes, scales = ref.block_codes(v)
+            assert (scales == 127).all()
+            got = codes.view(torch.float8_e4m3fn).double()[:, 1]
+            off = (got - v[:, 1].double()).abs()
+            worst = max(worst, (off / v[:, 1].double()).max().item())
+            assert (off <= torch.maximum(2.0 ** -4 * v[:, 1].double(), torch.tensor(2.0 ** -10))).all()
+        assert (worst <= 2.0 ** -4) == within, (shift, worst)
+    tiny = torch.full((1, 32), 2.0 ** -133)            # a scale held at 2^-127
+    codes, scales = ref.block_codes(tiny)
+    assert scales.item() == 0
+    value = codes.view(torch.float8_e4m3fn).double()[0, 0] * 2.0 ** -127
+    assert abs(value - 2.0 ** -133) <= 2.0 ** -137
