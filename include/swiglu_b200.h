@@ -518,11 +518,12 @@ int sgl_mgpu_destroy(sgl_mgpu* g);
  *   behind offsets[E] are left as they were.
  * sgl_expert_combine: out[t] = sum_j weights[t, j] * in[rows[t, j]], summed in fp32 in the order
  *   of j.  in: bf16, or fp32 (in_is_f32; its pitch a multiple of 8 elements too).  weights: fp32
- *   or bf16 [T, k], row pitch ld_w, or NULL for ones (which is dispatch's gradient).  Dropped slots add nothing; a token without any gets zeros.
+ *   or bf16 [T, k], row pitch ld_w, or NULL for ones (which is dispatch's gradient).  Dropped
+ *   slots add nothing; a token without any gets zeros.
  * sgl_expert_combine_grad: grad_rows[rows[t, j]] = weights[t, j] * grad_out[t] (other rows are left
  *   as they were; weights NULL: ones) and grad_weights[t, j] = <grad_out[t], in[rows[t, j]]>
- *   (fp32 sums, stored dense [T, k] in fp32 or, weights_bf16, bf16; 0 for dropped slots).  in and grad_weights may both be NULL:
- *   grad_rows alone.  grad_rows may be `in` itself.
+ *   (fp32 sums, stored dense [T, k] in fp32 or, weights_bf16, bf16; 0 for dropped slots).  in and
+ *   grad_weights may both be NULL: grad_rows alone.  grad_rows may be `in` itself.
  * D must be a multiple of 8; the bf16 tensors follow the conventions above.
  */
 int64_t sgl_expert_order_scratch_bytes(int64_t T, int64_t k, int64_t E);
@@ -532,8 +533,8 @@ int sgl_expert_order(const void* ids, int ids_are_int64, int64_t T, int64_t k, i
 int sgl_expert_dispatch(const void* x, const void* rows, void* out, int64_t T, int64_t k, int64_t D,
                         int64_t R, int64_t ldx, int64_t ldo, void* stream);
 int sgl_expert_combine(const void* in, int in_is_f32, const void* rows, const void* weights,
-                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R, int64_t ld_in,
-                       int64_t ld_w, int64_t ldo, void* stream);
+                       int weights_bf16, void* out, int64_t T, int64_t k, int64_t D, int64_t R,
+                       int64_t ld_in, int64_t ld_w, int64_t ldo, void* stream);
 int sgl_expert_combine_grad(const void* grad_out, const void* in, int in_is_f32, const void* rows,
                             const void* weights, int weights_bf16, void* grad_rows,
                             void* grad_weights, int64_t T, int64_t k, int64_t D, int64_t R,
@@ -620,7 +621,8 @@ int sgl_fused_swiglu_backward_saved(const void* x, const void* w, const void* dy
  *   y[t] = sum_j weights[t, j] * (silu(x[t] @ Wg) * (x[t] @ Wu)) @ Wd,  expert ids[t, j]
  * x[T, D], w[E, D, 2N], w_down[E, N, D_out], y[T, D_out].  `workspace`: caller-owned device memory
  * of sgl_experts_swiglu_workspace_bytes bytes, overwritten; calls that overlap on the GPU must not
- * share it.  With few rows per expert the down projection's sum is cut into ranges (a function of
+ * share it.  h is rounded to bf16 between the two products, everything else on the way to y stays
+ * in fp32.  With few rows per expert the down projection's sum is cut into ranges (a function of
  * the sizes alone) that are added in order: against the separate calls only the order of fp32
  * additions differs then.
  */
@@ -637,10 +639,12 @@ int sgl_experts_swiglu(const void* x, const void* ids, int ids_are_int64, const 
  * The layer in training, one call each way.  sgl_experts_swiglu_save: y[T, D_out] (dense) as above
  * (the down projection's sum in one range), and what the backward needs: order, an int32 buffer of
  * E + 1 + 2 * T * k words (offsets, slots, rows as by sgl_expert_order), pre and scales as by
- * sgl_grouped_fused_swiglu_save for T * k rows, and ys [T * k, D_out] fp32, the experts' outputs, which
- * only grad_weights needs.
- * sgl_experts_swiglu_backward: from grad_y[T, D_out] (dense) any of grad_x[T, D], grad_weights[T, k] (in
- * the weights' type), grad_w[E, D, 2N], grad_down[E, N, D_out], all dense; NULL for what is not needed.
+ * sgl_grouped_fused_swiglu_save for T * k rows, and ys [T * k, D_out] fp32, the experts' outputs,
+ * which only grad_weights needs.
+ * sgl_experts_swiglu_backward: from grad_y[T, D_out] (dense) any of grad_x[T, D],
+ * grad_weights[T, k] (in the weights' type), grad_w[E, D, 2N], grad_down[E, N, D_out], all dense;
+ * NULL for what is not needed.  The pre-activations' gradients and h are rounded to bf16 where a
+ * product reads them.
  * `workspace`: caller-owned, of sgl_experts_swiglu_train_workspace_bytes bytes, overwritten.
  */
 int64_t sgl_experts_swiglu_train_workspace_bytes(int64_t T, int64_t k, int64_t E, int64_t D,

@@ -145,8 +145,8 @@ int validate_groups(int64_t R, int64_t E, const void* offsets, bool need_offsets
   return SGL_OK;
 }
 
-// Distance of two experts' matrices of `rows` rows.  Operands may share what lies behind the last row's
-// start; a result's matrices (`cols` columns) may not share an element.
+// Distance of two experts' matrices of `rows` rows.  Operands may share their last row's elements
+// with the next matrix; results (`cols` columns) may not share an element.
 int validate_expert_stride(int64_t stride, int64_t rows, int64_t ld, int64_t E, const char* name,
                            int64_t cols = 0) {
   if (E == 1) return SGL_OK;
@@ -962,11 +962,13 @@ struct ExpertsWorkspace {
 };
 
 // Few rows make few tiles, and the down projection (long sums, narrow results) then leaves SMs
-// idle while others stream long columns of weight.  Its sum is cut into ranges of at least 512
-// whose partial rows the combine step adds up in order: as many as give every SM about four
-// tiles if all groups are used, while the partial rows written and read stay below an eighth of
-// the weight.  A function of the sizes alone.  1 token x 2 of 8 experts, 14336 -> 4096: 59 us
-// in one range, 43 us in eight.
+// idle while others stream long columns of weight.  Its sum is cut into ranges of at least 512 (the
+// last may be shorter, since the others are rounded up to whole blocks of 128) whose partial
+// rows the combine step adds up in order: as many as give every SM about four tiles if all
+// groups are used, while the partial rows written and read stay below an eighth of the weight.  A
+// function of the sizes alone, a B200's 148 SMs assumed: workspaces are sized, and the order of
+// the additions is fixed, without asking a device.  1 token x 2 of 8 experts, 14336 -> 4096: 59 us in
+// one range, 43 us in eight.
 static void down_ranges(int64_t R, int64_t E, int64_t N, int64_t D_out, int* splits,
                         int64_t* per_split) {
   *splits = 1;

@@ -183,7 +183,8 @@ __global__ void __launch_bounds__(kOrderThreads, 1) expert_order_kernel(const Or
 
 // The same, and x's rows sent on in the same launch (sgl_experts_swiglu with few slots): every CTA
 // orders all slots for itself, the first writes the order, and each copies its share of the
-// tokens.  64 tokens x 8 of 64 experts, 2048 x 1024: the layer takes 145 us instead of 151.
+// tokens.  64 tokens x 8 of 64 experts, 2048 x 1024: 6 us less (4 % of the layer) than an order and a
+// dispatch launch, both measured in one session.
 __global__ void __launch_bounds__(kOrderThreads, 1)
 expert_order_dispatch_kernel(const OrderParams p, const __nv_bfloat16* x, __nv_bfloat16* out,
                              int64_t ldx, int64_t ldo, int nvec) {
@@ -402,9 +403,8 @@ __device__ __forceinline__ int row_of(const RowParams& p, int64_t t, int j) {
 
 // kVecs vectors of each of kBatch rows are a thread's loads in flight.  Four in all is what 64
 // registers (four CTAs on an SM; three for fp32 rows) carry: 2 x 2 up to two choices a token, 1 x 4
-// beyond.  16384
-// tokens x 2 choices x 4096 columns: combine 64 us (6.3 TB/s) so and 77 us with 1 x 4; 4096 tokens
-// x 6 choices x 2048: 28 us with 2 x 2 and 23 us with 1 x 4.
+// beyond.  16384 tokens x 2 choices x 4096 columns: combine 64 us (6.3 TB/s) so and 77 us with
+// 1 x 4; 4096 tokens x 6 choices x 2048: 28 us with 2 x 2 and 23 us with 1 x 4.
 
 // out[rows[t, j]] = x[t]: x is read once, each of its rows written once.
 __global__ void __launch_bounds__(256) expert_dispatch_kernel(const RowParams p) {

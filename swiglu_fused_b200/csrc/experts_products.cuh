@@ -14,11 +14,17 @@
 //   EXP_WGRAD    C[e]  = a_e^T @ g_e   (the sum runs over the rows of the group; 0 if it is empty)
 // With offsets == NULL there is one group of all rows (the dense stage's 8-bit checkpoints).
 //
+// h and the pre-activations' gradients are rounded to bf16, the operand type of the product that reads
+// them next (fp32 operands would run at half its rate or less, as tf32); everything before that
+// rounding and every sum is fp32.  Results then carry two roundings: 2.3e-3 to 2.5e-3 of their
+// norm against 64 bits, where the last rounding alone makes 1.7e-3.
+//
 // Structure as the dense kernel's (swiglu_kernel.cuh): persistent CTAs (or CTA pairs on 256-row
-// tiles, tcgen05 cta_group::2), warps 0 and 6 = TMA producers (A, B), warp 1 = MMA issuer, a 256-column fp32 accumulator in two TMEM stages.  The epilogue has eight warps, two for each 32 rows, which
-// share a staging buffer and split its columns: a sum over a few hundred ends before four warps have
-// worked off a tile (the backward of 8000 rows, 1024 -> 512, in 8 bits: 25.9 us with four warps
-// and TMA stores of its three results, 20.5 us so).  What the groups change:
+// tiles, tcgen05 cta_group::2), warps 0 and 6 = TMA producers (A, B), warp 1 = MMA issuer, a
+// 256-column fp32 accumulator in two TMEM stages.  The epilogue has eight warps, two for each 32
+// rows, which share a staging buffer and split its columns: a sum over a few hundred ends before
+// four warps have worked off a tile (the backward of 8000 rows, 1024 -> 512, in 8 bits: 25.9 us
+// with four warps and TMA stores of its three results, 20.5 us so).  What the groups change:
 //   * every CTA turns the offsets into a table of first tile rows once, and finds the expert
 //     of a tile by bisection in it;
 //   * an A tile whose rows run past its group takes them along in the operand (their

@@ -6,8 +6,8 @@
 //
 // HBM bound: a row costs 2N (dy) + 2N + N/16 (codes and scales; 4N for bf16) bytes read and 4N
 // (+ 2N with h) written.  A thread owns kVecs times 8 columns and walks down the rows, two at a
-// time, so that the loads of both are in flight (16384 x 14336 in 8 bits without h: 292 us, 6.5 TB/s; one
-// row of 8 columns at a time took 455 us).
+// time, so that the loads of both are in flight (16384 x 14336 in 8 bits without h: 292 us,
+// 6.5 TB/s; one row of 8 columns at a time took 455 us).
 #pragma once
 
 #include <cstdint>

@@ -730,7 +730,8 @@ def _layer_operands(x, expert_ids, weights, W, W_down):
 def experts_swiglu(x, expert_ids, weights, W, W_down, *, out=None, workspace=None, stream=None):
     """The expert layer at inference, one library call:
     ``y[t] = sum_j weights[t, j] * (silu(x[t] @ W_gate[e]) * (x[t] @ W_up[e])) @ W_down[e]`` with
-    ``e = expert_ids[t, j]``.
+    ``e = expert_ids[t, j]``.  The activation's result is rounded to bf16, the down projection's operand
+    type; everything else on the way to ``y`` stays in fp32.
 
     x          : [T, D] bf16
     expert_ids : [T, k] int32 or int64; a slot outside ``[0, E)`` is dropped
@@ -774,7 +775,8 @@ class SavedExperts(NamedTuple):
 
 def experts_swiglu_save(x, expert_ids, weights, W, W_down, *, checkpoint: str = "bf16", stream=None):
     """The expert layer for training, one library call: ``(y [T, D_out], SavedExperts)``.  Operands as
-    for ``experts_swiglu``; ``checkpoint`` as for ``grouped_fused_swiglu_save``."""
+    for ``experts_swiglu``; ``checkpoint`` as for ``grouped_fused_swiglu_save``.  ``outputs`` takes
+    ``4 * D_out`` bytes a slot beside the checkpoint; drop it if ``weights`` needs no gradient."""
     bits = _checkpoint_bits(checkpoint)
     T, k, E, D, N, D_out, ldx, ld_ids, ldw, dev = _layer_operands(x, expert_ids, weights, W, W_down)
     R = T * k

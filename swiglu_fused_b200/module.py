@@ -151,7 +151,8 @@ class PackedSwiGLUExperts(torch.nn.Module):
     ``weight_down [num_experts, hidden_features, out_features]``.  ``forward(x, expert_ids, weights)``
     takes the router's choices, ``[..., k]`` beside ``x [..., in_features]``; ids outside
     ``[0, num_experts)`` are dropped.  With gradients the pre-activations are kept as
-    ``checkpoint`` says (``"bf16"`` or ``"e4m3"``); without, the layer is one library call."""
+    ``checkpoint`` says (``"bf16"`` or ``"e4m3"``; see ``autograd.fused_swiglu_experts`` for all that is
+    kept); without, the layer is one library call."""
 
     def __init__(self, in_features: int, hidden_features: int, num_experts: int, *,
                  out_features: int | None = None, checkpoint: str = "bf16", device=None,
